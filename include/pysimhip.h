@@ -37,7 +37,7 @@
 extern "C" {
 #endif
 
-#define PSH_VERSION 111
+#define PSH_VERSION 112
 
 #define PSH_MAX_STATE 8   /* largest state vector (QBallBalancer)                 */
 #define PSH_MAX_OBS 8     /* largest observation vector                            */
@@ -474,6 +474,136 @@ float psh_rollout_ms(psh_ctx* ctx, int32_t back);
 /* Diagnostic, no counterpart in the reference: the number of device allocations (hipMalloc) the library has made for
  * this ctx's scratch buffers since psh_create.  psh_rollout grows them on demand; psh_rollout_static never does. */
 int64_t psh_alloc_count(const psh_ctx* ctx);
+
+/* ---- operators of policies on recorded rollouts and in batched step loops ----------------------
+ * What a policy that the rollout kernels do not fuse computes on the device: the layers of a whole population of
+ * networks (ParameterExplorationSampler.sample, Pyrado/pyrado/sampling/parameter_exploration_sampler.py:174-201, and
+ * Policy.evaluate, Pyrado/pyrado/policies/base.py:131-156, for every member on its own rollouts), and the recurrence of
+ * a policy with memory.  Rows are steps; the steps of a rollout, and the rollouts of a policy, are consecutive rows.
+ *
+ * Element types: `dtype` is that of the rows; parameters of the memory operators, carried recurrence states and all sums
+ * are PSH_F64 for PSH_F64 rows and PSH_F32 for the others (called the wide type below).
+ *
+ * `offsets` [dev] int32 [n + 1] cut the rows into n consecutive parts, part i = rows offsets[i] .. offsets[i+1] - 1;
+ * parts may be empty.  offsets[0] is taken as 0, entries are limited to [0, rows], and entries that do not ascend give
+ * meaningless numbers, but no access outside the arrays.  Rows behind offsets[n] belong to no part: row-shaped outputs
+ * are zero there.  Two outputs of a call must not overlap, nor an output and an input.
+ *
+ * These calls keep no state in the context besides the error message: scratch memory is the caller's (`workspace`, of the size the
+ * _workspace function names, at least 256-byte aligned; it may be reused as soon as work issued later on the same stream
+ * needs it), they allocate nothing, record no events, leave the calling thread's current device as it was, and may be
+ * captured into graphs. */
+typedef enum psh_dtype { PSH_F64 = 0, PSH_F32 = 1, PSH_BF16 = 2 } psh_dtype;
+#define PSH_MAX_TAPS 8       /* longest causal convolution                                 */
+#define PSH_MAX_MEM_STATES 64 /* states per channel of the selective recurrence            */
+
+/* y[r, :] = f(W_g x[r, :] + b_g) for the rows r of group g (torch.nn.Linear with one weight per group).  W_g is
+ * [out_dim, in_dim] with unit column stride; row stride ld_w and group stride stride_w, in elements, so that the layers of a population may be
+ * views into its parameter matrix (the population layout of psh_policy.params). */
+typedef struct psh_linear_desc {
+    int32_t dtype;           /* psh_dtype of every array */
+    int32_t nonlin;          /* psh_nonlin of the epilogue */
+    int32_t n_groups;        /* G >= 1 */
+    int32_t rows;            /* R >= 0 */
+    int32_t in_dim, out_dim; /* >= 1 */
+    const int32_t* offsets;  /* [dev] [G + 1] */
+    const void* x;           /* [dev] [R, in_dim], row stride ld_x */
+    const void* weight;      /* [dev] */
+    const void* bias;        /* [dev] [G, out_dim], group stride stride_b, or NULL */
+    void* y;                 /* [dev] [R, out_dim] contiguous; the _grad call reads it (may be NULL there with PSH_NL_NONE) */
+    int64_t ld_x, ld_w, stride_w, stride_b;
+    /* psh_grouped_linear_grad: the loss gradient of y in, those of the inputs out (contiguous; NULL = not wanted) */
+    const void* dy;          /* [dev] [R, out_dim], row stride ld_dy */
+    int64_t ld_dy;
+    void* dx;                /* [dev] [R, in_dim] */
+    void* dweight;           /* [dev] [G, out_dim, in_dim] */
+    void* dbias;             /* [dev] [G, out_dim] */
+    void* workspace;
+    int64_t workspace_bytes;
+    void* stream;
+} psh_linear_desc;
+int psh_grouped_linear(psh_ctx* ctx, const psh_linear_desc* desc);
+int psh_grouped_linear_grad(psh_ctx* ctx, const psh_linear_desc* desc);
+/* bytes of workspace the _grad call needs for these sizes and wanted outputs (pointers are only compared with NULL) */
+int64_t psh_grouped_linear_grad_workspace(const psh_linear_desc* desc);
+
+/* Depthwise causal convolution along every sequence, followed by x sigmoid(x) with silu = 1:
+ *   y[t, d] = f(b[p, d] + sum_k w[p, d, k] x[t - (K-1) + k, d]),  x before a sequence's first row from `state` (zero if NULL)
+ * Sequence s uses the parameters of the policy p whose part of the sequences (`groups`, like offsets; NULL: one policy) it
+ * is in (groups[P] is taken as S).  `last` receives the K-1 newest inputs of every sequence (carried ones among them when it is shorter), what the next call takes as
+ * `state`.  With step = 1 every sequence is exactly one row (rows == n_seqs, offsets unused), and `last` may be `state`
+ * itself (in place). */
+typedef struct psh_conv_desc {
+    int32_t dtype, silu, step;
+    int32_t n_policies;      /* P >= 1 */
+    int32_t n_seqs;          /* S >= 0 */
+    int32_t rows;            /* R >= 0 */
+    int32_t channels;        /* D >= 1 */
+    int32_t taps;            /* K, 1..PSH_MAX_TAPS */
+    const int32_t* offsets;  /* [dev] [S + 1] */
+    const int32_t* groups;   /* [dev] [P + 1] or NULL */
+    const void* x;           /* [dev] [R, D], row stride ld_x */
+    const void* weight;      /* [dev] [P, D, K] contiguous, wide type */
+    const void* bias;        /* [dev] [P, D] contiguous, wide type, or NULL */
+    const void* state;       /* [dev] [S, D, K-1] rows of a sequence contiguous, sequence stride stride_state, or NULL */
+    void* y;                 /* [dev] [R, D] contiguous */
+    void* last;              /* [dev] [S, D, K-1], sequence stride stride_last, or NULL */
+    int64_t ld_x, stride_state, stride_last;
+    /* psh_causal_conv_grad: gradients of y and of `last` in, those of the inputs out (contiguous; NULL = not wanted) */
+    const void* dy; int64_t ld_dy; /* [dev] [R, D] */
+    const void* dlast;       /* [dev] [S, D, K-1] contiguous or NULL */
+    void* dx;                /* [dev] [R, D] */
+    void* dweight;           /* [dev] [P, D, K] wide type */
+    void* dbias;             /* [dev] [P, D] wide type */
+    void* dstate;            /* [dev] [S, D, K-1] */
+    void* workspace;
+    int64_t workspace_bytes;
+    void* stream;
+} psh_conv_desc;
+int psh_causal_conv(psh_ctx* ctx, const psh_conv_desc* desc);
+int psh_causal_conv_grad(psh_ctx* ctx, const psh_conv_desc* desc);
+int64_t psh_causal_conv_grad_workspace(const psh_conv_desc* desc);
+
+/* Selective state-space recurrence along every sequence, for channel d with N states:
+ *   dt = softplus(delta[t, d] + delta_bias[p, d])
+ *   h_t[n] = exp(dt A[p, d, n]) h_{t-1}[n] + dt B[t, n] u[t, d],   h before the first row from `state` (zero if NULL)
+ *   y[t, d] = (sum_n C[t, n] h_t[n] + D[p, d] u[t, d]) * z[t, d] sigmoid(z[t, d])
+ * D, z and delta_bias may be NULL (no such term or factor; a bias of zero).  Policies, `last` and `step` as in psh_conv_desc.
+ * psh_selective_scan with `check` given also stores the states that its _grad call starts from (sized by
+ * psh_selective_scan_check). */
+typedef struct psh_scan_desc {
+    int32_t dtype, step;
+    int32_t n_policies, n_seqs, rows;
+    int32_t channels;        /* D >= 1 */
+    int32_t states;          /* N, 1..PSH_MAX_MEM_STATES */
+    int32_t pad_;
+    const int32_t* offsets;  /* [dev] [S + 1] */
+    const int32_t* groups;   /* [dev] [P + 1] or NULL */
+    const void *u, *delta, *z;          /* [dev] [R, D], row strides ld_u, ld_delta, ld_z */
+    const void *B, *C;                  /* [dev] [R, N], row strides ld_B, ld_C */
+    const void *A, *D, *delta_bias;     /* [dev] [P, D, N], [P, D], [P, D] contiguous, wide type */
+    const void* state;       /* [dev] [S, D, N] wide type, sequence stride stride_state, or NULL */
+    void* y;                 /* [dev] [R, D] contiguous */
+    void* last;              /* [dev] [S, D, N] wide type, sequence stride stride_last, or NULL */
+    int64_t ld_u, ld_delta, ld_z, ld_B, ld_C, stride_state, stride_last;
+    void* check;             /* [dev] states at intervals, written by psh_selective_scan and read by its _grad call */
+    /* psh_selective_scan_grad: gradients of y and of `last` in, those of the inputs out (contiguous; NULL = not wanted) */
+    const void* dy; int64_t ld_dy;
+    const void* dlast;       /* [dev] [S, D, N] contiguous, wide type, or NULL */
+    void *du, *ddelta, *dz;  /* [dev] [R, D] */
+    void *dB, *dC;           /* [dev] [R, N] */
+    void *dA, *dD, *ddelta_bias; /* [dev] [P, D, N], [P, D], [P, D] wide type */
+    void* dstate;            /* [dev] [S, D, N] wide type */
+    void* workspace;
+    int64_t workspace_bytes;
+    void* stream;
+} psh_scan_desc;
+int psh_selective_scan(psh_ctx* ctx, const psh_scan_desc* desc);
+int psh_selective_scan_grad(psh_ctx* ctx, const psh_scan_desc* desc);
+/* bytes of `check`, of the forward call's workspace and of the _grad call's workspace */
+int64_t psh_selective_scan_check(const psh_scan_desc* desc);
+int64_t psh_selective_scan_workspace(const psh_scan_desc* desc);
+int64_t psh_selective_scan_grad_workspace(const psh_scan_desc* desc);
 
 #ifdef __cplusplus
 }

@@ -4,7 +4,7 @@ Field order and types must match the header exactly.
 """
 import ctypes as C
 
-PSH_VERSION = 111
+PSH_VERSION = 112
 PSH_MAX_STATE = 8
 PSH_MAX_OBS = 8
 PSH_MAX_ACT = 2
@@ -16,6 +16,8 @@ PSH_MAX_LIN_FEAT = 512
 PSH_MAX_DISTR = 32
 PSH_MAX_DELAY = 32
 PSH_MAX_WRAP = 6
+PSH_MAX_TAPS = 8
+PSH_MAX_MEM_STATES = 64
 PSH_STATIC_MAX_WEIGHT_DOUBLES = 16384
 PSH_STATIC_MAX_QBB_ENVS = 524288
 
@@ -28,6 +30,7 @@ POL_LINEAR, POL_FNN = 0, 1
 EXPL_NONE, EXPL_NORMAL, EXPL_UNIFORM = 0, 1, 2
 FEAT_IDS = dict(const=0, identity=1, sign=2, abs=3, squared=4, cubed=5, sig=6, bell=7, sin=8, cos=9, sinsin=10,
                 sincos=11, mult=12, rff=13, rbf=14)
+DTYPE_F64, DTYPE_F32, DTYPE_BF16 = range(3)
 NL_IDS = {None: 0, 'none': 0, 'tanh': 1, 'relu': 2, 'sigmoid': 3}
 F_STOP_ON_DONE, F_SIMPLIFIED_DYN, F_MAX_STEPS_INF, F_TRAJ_ENV_MAJOR = 1, 2, 4, 8
 ST_NAN, ST_FAILED, ST_TIMEOUT, ST_BERNOULLI, ST_BAD_INDEX, ST_INTERNAL = 1, 2, 4, 8, 16, 32
@@ -127,6 +130,44 @@ class PshInitDesc(C.Structure):
     ]
 
 
+class PshLinearDesc(C.Structure):
+    _fields_ = [
+        ('dtype', C.c_int32), ('nonlin', C.c_int32), ('n_groups', C.c_int32), ('rows', C.c_int32),
+        ('in_dim', C.c_int32), ('out_dim', C.c_int32), ('offsets', C.c_void_p), ('x', C.c_void_p),
+        ('weight', C.c_void_p), ('bias', C.c_void_p), ('y', C.c_void_p), ('ld_x', C.c_int64), ('ld_w', C.c_int64),
+        ('stride_w', C.c_int64), ('stride_b', C.c_int64), ('dy', C.c_void_p), ('ld_dy', C.c_int64),
+        ('dx', C.c_void_p), ('dweight', C.c_void_p), ('dbias', C.c_void_p), ('workspace', C.c_void_p),
+        ('workspace_bytes', C.c_int64), ('stream', C.c_void_p),
+    ]
+
+
+class PshConvDesc(C.Structure):
+    _fields_ = [
+        ('dtype', C.c_int32), ('silu', C.c_int32), ('step', C.c_int32), ('n_policies', C.c_int32),
+        ('n_seqs', C.c_int32), ('rows', C.c_int32), ('channels', C.c_int32), ('taps', C.c_int32),
+        ('offsets', C.c_void_p), ('groups', C.c_void_p), ('x', C.c_void_p), ('weight', C.c_void_p),
+        ('bias', C.c_void_p), ('state', C.c_void_p), ('y', C.c_void_p), ('last', C.c_void_p), ('ld_x', C.c_int64),
+        ('stride_state', C.c_int64), ('stride_last', C.c_int64), ('dy', C.c_void_p), ('ld_dy', C.c_int64),
+        ('dlast', C.c_void_p), ('dx', C.c_void_p), ('dweight', C.c_void_p), ('dbias', C.c_void_p),
+        ('dstate', C.c_void_p), ('workspace', C.c_void_p), ('workspace_bytes', C.c_int64), ('stream', C.c_void_p),
+    ]
+
+
+class PshScanDesc(C.Structure):
+    _fields_ = [
+        ('dtype', C.c_int32), ('step', C.c_int32), ('n_policies', C.c_int32), ('n_seqs', C.c_int32),
+        ('rows', C.c_int32), ('channels', C.c_int32), ('states', C.c_int32), ('pad_', C.c_int32),
+        ('offsets', C.c_void_p), ('groups', C.c_void_p), ('u', C.c_void_p), ('delta', C.c_void_p), ('z', C.c_void_p),
+        ('B', C.c_void_p), ('C', C.c_void_p), ('A', C.c_void_p), ('D', C.c_void_p), ('delta_bias', C.c_void_p),
+        ('state', C.c_void_p), ('y', C.c_void_p), ('last', C.c_void_p), ('ld_u', C.c_int64), ('ld_delta', C.c_int64),
+        ('ld_z', C.c_int64), ('ld_B', C.c_int64), ('ld_C', C.c_int64), ('stride_state', C.c_int64),
+        ('stride_last', C.c_int64), ('check', C.c_void_p), ('dy', C.c_void_p), ('ld_dy', C.c_int64),
+        ('dlast', C.c_void_p), ('du', C.c_void_p), ('ddelta', C.c_void_p), ('dz', C.c_void_p), ('dB', C.c_void_p),
+        ('dC', C.c_void_p), ('dA', C.c_void_p), ('dD', C.c_void_p), ('ddelta_bias', C.c_void_p),
+        ('dstate', C.c_void_p), ('workspace', C.c_void_p), ('workspace_bytes', C.c_int64), ('stream', C.c_void_p),
+    ]
+
+
 # every symbol include/pysimhip.h declares: name -> (restype, argtypes)
 PSH_SYMBOLS = {
     'psh_version': (C.c_int, []),
@@ -148,4 +189,15 @@ PSH_SYMBOLS = {
     'psh_rollout_ms': (C.c_float, [C.c_void_p, C.c_int32]),
     'psh_alloc_count': (C.c_int64, [C.c_void_p]),
     'psh_eval_math': (C.c_int, [C.c_void_p, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
+    'psh_grouped_linear': (C.c_int, [C.c_void_p, C.POINTER(PshLinearDesc)]),
+    'psh_grouped_linear_grad': (C.c_int, [C.c_void_p, C.POINTER(PshLinearDesc)]),
+    'psh_causal_conv': (C.c_int, [C.c_void_p, C.POINTER(PshConvDesc)]),
+    'psh_causal_conv_grad': (C.c_int, [C.c_void_p, C.POINTER(PshConvDesc)]),
+    'psh_selective_scan': (C.c_int, [C.c_void_p, C.POINTER(PshScanDesc)]),
+    'psh_selective_scan_grad': (C.c_int, [C.c_void_p, C.POINTER(PshScanDesc)]),
+    'psh_grouped_linear_grad_workspace': (C.c_int64, [C.POINTER(PshLinearDesc)]),
+    'psh_causal_conv_grad_workspace': (C.c_int64, [C.POINTER(PshConvDesc)]),
+    'psh_selective_scan_check': (C.c_int64, [C.POINTER(PshScanDesc)]),
+    'psh_selective_scan_workspace': (C.c_int64, [C.POINTER(PshScanDesc)]),
+    'psh_selective_scan_grad_workspace': (C.c_int64, [C.POINTER(PshScanDesc)]),
 }

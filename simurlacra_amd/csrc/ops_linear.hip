@@ -1,0 +1,529 @@
+// Layers of a population of networks: y[r] = f(W_g x[r] + b_g) for the rows r of group g, with ragged groups, and its
+// gradients (psh_grouped_linear, psh_grouped_linear_grad of include/pysimhip.h).
+//
+// One tiled matrix product serves the three of them, D[i, j] = sum_c P[i, c] Q[j, c] per group:
+//   forward  i = output unit,  j = row,          c = input unit     P = W_g          Q = x
+//   dx       i = input unit,   j = row,          c = output unit    P = W_g^T        Q = dp
+//   dW       i = output unit,  j = input unit,   c = row            P = dp^T         Q = x^T
+// with dp = dy f'(y).  Rows are the SECOND index of the matrix instruction: its result then holds four consecutive
+// units of one row per lane, which is what a row-major store wants.
+//
+// In LDS both operands lie as [index][128 bytes of c], whichever way they are laid out in memory; a lane's fragment is 16
+// bytes along c, so 8 bf16 are one operand of v_mfma_f32_16x16x32_bf16, 4 floats those of four v_mfma_f32_16x16x4_f32 and 2
+// doubles those of two v_mfma_f64_16x16x4_f64 (c is summed over, so which c meets in which instruction is free as long as
+// P and Q agree).  The 16-byte units of an index are permuted by XOR with (index ^ index / 8) & 7: 8 neighbouring
+// indices (fragment reads) and 8 indices 8 apart (transposing writes) lie in different banks.
+#include <hip/hip_runtime.h>
+
+#include "psh_ops.h"
+
+namespace {
+
+template <class T> struct Mfma;
+template <> struct Mfma<bf16_t> {
+    typedef v4f acc;
+    static constexpr int row(int q, int r) { return 4 * q + r; }   // index i of accumulator register r in lane group q
+    static PSH_OP void step(const v4u& p, const v4u& q, acc& d) {
+        d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, p), __builtin_bit_cast(v8bf, q), d, 0, 0, 0);
+    }
+};
+template <> struct Mfma<float> {
+    typedef v4f acc;
+    static constexpr int row(int q, int r) { return 4 * q + r; }
+    static PSH_OP void step(const v4u& p, const v4u& q, acc& d) {
+        const v4f a = __builtin_bit_cast(v4f, p), b = __builtin_bit_cast(v4f, q);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) d = __builtin_amdgcn_mfma_f32_16x16x4f32(a[k], b[k], d, 0, 0, 0);
+    }
+};
+template <> struct Mfma<double> {
+    typedef v4d acc;
+    static constexpr int row(int q, int r) { return 4 * r + q; }
+    static PSH_OP void step(const v4u& p, const v4u& q, acc& d) {
+        typedef double v2d __attribute__((ext_vector_type(2)));
+        const v2d a = __builtin_bit_cast(v2d, p), b = __builtin_bit_cast(v2d, q);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) d = __builtin_amdgcn_mfma_f64_16x16x4f64(a[k], b[k], d, 0, 0, 0);
+    }
+};
+
+// an operand: element (index i, c) at p[i * ld + c], or at p[c * ld + i] if it is read transposed
+template <class T> struct Operand {
+    const T* p;
+    long ld;
+    int n, nc;      // valid indices and valid c
+    bool wide;      // 16-byte loads are aligned
+};
+
+template <class T> PSH_OP int unit_of(int i, int u) { return u ^ ((i ^ (i >> 3)) & 7); }
+
+// One thread's part of a tile of N indices x 8 units of 16 bytes: loaded into registers while the previous tile is being
+// multiplied, stored to LDS afterwards.
+template <class T, int N, int THREADS, bool TR> struct Stager {
+    static constexpr int V = 16 / (int)sizeof(T);
+    static constexpr int WORK = TR ? (N / V) * 8 : N * 8;                 // V x V blocks, or units
+    static constexpr int PER = (WORK + THREADS - 1) / THREADS;
+    static constexpr int REGS = TR ? PER * V : PER;
+    v4u r[REGS];
+
+    static PSH_OP v4u load(const Operand<T>& o, const T* q, int first, int limit) {
+        // elements [first, first + V) of a line with `limit` valid ones
+        if (first >= limit) return v4u{0, 0, 0, 0};
+        if (o.wide && first + V <= limit) return *reinterpret_cast<const v4u*>(q + first);
+        T e[V];
+#pragma unroll
+        for (int k = 0; k < V; ++k) e[k] = first + k < limit ? q[first + k] : T(0);
+        return __builtin_bit_cast(v4u, e);
+    }
+    PSH_OP void fetch(const Operand<T>& o, int c0) {
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            const int id = (int)threadIdx.x + k * THREADS;
+            if constexpr (!TR) {
+                const int i = id >> 3, u = id & 7;
+                r[k] = i < o.n && id < WORK ? load(o, o.p + i * o.ld, c0 + u * V, o.nc) : v4u{0, 0, 0, 0};
+            } else {
+                const int ib = id % (N / V), u = id / (N / V);
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const int c = c0 + u * V + j;
+                    r[k * V + j] = c < o.nc && id < WORK ? load(o, o.p + (long)c * o.ld, ib * V, o.n) : v4u{0, 0, 0, 0};
+                }
+            }
+        }
+    }
+    PSH_OP void store(unsigned char* lds) const {
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            const int id = (int)threadIdx.x + k * THREADS;
+            if (id >= WORK) continue;
+            if constexpr (!TR) {
+                const int i = id >> 3, u = id & 7;
+                *reinterpret_cast<v4u*>(lds + i * 128 + unit_of<T>(i, u) * 16) = r[k];
+            } else {
+                const int ib = id % (N / V), u = id / (N / V);
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    T e[V];
+#pragma unroll
+                    for (int m = 0; m < V; ++m) {
+                        T line[V];
+                        __builtin_memcpy(line, &r[k * V + m], 16);
+                        e[m] = line[j];
+                    }
+                    const int i = ib * V + j;
+                    *reinterpret_cast<v4u*>(lds + i * 128 + unit_of<T>(i, u) * 16) = __builtin_bit_cast(v4u, e);
+                }
+            }
+        }
+    }
+};
+
+template <class T, int BI, int BJ, int WI, int WJ> struct Tile {
+    static constexpr int THREADS = 64 * WI * WJ, MI = BI / WI / 16, MJ = BJ / WJ / 16;
+    typedef typename Mfma<T>::acc acc_t;
+    acc_t acc[MI][MJ];
+    acc_t ones[MI];   // sums of P over c, in every column (the bias gradient), if asked for
+
+    // D += P Q^T over all c.  LDS: two buffers of (BI + BJ) * 128 bytes.
+    template <bool TP, bool TQ, bool SUMS> PSH_OP void multiply(const Operand<T>& p, const Operand<T>& q, unsigned char* lds) {
+        constexpr int KC = 128 / (int)sizeof(T);
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        const int wi = (wave % WI) * (BI / WI), wj = (wave / WI) * (BJ / WJ);
+        const int l = lane & 15, g = lane >> 4;
+#pragma unroll
+        for (int a = 0; a < MI; ++a) {
+            ones[a] = acc_t{0, 0, 0, 0};
+#pragma unroll
+            for (int b = 0; b < MJ; ++b) acc[a][b] = acc_t{0, 0, 0, 0};
+        }
+        v4u unit;
+        if constexpr (SUMS) {
+            T e[16 / sizeof(T)];
+#pragma unroll
+            for (int k = 0; k < (int)(16 / sizeof(T)); ++k) e[k] = to_elem<T>(1);
+            unit = __builtin_bit_cast(v4u, e);
+        }
+        Stager<T, BI, THREADS, TP> sp;
+        Stager<T, BJ, THREADS, TQ> sq;
+        const int nc = p.nc, tiles = (nc + KC - 1) / KC;
+        if (tiles <= 0) return;
+        sp.fetch(p, 0);
+        sq.fetch(q, 0);
+        sp.store(lds);
+        sq.store(lds + BI * 128);
+        __syncthreads();
+        for (int t = 0; t < tiles; ++t) {
+            unsigned char* const cur = lds + (t & 1) * (BI + BJ) * 128;
+            unsigned char* const nxt = lds + (~t & 1) * (BI + BJ) * 128;
+            if (t + 1 < tiles) {
+                sp.fetch(p, (t + 1) * KC);
+                sq.fetch(q, (t + 1) * KC);
+            }
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                v4u fp[MI], fq[MJ];
+#pragma unroll
+                for (int a = 0; a < MI; ++a) {
+                    const int i = wi + a * 16 + l;
+                    fp[a] = *reinterpret_cast<const v4u*>(cur + i * 128 + unit_of<T>(i, s * 4 + g) * 16);
+                }
+#pragma unroll
+                for (int b = 0; b < MJ; ++b) {
+                    const int j = wj + b * 16 + l;
+                    fq[b] = *reinterpret_cast<const v4u*>(cur + BI * 128 + j * 128 + unit_of<T>(j, s * 4 + g) * 16);
+                }
+#pragma unroll
+                for (int a = 0; a < MI; ++a) {
+#pragma unroll
+                    for (int b = 0; b < MJ; ++b) Mfma<T>::step(fp[a], fq[b], acc[a][b]);
+                    if constexpr (SUMS) Mfma<T>::step(fp[a], unit, ones[a]);
+                }
+            }
+            if (t + 1 < tiles) {
+                sp.store(nxt);
+                sq.store(nxt + BI * 128);
+            }
+            __syncthreads();
+        }
+    }
+
+    // f(i, j, v[4]) for the results of this lane: units i .. i + 3 of row j for fp32 accumulators; for fp64 ones the
+    // four units are i, i + 4, i + 8, i + 12
+    template <class F> PSH_OP void each(F f) {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        const int wi = (wave % WI) * (BI / WI), wj = (wave / WI) * (BJ / WJ);
+#pragma unroll
+        for (int a = 0; a < MI; ++a)
+#pragma unroll
+            for (int b = 0; b < MJ; ++b)
+                f(wi + a * 16 + Mfma<T>::row(lane >> 4, 0), wj + b * 16 + (lane & 15), acc[a][b]);
+    }
+};
+
+// consecutive tiles on one XCD: workgroups go to the 8 XCDs in turn, each of which has an L2 of its own
+PSH_OP long xcd_order(long b, long total) {
+    const long per = (total + 7) / 8;
+    return (b & 7) * per + (b >> 3);
+}
+
+template <class T> struct RowsArgs {   // forward and dx
+    Parts parts;
+    const T* rows_in; long ld_in;      // x, or dp
+    const T* weight; long ld_w, stride_w;
+    const T* bias; long stride_b;
+    T* out;                            // [rows, n_out] contiguous
+    int n_in, n_out, nonlin;
+    long slots, tiles_i;
+    bool wide_in, wide_w, wide_out;
+};
+
+// store up to four units of one row
+template <class T, class A> PSH_OP void store_units(T* row, int i, int n, const A& v, bool wide) {
+    if constexpr (sizeof(T) == 8) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (i + 4 * r < n) row[i + 4 * r] = v[r];
+    } else if (wide && i + 4 <= n) {
+        T e[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) e[r] = to_elem<T>(v[r]);
+        if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(row + i) = __builtin_bit_cast(uint2, e);
+        else *reinterpret_cast<v4u*>(row + i) = __builtin_bit_cast(v4u, e);
+    } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (i + r < n) row[i + r] = to_elem<T>(v[r]);
+    }
+}
+
+template <class T, int BI, int BJ, int WI, int WJ, bool TW>
+__global__ __launch_bounds__(64 * WI * WJ) void k_rows(const RowsArgs<T> a) {
+    extern __shared__ __align__(16) unsigned char lds[];
+    const long id = xcd_order(blockIdx.x, a.slots * a.tiles_i);
+    if (id >= a.slots * a.tiles_i) return;
+    const Piece q = find_piece(a.parts, (int)(id / a.tiles_i));
+    const int i0 = (int)(id % a.tiles_i) * BI;
+    const int nj = q.end - q.begin, ni = min(BI, a.n_out - i0);
+    if (nj <= 0) return;
+    if (q.part >= a.parts.n) {   // rows behind the last group
+        for (int k = threadIdx.x; k < nj * ni; k += blockDim.x) a.out[(long)(q.begin + k / ni) * a.n_out + i0 + k % ni] = T(0);
+        return;
+    }
+    const T* const w = a.weight + (long)q.part * a.stride_w;
+    const Operand<T> p{TW ? w + i0 : w + (long)i0 * a.ld_w, a.ld_w, ni, a.n_in, a.wide_w};
+    const Operand<T> x{a.rows_in + (long)q.begin * a.ld_in, a.ld_in, nj, a.n_in, a.wide_in};
+    Tile<T, BI, BJ, WI, WJ> tile;
+    tile.template multiply<TW, false, false>(p, x, lds);
+    typedef typename Wide<T>::type W;
+    const T* const b = a.bias ? a.bias + (long)q.part * a.stride_b + i0 : nullptr;
+    tile.each([&](int i, int j, auto v) {
+        if (j >= nj) return;
+        constexpr int step = sizeof(T) == 8 ? 4 : 1;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            W s = v[r];
+            if (b && i + step * r < ni) s += to_wide(b[i + step * r]);
+            v[r] = nonlin_w(a.nonlin, s);
+        }
+        store_units(a.out + (long)(q.begin + j) * a.n_out + i0, i, ni, v, a.wide_out);
+    });
+}
+
+// dp = dy f'(y), rounded to the element type as the gradient that reaches a layer's product in any composition of
+// layers is.  Rows behind the last group have no part in any sum.
+template <class T> __global__ __launch_bounds__(256) void k_preact(long n, int cols, const T* dy, long ld, const T* y, int nonlin, T* dp) {
+    for (long k = (long)blockIdx.x * 256 + threadIdx.x; k < n; k += (long)gridDim.x * 256) {
+        const long r = k / cols;
+        dp[k] = to_elem<T>(to_wide(dy[r * ld + (k - r * cols)]) * nonlin_slope_w(nonlin, to_wide(y[k])));
+    }
+}
+
+template <class T> struct GradArgs {   // dW, db
+    Parts parts;                       // pieces of the contraction
+    const T* dp; long ld_dp;
+    const T* x; long ld_x;
+    T* dw; T* db;                      // [G, n, k], [G, n]
+    typename Wide<T>::type* part_w;    // [slots, n, k] and [slots, n]: sums of groups that are cut into several pieces
+    typename Wide<T>::type* part_b;
+    int n, k;
+    long slots, tiles_i, tiles_j;
+    bool wide_dp, wide_x, wide_out;
+};
+
+template <class T, int BI, int BJ, int WI, int WJ>
+__global__ __launch_bounds__(64 * WI * WJ) void k_weights(const GradArgs<T> a) {
+    extern __shared__ __align__(16) unsigned char lds[];
+    const long tiles = a.tiles_i * a.tiles_j, total = a.slots * tiles;
+    const long id = xcd_order(blockIdx.x, total);
+    if (id >= total) return;
+    const int slot = (int)(id / tiles);
+    const Piece q = find_piece(a.parts, slot);
+    if (q.part >= a.parts.n || (q.j > 0 && q.begin >= q.end)) return;
+    const int i0 = (int)(id % tiles / a.tiles_j) * BI, j0 = (int)(id % a.tiles_j) * BJ;
+    const int ni = min(BI, a.n - i0), nj = min(BJ, a.k - j0), rows = max(0, q.end - q.begin);
+    const Operand<T> p{a.dp + (long)q.begin * a.ld_dp + i0, a.ld_dp, ni, rows, a.wide_dp};
+    const Operand<T> x{a.x + (long)q.begin * a.ld_x + j0, a.ld_x, nj, rows, a.wide_x};
+    Tile<T, BI, BJ, WI, WJ> tile;
+    const bool whole = q.part_end - q.part_begin <= a.parts.L;   // no other piece: the result itself
+    const bool sums = j0 == 0 && a.db;
+    if (sums) tile.template multiply<true, true, true>(p, x, lds);
+    else tile.template multiply<true, true, false>(p, x, lds);
+    constexpr int step = sizeof(T) == 8 ? 4 : 1;
+    const long at = (long)(whole ? q.part : slot) * a.n;
+    if (a.dw) tile.each([&](int i, int j, auto v) {
+        if (j >= nj) return;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            if (i + step * r >= ni) continue;
+            const long o = (at + i0 + i + step * r) * a.k + j0 + j;
+            if (whole) a.dw[o] = to_elem<T>(v[r]);
+            else a.part_w[o] = v[r];
+        }
+    });
+    if (sums && (threadIdx.x & 15) == 0 && (threadIdx.x >> 6) / WI == 0) {
+        const int wi = ((threadIdx.x >> 6) % WI) * (BI / WI);
+#pragma unroll
+        for (int m = 0; m < BI / WI / 16; ++m)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int i = wi + m * 16 + Mfma<T>::row((threadIdx.x & 63) >> 4, r);
+                if (i >= ni) continue;
+                if (whole) a.db[at + i0 + i] = to_elem<T>(tile.ones[m][r]);
+                else a.part_b[at + i0 + i] = tile.ones[m][r];
+            }
+    }
+}
+
+// sums of the pieces of the groups that have several, in the order of the rows
+template <class T> __global__ __launch_bounds__(256) void k_join(const GradArgs<T> a) {
+    const long nw = a.dw ? (long)a.n * a.k : 0, nb = a.db ? a.n : 0;
+    for (int g = blockIdx.y; g < a.parts.n; g += gridDim.y) {
+        const int begin = a.parts.at(g), end = a.parts.at(g + 1);
+        if (end - begin <= a.parts.L) continue;
+        const int pieces = (int)(((long)end - begin + a.parts.L - 1) / a.parts.L), first = a.parts.first_slot(g);
+        for (long e = (long)blockIdx.x * 256 + threadIdx.x; e < nw + nb; e += (long)gridDim.x * 256) {
+            const bool w = e < nw;
+            const typename Wide<T>::type* const src = w ? a.part_w + (long)first * nw + e : a.part_b + (long)first * nb + (e - nw);
+            const long stride = w ? nw : nb;
+            typename Wide<T>::type s = 0;
+            for (int j = 0; j < pieces; ++j) s += src[j * stride];
+            if (w) a.dw[(long)g * nw + e] = to_elem<T>(s);
+            else a.db[(long)g * nb + e - nw] = to_elem<T>(s);
+        }
+    }
+}
+
+inline bool wide_ok(const void* p, int size, int64_t ld, int64_t stride = 0) {
+    return ((uintptr_t)p & 15) == 0 && (ld * size) % 16 == 0 && (stride * size) % 16 == 0;
+}
+
+template <class K> int allow_lds(psh_ctx* c, K kernel, int bytes) {
+    if (bytes > 64 * 1024) PSH_HIP(c, hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    return PSH_OK;
+}
+
+template <class T, int BI, int BJ, int WI, int WJ, bool TW> int launch_rows(psh_ctx* c, RowsArgs<T>& a, int rows, hipStream_t st) {
+    a.parts.L = BJ;
+    a.slots = parts_slots(rows, a.parts.n, BJ);
+    a.tiles_i = (a.n_out + BI - 1) / BI;
+    const long total = (a.slots * a.tiles_i + 7) / 8 * 8;
+    if (total > 0x7fffffffL) { set_err(c, "grouped_linear: too many tiles for one launch"); return PSH_ERR_UNSUPPORTED; }
+    constexpr int lds = 2 * (BI + BJ) * 128;
+    const auto kernel = k_rows<T, BI, BJ, WI, WJ, TW>;
+    const int rc = allow_lds(c, kernel, lds);
+    if (rc != PSH_OK) return rc;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)total), dim3(64 * WI * WJ), lds, st, a);
+    PSH_HIP(c, hipGetLastError());
+    return PSH_OK;
+}
+
+template <class T, bool TW> int run_rows(psh_ctx* c, RowsArgs<T>& a, int rows, hipStream_t st) {
+    return launch_rows<T, 64, 64, 2, 2, TW>(c, a, rows, st);
+}
+
+// rows of one piece of the weight gradient's contraction
+int64_t grad_piece(const psh_linear_desc* d) {
+    const int64_t tiles = (int64_t)((d->out_dim + 63) / 64) * ((d->in_dim + 63) / 64);
+    const int64_t whole = ((int64_t)d->rows + 64) / 64 * 64;
+    if (tiles >= 512) return whole;
+    int64_t L = ((int64_t)d->rows * tiles / 1024 + 63) / 64 * 64;
+    if (L < 256) L = 256;
+    return L < whole ? L : whole;
+}
+
+struct GradSpace { int64_t dp, part_w, part_b, total; };
+GradSpace grad_space(const psh_linear_desc* d) {
+    GradSpace s{};
+    const int64_t slots = parts_slots(d->rows, d->n_groups, grad_piece(d));
+    if (d->nonlin != PSH_NL_NONE) s.dp = align256((int64_t)d->rows * d->out_dim * elem_size(d->dtype));
+    if (d->dweight) s.part_w = align256(slots * d->out_dim * d->in_dim * wide_size(d->dtype));
+    if (d->dbias) s.part_b = align256(slots * d->out_dim * wide_size(d->dtype));
+    if (d->rows <= grad_piece(d)) s.part_w = s.part_b = 0;   // no group has a second piece
+    s.total = s.dp + s.part_w + s.part_b;
+    return s;
+}
+
+int check(psh_ctx* c, const psh_linear_desc* d, bool grad) {
+    if (!c || !d) return PSH_ERR_ARG;
+    if (d->dtype < PSH_F64 || d->dtype > PSH_BF16 || d->nonlin < PSH_NL_NONE || d->nonlin > PSH_NL_SIGMOID) {
+        set_err(c, "grouped_linear: unknown dtype or nonlinearity");
+        return PSH_ERR_ARG;
+    }
+    if (d->n_groups < 1 || d->rows < 0 || d->in_dim < 1 || d->out_dim < 1) { set_err(c, "grouped_linear: invalid sizes"); return PSH_ERR_ARG; }
+    if (d->n_groups > (1 << 30) || d->rows > (1 << 30)) { set_err(c, "grouped_linear: at most 2^30 rows and groups"); return PSH_ERR_UNSUPPORTED; }
+    if (!d->offsets || (d->rows > 0 && !d->x) || !d->weight || d->ld_x < d->in_dim || d->ld_w < d->in_dim || d->stride_w < 0 || d->stride_b < 0) {
+        set_err(c, "grouped_linear: NULL array or a row stride below the row's length");
+        return PSH_ERR_ARG;
+    }
+    if (!grad) {
+        if (d->rows > 0 && !d->y) { set_err(c, "grouped_linear: y is NULL"); return PSH_ERR_ARG; }
+        return PSH_OK;
+    }
+    if (d->rows > 0 && (!d->dy || d->ld_dy < d->out_dim || (d->nonlin != PSH_NL_NONE && !d->y))) {
+        set_err(c, "grouped_linear_grad: dy (and y, with a nonlinearity) must be given");
+        return PSH_ERR_ARG;
+    }
+    const GradSpace s = grad_space(d);
+    if (s.total > 0 && (!d->workspace || d->workspace_bytes < s.total || ((uintptr_t)d->workspace & 255))) {
+        set_err(c, "grouped_linear_grad: the workspace is too small or not 256-byte aligned");
+        return PSH_ERR_ARG;
+    }
+    return PSH_OK;
+}
+
+template <class T> int forward(psh_ctx* c, const psh_linear_desc* d) {
+    RowsArgs<T> a{};
+    a.parts = Parts{d->offsets, d->n_groups, d->rows, 0};
+    a.rows_in = (const T*)d->x; a.ld_in = d->ld_x;
+    a.weight = (const T*)d->weight; a.ld_w = d->ld_w; a.stride_w = d->stride_w;
+    a.bias = (const T*)d->bias; a.stride_b = d->stride_b;
+    a.out = (T*)d->y;
+    a.n_in = d->in_dim; a.n_out = d->out_dim; a.nonlin = d->nonlin;
+    a.wide_in = wide_ok(d->x, sizeof(T), d->ld_x);
+    a.wide_w = wide_ok(d->weight, sizeof(T), d->ld_w, d->stride_w);
+    a.wide_out = wide_ok(d->y, sizeof(T), 4) && d->out_dim % 4 == 0;
+    return run_rows<T, false>(c, a, d->rows, (hipStream_t)d->stream);
+}
+
+template <class T> int backward(psh_ctx* c, const psh_linear_desc* d) {
+    typedef typename Wide<T>::type W;
+    hipStream_t st = (hipStream_t)d->stream;
+    const GradSpace s = grad_space(d);
+    unsigned char* const space = (unsigned char*)d->workspace;
+    const T* dp = (const T*)d->dy;
+    long ld_dp = d->ld_dy;
+    if (d->nonlin != PSH_NL_NONE && d->rows > 0) {
+        const long n = (long)d->rows * d->out_dim;
+        const long blocks = (n + 1023) / 1024;
+        hipLaunchKernelGGL(k_preact<T>, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, n, (int)d->out_dim, dp, ld_dp,
+                           (const T*)d->y, (int)d->nonlin, (T*)space);
+        PSH_HIP(c, hipGetLastError());
+        dp = (const T*)space;
+        ld_dp = d->out_dim;
+    }
+    if (d->dx && d->rows > 0) {
+        RowsArgs<T> a{};
+        a.parts = Parts{d->offsets, d->n_groups, d->rows, 0};
+        a.rows_in = dp; a.ld_in = ld_dp;
+        a.weight = (const T*)d->weight; a.ld_w = d->ld_w; a.stride_w = d->stride_w;
+        a.out = (T*)d->dx;
+        a.n_in = d->out_dim; a.n_out = d->in_dim; a.nonlin = PSH_NL_NONE;
+        a.wide_in = wide_ok(dp, sizeof(T), ld_dp);
+        a.wide_w = wide_ok(d->weight, sizeof(T), d->ld_w, d->stride_w);
+        a.wide_out = wide_ok(d->dx, sizeof(T), 4) && d->in_dim % 4 == 0;
+        const int rc = run_rows<T, true>(c, a, d->rows, st);
+        if (rc != PSH_OK) return rc;
+    }
+    if (d->dweight || d->dbias) {
+        GradArgs<T> a{};
+        a.parts = Parts{d->offsets, d->n_groups, d->rows, (int)grad_piece(d)};
+        a.dp = dp; a.ld_dp = ld_dp;
+        a.x = (const T*)d->x; a.ld_x = d->ld_x;
+        a.dw = (T*)d->dweight; a.db = (T*)d->dbias;
+        a.part_w = (W*)(space + s.dp); a.part_b = (W*)(space + s.dp + s.part_w);
+        a.n = d->out_dim; a.k = d->in_dim;
+        a.wide_dp = wide_ok(dp, sizeof(T), ld_dp);
+        a.wide_x = wide_ok(d->x, sizeof(T), d->ld_x);
+        a.slots = parts_slots(d->rows, d->n_groups, a.parts.L);
+        a.tiles_i = (a.n + 63) / 64;
+        a.tiles_j = d->dweight ? (a.k + 63) / 64 : 1;
+        const long total = (a.slots * a.tiles_i * a.tiles_j + 7) / 8 * 8;
+        if (total > 0x7fffffffL) { set_err(c, "grouped_linear_grad: too many tiles for one launch"); return PSH_ERR_UNSUPPORTED; }
+        hipLaunchKernelGGL((k_weights<T, 64, 64, 2, 2>), dim3((unsigned)total), dim3(256), 2 * 128 * 128, st, a);
+        PSH_HIP(c, hipGetLastError());
+        if (s.part_w + s.part_b > 0) {
+            const long n = (long)a.n * (a.k + 1);
+            const unsigned bx = (unsigned)((n + 255) / 256 < 1024 ? (n + 255) / 256 : 1024);
+            const unsigned gy = (unsigned)(d->n_groups < 65535 ? d->n_groups : 65535);
+            hipLaunchKernelGGL(k_join<T>, dim3(bx, gy), dim3(256), 0, st, a);
+            PSH_HIP(c, hipGetLastError());
+        }
+    }
+    return PSH_OK;
+}
+
+}  // namespace
+
+extern "C" int64_t psh_grouped_linear_grad_workspace(const psh_linear_desc* d) {
+    if (!d || d->n_groups < 1 || d->rows < 0 || d->in_dim < 1 || d->out_dim < 1) return PSH_ERR_ARG;
+    return grad_space(d).total;
+}
+
+extern "C" int psh_grouped_linear(psh_ctx* c, const psh_linear_desc* d) {
+    const int rc = check(c, d, false);
+    if (rc != PSH_OK || d->rows == 0) return rc;
+    PSH_ON_DEVICE(c);
+    if (d->dtype == PSH_F64) return forward<double>(c, d);
+    if (d->dtype == PSH_F32) return forward<float>(c, d);
+    return forward<bf16_t>(c, d);
+}
+
+extern "C" int psh_grouped_linear_grad(psh_ctx* c, const psh_linear_desc* d) {
+    const int rc = check(c, d, true);
+    if (rc != PSH_OK) return rc;
+    PSH_ON_DEVICE(c);
+    if (d->dtype == PSH_F64) return backward<double>(c, d);
+    if (d->dtype == PSH_F32) return backward<float>(c, d);
+    return backward<bf16_t>(c, d);
+}

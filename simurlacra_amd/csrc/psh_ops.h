@@ -1,0 +1,143 @@
+// What the translation units of the policy operators (ops_linear.hip, ops_memory.hip) share: element types, the search
+// for the part of the rows that a workgroup works on, and the fp32 / fp64 elementary functions.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "psh_ctx.h"
+#include "psh_math.h"
+
+#define PSH_OP __device__ __forceinline__
+
+typedef unsigned short bf16_t;  // storage; arithmetic is fp32
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef double v4d __attribute__((ext_vector_type(4)));
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef unsigned int v4u __attribute__((ext_vector_type(4)));
+
+template <class T> struct Wide { typedef float type; };
+template <> struct Wide<double> { typedef double type; };
+
+PSH_OP float to_wide(bf16_t x) { return __uint_as_float((unsigned)x << 16); }
+PSH_OP float to_wide(float x) { return x; }
+PSH_OP double to_wide(double x) { return x; }
+// to the nearest, ties to even; a NaN stays one.  The hardware conversion (v_cvt_pk_bf16_f32) rounds the same way.
+template <class T> PSH_OP T to_elem(typename Wide<T>::type x);
+template <> PSH_OP float to_elem<float>(float x) { return x; }
+template <> PSH_OP double to_elem<double>(double x) { return x; }
+template <> PSH_OP bf16_t to_elem<bf16_t>(float x) {
+    const __bf16 b = (__bf16)x;
+    return __builtin_bit_cast(bf16_t, b);
+}
+
+// ------------------------------------------------------------------------------------------ elementary functions
+// fp32: v_exp_f32 / v_log_f32 / v_rcp_f32 are within 1 ulp of the power, logarithm and reciprocal; what the argument's
+// scaling by log2(e) adds is |x| 2^-24 relative, which an exponential of a negative argument shrinks again.
+#define PSH_LOG2E 1.4426950408889634
+#define PSH_LN2 0.6931471805599453
+PSH_OP float exp2_w(float x) { return __builtin_amdgcn_exp2f(x); }
+PSH_OP float exp_w(float x) { return __builtin_amdgcn_exp2f(x * (float)PSH_LOG2E); }
+PSH_OP double exp_w(double x) { return psh_exp(x); }
+PSH_OP float rcp_w(float x) { return __builtin_amdgcn_rcpf(x); }
+PSH_OP float sigmoid_w(float x) { return rcp_w(1.f + exp_w(-x)); }
+PSH_OP double sigmoid_w(double x) { return psh_sigmoid(x); }
+template <class W> PSH_OP W silu_w(W x) { return x * sigmoid_w(x); }
+// d/dx of x sigmoid(x) from s = sigmoid(x)
+template <class W> PSH_OP W silu_slope_w(W x, W s) { return s * (W(1) + x * (W(1) - s)); }
+// log(1 + e^x) = max(x, 0) + log1p(e^-|x|).  log1p keeps the digits of a small e, where the step sizes of a slow memory are.
+PSH_OP float softplus_w(float x) { return fmaxf(x, 0.f) + (x != x ? x : log1pf(exp_w(-fabsf(x)))); }
+PSH_OP double softplus_w(double x) { return fmax(x, 0.) + (x != x ? x : log1p(psh_exp(-fabs(x)))); }
+PSH_OP float tanh_w(float x) { return tanhf(x); }
+PSH_OP double tanh_w(double x) { return psh_tanh(x); }
+
+template <class W> PSH_OP W nonlin_w(int kind, W x) {
+    if (kind == PSH_NL_TANH) return tanh_w(x);
+    if (kind == PSH_NL_SIGMOID) return sigmoid_w(x);
+    if (kind == PSH_NL_RELU) return x <= W(0) ? W(0) : x;  // a NaN stays one
+    return x;
+}
+// derivative of the nonlinearity from its value
+template <class W> PSH_OP W nonlin_slope_w(int kind, W y) {
+    if (kind == PSH_NL_TANH) return W(1) - y * y;
+    if (kind == PSH_NL_SIGMOID) return y * (W(1) - y);
+    if (kind == PSH_NL_RELU) return y <= W(0) ? W(0) : W(1);
+    return W(1);
+}
+
+// ------------------------------------------------------------------------------------------ parts of the rows
+// Rows are cut into n parts by offsets (device memory, so the host cannot count tiles) and a launch works in pieces of L
+// rows.  Piece j of part i gets the slot  floor(off[i] / L) + i + j.  Two parts never share a slot: with off[i] = a L + r
+// and off[i+1] = b L + r', part i has ceil((b - a) + (r' - r) / L) <= b - a + 1 pieces, exactly the distance of the two
+// parts' first slots.  So slots are found without a prefix sum or a second launch, there are at most rows / L + n + 1 of
+// them, and every part owns at least one, empty parts too.  Part n stands for the rows behind the last offset.
+struct Parts {
+    const int* off;
+    int n, rows, L;
+    PSH_OP int at(int i) const {
+        if (i <= 0) return 0;
+        if (i > n) return rows;
+        const int o = off[i];
+        return o < 0 ? 0 : (o > rows ? rows : o);
+    }
+    PSH_OP int first_slot(int i) const { return at(i) / L + i; }
+};
+static inline long parts_slots(long rows, long n, long L) { return rows / L + n + 1; }
+
+struct Piece {
+    int part, j;      // piece j of the part
+    int begin, end;   // its rows (begin >= end: none)
+    int part_begin, part_end;
+};
+
+// the largest i in [0, n] with key(i) <= slot, for ascending keys with key(0) <= slot: every lane of the wave probes one of 64
+// candidates at once, so 4096 parts take two rounds of loads where a binary search takes twelve
+template <class F> PSH_OP int wave_search(int n, int slot, F key) {
+    const int lane = __lane_id();
+    int lo = 0, count = n + 1;
+    while (count > 1) {
+        const int step = (count + 63) / 64;
+        const int i = lo + lane * step;
+        const bool below = lane * step < count && key(i) <= slot;
+        const int next = lo + (63 - __clzll(__ballot(below) | 1)) * step;   // (lane 0 probes lo itself: key(lo) <= slot)
+        count = min(step, lo + count - next);
+        lo = next;
+    }
+    return __builtin_amdgcn_readfirstlane(lo);
+}
+
+PSH_OP Piece find_piece(const Parts& p, int slot) {
+    Piece q;
+    q.part = wave_search(p.n, slot, [&](int i) { return p.first_slot(i); });
+    q.part_begin = __builtin_amdgcn_readfirstlane(p.at(q.part));
+    q.part_end = __builtin_amdgcn_readfirstlane(p.at(q.part + 1));
+    q.j = slot - (q.part_begin / p.L + q.part);
+    const long b = (long)q.part_begin + (long)q.j * p.L, e = b + p.L;
+    q.begin = (int)(b < p.rows ? b : p.rows);
+    q.end = (int)(e < q.part_end ? e : q.part_end);
+    return q;
+}
+
+// ------------------------------------------------------------------------------------------ host side
+// the calling thread's current device is the context's for the duration of a call
+struct DeviceScope {
+    int before = -1;
+    bool ok = false;
+    explicit DeviceScope(int device) {
+        ok = hipGetDevice(&before) == hipSuccess && (before == device || hipSetDevice(device) == hipSuccess);
+        if (before == device) before = -1;
+    }
+    ~DeviceScope() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+};
+#define PSH_ON_DEVICE(ctx)                                                         \
+    DeviceScope scope_((ctx)->device);                                             \
+    if (!scope_.ok) {                                                              \
+        set_err(ctx, "cannot make the context's GPU current");                     \
+        return PSH_ERR_HIP;                                                        \
+    }
+static inline int64_t align256(int64_t n) { return (n + 255) & ~(int64_t)255; }
+static inline int elem_size(int dtype) { return dtype == PSH_F64 ? 8 : dtype == PSH_F32 ? 4 : 2; }
+static inline int wide_size(int dtype) { return dtype == PSH_F64 ? 8 : 4; }
