@@ -64,4 +64,4 @@ class LogScaleNoise(nn.Module):
             self._set_scale(scale)
 
     def _center(self, value: to.Tensor) -> to.Tensor:
-        return value if self.mean is None else value + self.mean
+        return value if self.mean is None else value + self.mean.to(value.device)

@@ -36,7 +36,7 @@ class DiagNormalNoise(LogScaleNoise):
         self._adapt(mean, std)
 
     def forward(self, value: to.Tensor) -> Normal:
-        return Normal(self._center(value), self.std)
+        return Normal(self._center(value), self.std.to(value.device))
 
     def get_entropy(self) -> to.Tensor:
         # differential entropy of N(., diag(std^2)) written as in the reference: 1/2 + ln(2 pi)/2 + ln(prod std^2)/2

@@ -32,7 +32,13 @@ class StochasticActionExplStrat(Policy, ABC):
     def reset(self):
         self.policy.reset()
 
+    def init_hidden(self, batch_size: int = None) -> to.Tensor:
+        return self.policy.init_hidden(batch_size)
+
     def forward(self, obs: to.Tensor, *extra) -> to.Tensor:
+        if self.is_recurrent:
+            act, hidden = self.policy(obs, *extra)
+            return self.action_dist_at(act).rsample(), hidden
         act = self.policy(obs, *extra)
         return self.action_dist_at(act).rsample()  # reparametrised sample around the policy's output
 

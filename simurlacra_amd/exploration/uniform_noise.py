@@ -34,7 +34,7 @@ class UniformNoise(LogScaleNoise):
         self._adapt(mean, halfspan)
 
     def forward(self, value: to.Tensor) -> Uniform:
-        center, h = self._center(value), self.halfspan
+        center, h = self._center(value), self.halfspan.to(value.device)
         return Uniform(low=center - h, high=center + h)
 
     def get_entropy(self) -> to.Tensor:

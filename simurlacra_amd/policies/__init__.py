@@ -5,4 +5,5 @@ from .features import (FeatureStack, MultFeat, RandFourierFeat, RBFFeat, abs_fea
 from .fnn import FNN, FNNPolicy
 from .linear import LinearPolicy
 from .initialization import init_param
+from .recurrent import RecurrentPolicy, SSMPolicy
 from .time import TimePolicy

@@ -7,8 +7,10 @@ import torch as to
 import torch.nn as nn
 from torch.nn.utils import convert_parameters as cp
 
+from .. import operators as ops
 from ..specs import PolicySpec
 from ..utils.data_types import EnvSpec
+from ..utils.exceptions import ShapeErr
 from .base import Policy
 from .initialization import init_param
 
@@ -117,3 +119,30 @@ class FNNPolicy(Policy):
             return None
         return PolicySpec('fnn', self.env_spec.obs_space.flat_dim, self.env_spec.act_space.flat_dim, hidden=hidden,
                           hidden_nonlin=nls, out_nonlin=out_nl)
+
+    # ---- populations of networks of any width and depth (those that the rollout kernels do not take), layer by layer
+    @property
+    def supports_population(self) -> bool:
+        """ Whether the nonlinearities are among those of operators.grouped_linear, and none is random. """
+        try:
+            return self.net.dropout == 0 and all(nl in _FUSABLE_NL for nl in [*self.net.hidden_nonlin, self.net.output_nonlin])
+        except TypeError:
+            return False
+
+    def population_forward(self, params: to.Tensor, obs: to.Tensor, rows: to.Tensor) -> to.Tensor:
+        """ Policy p, with the parameters params[p], acts on obs[rows[p]:rows[p + 1]] (GPU tensors, float64). """
+        if not self.supports_population:
+            raise NotImplementedError('a population needs networks without dropout whose nonlinearities are tanh, relu, sigmoid or none')
+        if params.dim() != 2 or params.shape[1] != self.num_param:
+            raise ShapeErr(msg=f'params must have the shape [policies, {self.num_param}], but has {list(params.shape)}!')
+        layers = [l for l in self.net.hidden_layers if isinstance(l, nn.Linear)] + [self.net.output_layer]
+        x, at, P = obs, 0, params.shape[0]
+        for l, nl in zip(layers, [*self.net.hidden_nonlin, self.net.output_nonlin]):
+            mid, end = at + l.weight.numel(), at + l.weight.numel() + l.bias.numel()
+            x = ops.grouped_linear(x, params[:, at:mid].view(P, *l.weight.shape), params[:, mid:end], rows, _FUSABLE_NL[nl])
+            at = end
+        return x
+
+    def population_evaluate(self, params: to.Tensor, obs: to.Tensor, offsets: to.Tensor, groups: to.Tensor) -> to.Tensor:
+        """ The actions for whole episodes obs[offsets[s]:offsets[s + 1]], of which groups[p] .. groups[p + 1] - 1 are policy p's. """
+        return self.population_forward(params, obs, offsets[groups.long()])

@@ -216,10 +216,16 @@ def run_batch(plan: EnvPlan, eng, policy, init_state, dp, dp_index=None, *, max_
         return eng.rollout(plan.kind, plan.sim.dt, T, task_c, spec, params, init_state, dp, flags=plan.flags(stop_on_done),
                            dp_index=dp_index, policy_index=policy_index, policy_group=policy_group, record=record,
                            wrap=wrap, bernoulli_reset=p_reset)
-    if params is not None:
-        raise NotImplementedError('per-environment policy parameters need a fusable policy')
+    if params is not None and (policy_index is not None or not _steps_as_population(policy)):
+        raise NotImplementedError('per-environment policy parameters need a fusable policy, or one with population_forward() '
+                                  'and the environments of a policy side by side')
     return _run_batch_stepwise(plan, eng, policy, init_state, dp, dp_index, T, stop_on_done, record, task_c, wrap,
-                               p_reset)
+                               p_reset, params)
+
+
+def _steps_as_population(policy) -> bool:
+    """ Whether the step loop can run a population of this policy. """
+    return hasattr(policy, 'population_forward') and getattr(policy, 'supports_population', True)
 
 
 def _obs_bounds(plan, dp, dp_index, N):
@@ -253,10 +259,11 @@ def _obs_bounds(plan, dp, dp_index, N):
 
 
 def _run_batch_stepwise(plan, eng, policy, init_state, dp, dp_index, T, stop_on_done, record, task_c, wrap=None,
-                        p_reset=0.):
+                        p_reset=0., params=None):
     """ rollout() loop (Pyrado/pyrado/sampling/rollout.py:133-254) for N envs at once with an arbitrary torch policy;
     the wrappers of the chain are applied to the whole batch between policy and psh_step.  Noise comes from torch's
-    generator here (the fused kernels use their own counter-based one). """
+    generator here (the fused kernels use their own counter-based one).  A policy with memory carries one hidden state
+    per environment.  params [P, num_param]: a population, of which each policy has N/P neighbouring environments. """
     kind, dt, dev = plan.kind, plan.sim.dt, eng.device
     init_state, dp = eng.f64(init_state), eng.f64(dp)
     dp_index = eng.i32(dp_index)
@@ -301,6 +308,27 @@ def _run_batch_stepwise(plan, eng, policy, init_state, dp, dp_index, T, stop_on_
         delays = delays.expand(N).clamp(0, abi.PSH_MAX_DELAY).long()
         H = int(delays.max().item()) + 1
         hist = torch.zeros((H, A, N), dtype=torch.float64, device=dev)
+    recurrent = getattr(policy, 'is_recurrent', False)
+    hidden = policy.init_hidden(N) if recurrent else None
+    if params is not None:
+        params = torch.atleast_2d(params).to(dev)
+        if N % max(1, params.shape[0]):
+            raise ValueErr(msg=f'{N} environments are not the same number for each of {params.shape[0]} policies!')
+        if recurrent:
+            params = params.to(policy.dtype)
+        rows = torch.arange(params.shape[0] + 1, dtype=torch.int32, device=dev)*(N//max(1, params.shape[0]))
+
+    def act_on(obs):
+        """ the policy's actions for obs [N, Oe], its hidden states advanced """
+        nonlocal hidden
+        extra = () if hidden is None else (hidden,)
+        if params is not None:
+            got = policy.population_forward(params, obs, rows, *extra)
+        else:
+            got = policy(obs.to(pol_dev), *extra)
+        if recurrent:
+            got, hidden = got
+        return got
     alias = not ('act_norm' in ops or 'act_noise' in ops)
     lane = torch.arange(N, device=dev)
     if hasattr(policy, 'reset'):
@@ -311,7 +339,7 @@ def _run_batch_stepwise(plan, eng, policy, init_state, dp, dp_index, T, stop_on_
         if record:
             out['obs'][k][:, live] = obs[:, live]
         with torch.no_grad():
-            act = policy(obs.t().to(pol_dev)).to(dev, torch.float64).reshape(N, A).t().contiguous()
+            act = act_on(obs.t()).to(dev, torch.float64).reshape(N, A).t().contiguous()
         nan = torch.isnan(act).any(dim=0) | torch.isnan(obs).any(dim=0)
         inner = act.clone()
         for op in ops:  # action wrappers, outermost first

@@ -16,7 +16,8 @@ from ..environment_wrappers.utils import typed_env
 from . import distributed as D
 from .. import _abi as abi
 from ..utils.exceptions import ValueErr
-from .batch import EnvPlan, RolloutBatch, SummaryRollouts, run_batch, sample_domain_params, sample_init_states
+from .batch import (EnvPlan, RolloutBatch, SummaryRollouts, _steps_as_population, run_batch, sample_domain_params,
+                    sample_init_states)
 
 
 class ParameterSample(NamedTuple):
@@ -59,8 +60,9 @@ class _LazySamples(Sequence):
 
 class ParameterSamplingResult(Sequence):
     def __init__(self, samples: Sequence, mean_returns: np.ndarray = None, mean_returns_device=None,
-                 param_sets: to.Tensor = None, num_rollouts: int = None):
+                 param_sets: to.Tensor = None, num_rollouts: int = None, batch: RolloutBatch = None):
         self._samples = samples
+        self.batch = batch        # the rollouts of all parameter sets, one set after the other (None: not all on this GPU)
         self._mean_returns = mean_returns
         self._means_dev = mean_returns_device     # the same means, still on the GPU (all parameter sets, every rank)
         self._param_sets, self._num_rollouts = param_sets, num_rollouts
@@ -150,11 +152,12 @@ class ParameterExplorationSampler:
         r_idx = to.arange(R, dtype=to.int32, device=dev).repeat(my)
         init = init_r[:, r_idx.long()].contiguous()
         spec = self.policy.fused_spec() if hasattr(self.policy, 'fused_spec') else None
-        if spec is None:
+        if spec is None and not _steps_as_population(self.policy):
             raise NotImplementedError('ParameterExplorationSampler needs a LinearPolicy or FNNPolicy that the rollout '
-                                      'kernels can fuse')
+                                      'kernels can fuse, or a policy with population_forward()')
         my_params = param_sets[p0:p1].to(dev)
-        # one launch for the whole population: lane j*R + r runs parameter set j on the shared pair r
+        # one launch for the whole population (for a policy that is not fused, one step loop): lane j*R + r runs parameter
+        # set j on the shared pair r
         out = run_batch(plan, eng, self.policy, init, dp, r_idx, record=self.record_trajectories, params=my_params,
                         policy_group=R if my > 1 else 0, noise_seed=key, env_offset=p0*R)
         batch = RolloutBatch(plan, out, dp, r_idx)
@@ -164,7 +167,7 @@ class ParameterExplorationSampler:
         if ws == 1:
             batch.check()
             samples = _LazySamples(pop, lambda j: ParameterSample(params=param_sets[j], rollouts=batch.slice(j*R, R)))
-            return ParameterSamplingResult(samples, means, means_dev, param_sets, pop*R)
+            return ParameterSamplingResult(samples, means, means_dev, param_sets, pop*R, batch)
         # every rank gets the returns, lengths and status words of ALL parameter sets ([pop, R] each; trajectories
         # stay where they were produced), so num_rollouts, len(rollout) and slicing of the result agree on all ranks
         ret = D.all_gather_rows(out['ret'].view(my, R), pop).cpu().numpy()
