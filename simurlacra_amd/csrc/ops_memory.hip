@@ -22,14 +22,15 @@ struct Policies {
     PSH_OP int of(int seq) const { return n == 1 || !groups ? 0 : wave_search(n - 1, seq, [&](int p) { return at(p); }); }
 };
 
-template <class T, int E> struct alignas(sizeof(T) * E) Pack { T v[E]; };
+// (vectors and not arrays in a struct: those the compiler keeps in memory once a branch writes them)
+template <class T, int E> struct Vec { typedef T type __attribute__((ext_vector_type(E))); };
 
 // E elements of a line with n valid ones starting at c; elements behind it are zero
 template <int E, class T> PSH_OP void load_line(typename Wide<T>::type (&out)[E], const T* line, int c, int n, bool vec) {
     if (vec && c + E <= n) {
-        const Pack<T, E> p = *reinterpret_cast<const Pack<T, E>*>(line + c);
+        const typename Vec<T, E>::type p = *reinterpret_cast<const typename Vec<T, E>::type*>(line + c);
 #pragma unroll
-        for (int e = 0; e < E; ++e) out[e] = to_wide(p.v[e]);
+        for (int e = 0; e < E; ++e) out[e] = to_wide((T)p[e]);
     } else {
 #pragma unroll
         for (int e = 0; e < E; ++e) out[e] = c + e < n ? to_wide(line[c + e]) : typename Wide<T>::type(0);
@@ -37,15 +38,23 @@ template <int E, class T> PSH_OP void load_line(typename Wide<T>::type (&out)[E]
 }
 template <int E, class T> PSH_OP void store_line(T* line, const typename Wide<T>::type (&in)[E], int c, int n, bool vec) {
     if (vec && c + E <= n) {
-        Pack<T, E> p;
+        typename Vec<T, E>::type p;
 #pragma unroll
-        for (int e = 0; e < E; ++e) p.v[e] = to_elem<T>(in[e]);
-        *reinterpret_cast<Pack<T, E>*>(line + c) = p;
+        for (int e = 0; e < E; ++e) p[e] = to_elem<T>(in[e]);
+        *reinterpret_cast<typename Vec<T, E>::type*>(line + c) = p;
     } else {
 #pragma unroll
         for (int e = 0; e < E; ++e)
             if (c + e < n) line[c + e] = to_elem<T>(in[e]);
     }
+}
+
+template <int E, class T> PSH_OP typename Vec<T, E>::type load_raw(const T* line, int c, int n, bool vec) {
+    if (vec && c + E <= n) return *reinterpret_cast<const typename Vec<T, E>::type*>(line + c);
+    typename Vec<T, E>::type out;
+#pragma unroll
+    for (int e = 0; e < E; ++e) out[e] = c + e < n ? line[c + e] : T(0);
+    return out;
 }
 
 // ====================================================================================================== convolution
@@ -70,6 +79,7 @@ template <class T> struct ConvArgs {
 };
 constexpr int CONV_ROWS = 16;        // rows of one lane's run
 constexpr int CONV_GRAD_ROWS = 32;
+constexpr int CONV_BATCH = 4;        // rows whose loads are in flight together
 
 template <class T, int K> PSH_OP void conv_params(typename Wide<T>::type (&w)[K], typename Wide<T>::type& b, const ConvArgs<T>& a, int p, int c) {
     const bool in = c < a.D;
@@ -123,21 +133,28 @@ template <class T, int V, int K> __global__ __launch_bounds__(256) void k_conv(c
     for (int e = 0; e < V; ++e) conv_params<T, K>(w[e], b[e], a, p, c + e);
 #pragma unroll
     for (int k = 0; k < K - 1; ++k) conv_input<V, K>(win[k], a, q, r0 - (K - 1) + k, c);
-    for (int r = r0; r < r1; ++r) {
-        load_line<V>(win[K - 1], a.x + (long)r * a.ld_x, c, a.D, a.vec);
-        W y[V];
+    for (int r = r0; r < r1; r += CONV_BATCH) {
+        typename Vec<T, V>::type in[CONV_BATCH];
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-            W s = b[e];
+        for (int i = 0; i < CONV_BATCH; ++i) in[i] = load_raw<V>(a.x + (long)min(r + i, r1 - 1) * a.ld_x, c, a.D, a.vec);
 #pragma unroll
-            for (int k = 0; k < K; ++k) s += w[e][k] * win[k][e];
-            y[e] = a.silu ? silu_w(s) : s;
+        for (int i = 0; i < CONV_BATCH; ++i) {
+            if (r + i >= r1) break;
+            W y[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                win[K - 1][e] = to_wide((T)in[i][e]);
+                W s = b[e];
+#pragma unroll
+                for (int k = 0; k < K; ++k) s += w[e][k] * win[k][e];
+                y[e] = a.silu ? silu_w(s) : s;
+            }
+            store_line<V>(a.y + (long)(r + i) * a.D, y, c, a.D, a.vec);
+#pragma unroll
+            for (int k = 0; k < K - 1; ++k)
+#pragma unroll
+                for (int e = 0; e < V; ++e) win[k][e] = win[k + 1][e];
         }
-        store_line<V>(a.y + (long)r * a.D, y, c, a.D, a.vec);
-#pragma unroll
-        for (int k = 0; k < K - 1; ++k)
-#pragma unroll
-            for (int e = 0; e < V; ++e) win[k][e] = win[k + 1][e];
     }
 }
 
@@ -205,17 +222,30 @@ template <class T, int V, int K> __global__ __launch_bounds__(256) void k_conv_g
 #pragma unroll
         for (int k = 0; k < K - 1; ++k) conv_input<V, K>(win[k], a, q, start - (K - 1) + k, c);
         // rows start .. stop + K - 2; those behind the run only for dpre, those behind the sequence not at all
-        for (int t = start; t < stop + K - 1; ++t) {
+        for (int t0 = start; t0 < stop + K - 1; t0 += CONV_BATCH) {
+        typename Vec<T, V>::type in[CONV_BATCH], up[CONV_BATCH];
+#pragma unroll
+        for (int i = 0; i < CONV_BATCH; ++i) {
+            const int t = t0 + i;
+            in[i] = up[i] = T(0);
+            if (t < q.part_end && t < stop + K - 1) {
+                in[i] = load_raw<V>(a.x + (long)t * a.ld_x, c, a.D, a.vec);
+                up[i] = load_raw<V>(a.dy + (long)t * a.ld_dy, c, a.D, a.vec);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < CONV_BATCH; ++i) {
+            const int t = t0 + i;
+            if (t >= stop + K - 1) break;
             if (t < q.part_end) {
-                load_line<V>(win[K - 1], a.x + (long)t * a.ld_x, c, a.D, a.vec);
-                W dy[V];
-                load_line<V>(dy, a.dy + (long)t * a.ld_dy, c, a.D, a.vec);
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
+                    win[K - 1][e] = to_wide((T)in[i][e]);
+                    const W dy = to_wide((T)up[i][e]);
                     W s = b[e];
 #pragma unroll
                     for (int k = 0; k < K; ++k) s += w[e][k] * win[k][e];
-                    dp[K - 1][e] = a.silu ? dy[e] * silu_slope_w(s, sigmoid_w(s)) : dy[e];
+                    dp[K - 1][e] = a.silu ? dy * silu_slope_w(s, sigmoid_w(s)) : dy;
                     if (t < stop) {
                         db[e] += dp[K - 1][e];
 #pragma unroll
@@ -255,6 +285,7 @@ template <class T, int V, int K> __global__ __launch_bounds__(256) void k_conv_g
                     win[k][e] = win[k + 1][e];
                     dp[k][e] = dp[k + 1][e];
                 }
+        }
         }
     }
     if (!a.part) return;
@@ -366,6 +397,7 @@ template <class T> struct ScanArgs {
     W* check;                // [rows / TS + n + 1, D, N] states before every tile
     W* carry;                // [slots, D, N]: states (adjoint states) at the pieces' beginnings (ends), NULL: pieces are whole sequences
     W* carry_dt;             // [slots, D]
+    const int* order;        // slot of every workgroup, NULL: its number
     bool vec_d, vec_n;       // wide loads of channel rows / of states
     // gradients
     const T* dy; long ld_dy;
@@ -380,7 +412,13 @@ template <class T> struct ScanArgs {
 PSH_OP float decay_rate(float a) { return a * (float)PSH_LOG2E; }
 PSH_OP double decay_rate(double a) { return a; }
 PSH_OP float decay(float dt, float rate) { return exp2_w(dt * rate); }
-PSH_OP double decay(double dt, double rate) { return psh_exp(dt * rate); }
+// (psh_exp without its branch, which would keep the states of a step from running side by side: the core is right, and over- or
+// underflows, for every |x| < 2^30, so only the high word of what lies beyond is replaced; a NaN stays one)
+PSH_OP double decay(double dt, double rate) {
+    const double x = dt * rate;
+    const int hi = __double2hiint(x);
+    return psh_exp_core(__hiloint2double(fabs(x) > 1e9 ? (hi & (int)0x80000000) | 0x41cdcd65 : hi, __double2loint(x)));
+}
 // sum of g a h' A from a sum with prepared rates
 PSH_OP float rate_unit(float) { return (float)PSH_LN2; }
 PSH_OP double rate_unit(double) { return 1.; }
@@ -420,16 +458,21 @@ PSH_OP double halves16(double a, double b) {
     return __hiloint2double((int)h[0], (int)l[0]) + __hiloint2double((int)h[1], (int)l[1]);
 }
 
+// Keeps the scheduler from running several steps' exponentials side by side: in fp64 one step has enough of them to fill the
+// pipe, and more do not fit into the registers.
+template <class W> PSH_OP void step_fence() {
+    if constexpr (sizeof(W) == 8) __builtin_amdgcn_sched_barrier(0);
+}
+
 template <class W> struct alignas(2 * sizeof(W)) Pair { W dt, dtu; };
 
 // NP states of a lane from / to [.., D, N] memory
 template <int NP, class W> PSH_OP void load_states(W (&h)[NP], const W* p, int n, int N, bool vec) { load_line<NP>(h, p, n, N, vec); }
 
-// What a thread loads of a tile: E channels of one step.
+// What a thread loads of a tile: E channels of one step, as they are in memory.
 template <class T, int E> struct Rows {
-    typename Wide<T>::type u[E], delta[E], z[E], dy[E];
+    typename Vec<T, E>::type u, delta, z, dy;
 };
-
 template <class T, class SH> struct Loader {
     typedef typename Wide<T>::type W;
     static constexpr int E = SH::E, TS = SH::TS, CB = SH::CB;
@@ -452,14 +495,13 @@ template <class T, class SH> struct Loader {
     template <bool GRAD> PSH_OP void fetch(Rows<T, E>& r, const ScanArgs<T>& a, int row0, int end) const {
         const long row = row0 + t;
         if (!on || row >= end) {
-#pragma unroll
-            for (int e = 0; e < E; ++e) r.u[e] = r.delta[e] = r.z[e] = r.dy[e] = 0;
+            r.u = r.delta = r.z = r.dy = T(0);
             return;
         }
-        load_line<E>(r.u, a.u + row * a.ld_u, d, a.D, a.vec_d);
-        load_line<E>(r.delta, a.delta + row * a.ld_delta, d, a.D, a.vec_d);
-        if (a.z) load_line<E>(r.z, a.z + row * a.ld_z, d, a.D, a.vec_d);
-        if constexpr (GRAD) load_line<E>(r.dy, a.dy + row * a.ld_dy, d, a.D, a.vec_d);
+        r.u = load_raw<E>(a.u + row * a.ld_u, d, a.D, a.vec_d);
+        r.delta = load_raw<E>(a.delta + row * a.ld_delta, d, a.D, a.vec_d);
+        if (a.z) r.z = load_raw<E>(a.z + row * a.ld_z, d, a.D, a.vec_d);
+        if constexpr (GRAD) r.dy = load_raw<E>(a.dy + row * a.ld_dy, d, a.D, a.vec_d);
     }
 };
 
@@ -489,6 +531,44 @@ template <class T, class SH> struct StepRows {
     }
 };
 
+// Sequences from the longest to the shortest (to 1/256 of the longest), for launches of whole sequences: workgroups are
+// handed out in this order, so that those that run last, or that share a CU, are not by chance the long ones.
+constexpr int ORDER_MOST = 16384;   // sequences; with more, chance evens the CUs out
+__global__ __launch_bounds__(1024) void k_order(const Parts p, int* order) {
+    __shared__ int count[256], most;
+    const int tid = threadIdx.x;
+    if (tid == 0) most = 1;
+    if (tid < 256) count[tid] = 0;
+    __syncthreads();
+    int m = 1;
+    for (int s = tid; s < p.n; s += 1024) m = max(m, p.at(s + 1) - p.at(s));
+    for (int k = 32; k > 0; k /= 2) m = max(m, __shfl_xor(m, k));
+    if ((tid & 63) == 0) atomicMax(&most, m);
+    __syncthreads();
+    const float scale = 255.f / (float)most;
+    for (int s = tid; s < p.n; s += 1024) atomicAdd(&count[255 - min(255, (int)((float)max(0, p.at(s + 1) - p.at(s)) * scale))], 1);
+    __syncthreads();
+    if (tid < 64) {   // exclusive prefix sums of 4 buckets a lane
+        int c[4], sum = 0;
+        for (int i = 0; i < 4; ++i) {
+            c[i] = count[tid * 4 + i];
+            sum += c[i];
+        }
+        int before = sum;
+        for (int k = 1; k < 64; k *= 2) {
+            const int o = __shfl_up(before, k);
+            before += tid >= k ? o : 0;
+        }
+        before -= sum;
+        for (int i = 0; i < 4; ++i) {
+            count[tid * 4 + i] = before;
+            before += c[i];
+        }
+    }
+    __syncthreads();
+    for (int s = tid; s < p.n; s += 1024) order[atomicAdd(&count[255 - min(255, (int)((float)max(0, p.at(s + 1) - p.at(s)) * scale))], 1)] = s;
+}
+
 // h_t along a piece.  CARRY: only the state at the piece's end from zero and the sum of its step sizes, for the joining
 // of pieces; otherwise y as well, from the state at the piece's beginning.
 template <class T, int NP, int LPC, bool CARRY> __global__ __launch_bounds__(THREADS) void k_scan(const ScanArgs<T> a) {
@@ -499,7 +579,7 @@ template <class T, int NP, int LPC, bool CARRY> __global__ __launch_bounds__(THR
     __shared__ __align__(16) W s_b[TS * NL];
     __shared__ __align__(16) W s_c[CARRY ? 1 : TS * NL];
     __shared__ __align__(16) W s_y[CARRY ? 1 : TS][CB];
-    const int slot = blockIdx.x, c0 = (int)blockIdx.y * CB;
+    const int slot = a.order && (int)blockIdx.x < a.parts.n ? a.order[blockIdx.x] : (int)blockIdx.x, c0 = (int)blockIdx.y * CB;
     const Piece q = find_piece(a.parts, slot);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int ql = lane % LPC, cl = wave * (64 / LPC) + lane / LPC;     // lane of the channel, channel of the block
@@ -541,8 +621,8 @@ template <class T, int NP, int LPC, bool CARRY> __global__ __launch_bounds__(THR
         if (ld.on) {
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                const W dt = r0 + ld.t < q.end ? softplus_w(now.delta[e] + ld.bias[e]) : W(0);
-                s_dt[ld.t][ld.c + e] = Pair<W>{dt, dt * now.u[e]};
+                const W dt = r0 + ld.t < q.end ? softplus_w(to_wide((T)now.delta[e]) + ld.bias[e]) : W(0);
+                s_dt[ld.t][ld.c + e] = Pair<W>{dt, dt * to_wide((T)now.u[e])};
             }
         }
         bc.template store<!CARRY>(s_b, s_c);
@@ -554,7 +634,7 @@ template <class T, int NP, int LPC, bool CARRY> __global__ __launch_bounds__(THR
         if constexpr (!CARRY) {
             if (a.check && d < a.D) store_line<NP>(a.check + ((check0 + tile) * a.D + d) * a.N, h, n0, a.N, a.vec_n);
         }
-#pragma unroll
+#pragma unroll 1
         for (int t1 = 0; t1 < TS; t1 += LPC < TS ? LPC : TS) {
             W keep = 0;
 #pragma unroll
@@ -575,6 +655,7 @@ template <class T, int NP, int LPC, bool CARRY> __global__ __launch_bounds__(THR
                     y = sum_states<LPC>(y);
                     keep = ql == t2 ? y : keep;
                 }
+                step_fence<W>();
             }
             if constexpr (!CARRY) {
                 if (ql < TS) s_y[t1 + ql][cl] = keep;
@@ -588,8 +669,8 @@ template <class T, int NP, int LPC, bool CARRY> __global__ __launch_bounds__(THR
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
                     W v = s_y[ld.t][ld.c + e];
-                    if (a.skip) v += ld.skip[e] * now.u[e];
-                    out[e] = a.z ? v * silu_w(now.z[e]) : v;
+                    if (a.skip) v += ld.skip[e] * to_wide((T)now.u[e]);
+                    out[e] = a.z ? v * silu_w(to_wide((T)now.z[e])) : v;
                 }
                 store_line<E>(a.y + row * a.D, out, ld.d, a.D, a.vec_d);
             }
@@ -619,28 +700,40 @@ template <class T, bool BACK> __global__ __launch_bounds__(256) void k_scan_join
     W h = 0;
     if (BACK) h = a.dlast ? a.dlast[s * cols + m] : W(0);
     else h = a.state ? a.state[s * a.stride_state + m] : W(0);
-    for (int k = 0; k < n; ++k) {
-        const long slot = BACK ? first + n - 1 - k : first + k;
-        const W own = a.carry[slot * cols + m], dt = a.carry_dt[slot * a.D + d];
-        a.carry[slot * cols + m] = h;
-        h = decay(dt, rate) * h + own;
+    constexpr int AHEAD = 8;   // loads in flight: the chain itself is one fma a piece
+    for (int k = 0; k < n; k += AHEAD) {
+        W own[AHEAD], dt[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const long slot = BACK ? first + max(0, n - 1 - k - i) : first + min(n - 1, k + i);
+            own[i] = a.carry[slot * cols + m];
+            dt[i] = a.carry_dt[slot * a.D + d];
+        }
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            if (k + i >= n) break;
+            const long slot = BACK ? first + n - 1 - k - i : first + k + i;
+            a.carry[slot * cols + m] = h;
+            h = decay(dt[i], rate) * h + own[i];
+        }
     }
 }
 
 // The adjoint recurrence of a piece, tiles of TS steps from its end:  g_t = C_t dy0_t + G_{t+1},  G_t = a_t g_t,  where dy0 = dy silu(z).
 // Each tile first runs forward from its stored state and keeps a_t and h_{t-1} of its steps in registers (2 TS NP values
 // per lane), then backward.  CARRY: only G at the piece's beginning, from zero.
-template <class T, int NP, int LPC, bool CARRY> __global__ __launch_bounds__(THREADS) void k_scan_grad(const ScanArgs<T> a) {
+template <class T, int NP, int LPC, bool CARRY> __global__ __launch_bounds__(THREADS, 2) void k_scan_grad(const ScanArgs<T> a) {
     typedef typename Wide<T>::type W;
     typedef Shape<W, NP, LPC> SH;
     constexpr int TS = SH::TS, CB = SH::CB, E = SH::E, NL = SH::NL;
     constexpr int NV = 2 * NP < 4 ? 4 : 2 * NP;     // gradients of B and C of a step and lane, padded
     __shared__ Pair<W> s_dt[TS][CB];
     __shared__ __align__(16) W s_dy[TS][CB];
+    __shared__ __align__(16) W s_sz[CARRY ? 1 : TS][CB], s_sd[CARRY ? 1 : TS][CB];   // sigmoids of z and of delta + bias
     __shared__ __align__(16) W s_b[TS * NL], s_c[TS * NL];
     __shared__ __align__(16) W s_1[CARRY ? 1 : TS][CB], s_2[CARRY ? 1 : TS][CB], s_y[CARRY ? 1 : TS][CB];
     __shared__ __align__(16) W s_bc[CARRY ? 1 : 4 * TS * 2 * NL];
-    const int slot = blockIdx.x, c0 = (int)blockIdx.y * CB;
+    const int slot = a.order && (int)blockIdx.x < a.parts.n ? a.order[blockIdx.x] : (int)blockIdx.x, c0 = (int)blockIdx.y * CB;
     const Piece q = find_piece(a.parts, slot);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int ql = lane % LPC, cl = wave * (64 / LPC) + lane / LPC;
@@ -699,9 +792,17 @@ template <class T, int NP, int LPC, bool CARRY> __global__ __launch_bounds__(THR
         if (ld.on) {
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                dt[e] = r0 + ld.t < q.end ? softplus_w(now.delta[e] + ld.bias[e]) : W(0);
-                s_dt[ld.t][ld.c + e] = Pair<W>{dt[e], dt[e] * now.u[e]};
-                s_dy[ld.t][ld.c + e] = a.z ? now.dy[e] * silu_w(now.z[e]) : now.dy[e];
+                const W raw = to_wide((T)now.delta[e]) + ld.bias[e];
+                dt[e] = r0 + ld.t < q.end ? softplus_w(raw) : W(0);
+                s_dt[ld.t][ld.c + e] = Pair<W>{dt[e], dt[e] * to_wide((T)now.u[e])};
+                W dy = to_wide((T)now.dy[e]);
+                if (a.z) {
+                    const W z = to_wide((T)now.z[e]), sz = sigmoid_w(z);
+                    dy *= z * sz;
+                    if constexpr (!CARRY) s_sz[ld.t][ld.c + e] = sz;
+                }
+                s_dy[ld.t][ld.c + e] = dy;
+                if constexpr (!CARRY) s_sd[ld.t][ld.c + e] = sigmoid_w(raw);
             }
         }
         bc.template store<true>(s_b, s_c);
@@ -723,6 +824,7 @@ template <class T, int NP, int LPC, bool CARRY> __global__ __launch_bounds__(THR
                 total += step;
 #pragma unroll
                 for (int i = 0; i < NP; ++i) g[i] = decay(step, rate[i]) * (s_c[t * NL + n0 + i] * dy + g[i]);
+                step_fence<W>();
             }
         } else {
             W av[TS][NP], hv[TS][NP];   // a_t and h_{t-1}
@@ -745,8 +847,10 @@ template <class T, int NP, int LPC, bool CARRY> __global__ __launch_bounds__(THR
                         y = sum_states<LPC>(y);
                         keep = ql == t2 ? y : keep;
                     }
+                    step_fence<W>();
                 }
                 if (a.z && ql < TS) s_y[t1 + ql][cl] = keep;
+                __builtin_amdgcn_sched_barrier(0);   // (else every LDS read of the tile is hoisted to its top, into registers that it has not got)
             }
 #pragma unroll
             for (int t1 = TS - (LPC < TS ? LPC : TS); t1 >= 0; t1 -= LPC < TS ? LPC : TS) {
@@ -789,11 +893,13 @@ template <class T, int NP, int LPC, bool CARRY> __global__ __launch_bounds__(THR
                         if ((lane & 15) < LPC && k < 2 * NP)
                             s_bc[((wave * TS + t) * 2 + k / NP) * NL + n0 + k % NP] = s;
                     }
+                    step_fence<W>();
                 }
                 if (ql < TS) {
                     s_1[t1 + ql][cl] = keep1;
                     s_2[t1 + ql][cl] = keep2;
                 }
+                __builtin_amdgcn_sched_barrier(0);
             }
             __syncthreads();
             const long row = r0 + ld.t;
@@ -802,15 +908,15 @@ template <class T, int NP, int LPC, bool CARRY> __global__ __launch_bounds__(THR
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
                     const W dy0 = s_dy[ld.t][ld.c + e], s2 = s_2[ld.t][ld.c + e];
-                    const W ddt = s_1[ld.t][ld.c + e] * rate_unit(W(0)) + s2 * now.u[e];
-                    dd[e] = ddt * sigmoid_w(now.delta[e] + ld.bias[e]);
+                    const W ddt = s_1[ld.t][ld.c + e] * rate_unit(W(0)) + s2 * to_wide((T)now.u[e]);
+                    dd[e] = ddt * s_sd[ld.t][ld.c + e];
                     du[e] = dt[e] * s2 + (a.skip ? ld.skip[e] * dy0 : W(0));
                     dbias[e] += dd[e];
-                    dD[e] += dy0 * now.u[e];
+                    dD[e] += dy0 * to_wide((T)now.u[e]);
                     dz[e] = 0;
                     if (a.z) {
-                        const W y0 = s_y[ld.t][ld.c + e] + (a.skip ? ld.skip[e] * now.u[e] : W(0));
-                        dz[e] = now.dy[e] * y0 * silu_slope_w(now.z[e], sigmoid_w(now.z[e]));
+                        const W y0 = s_y[ld.t][ld.c + e] + (a.skip ? ld.skip[e] * to_wide((T)now.u[e]) : W(0));
+                        dz[e] = to_wide((T)now.dy[e]) * y0 * silu_slope_w(to_wide((T)now.z[e]), s_sz[ld.t][ld.c + e]);
                     }
                 }
                 if (a.du) store_line<E>(a.du + row * a.D, du, ld.d, a.D, a.vec_d);
@@ -930,17 +1036,25 @@ int channel_blocks(const psh_scan_desc* d) {
     const int cb = THREADS / lanes_per_channel(d->states);
     return (d->channels + cb - 1) / cb;
 }
-// rows of a piece: whole sequences
+// Rows of a piece.  A step of the recurrence takes a wave about 200 cycles however many waves there are, so a launch wants 4 workgroups
+// for every CU before its steps are throughput and not latency.  Sequences that are too few for that are cut, down to 64
+// rows, at the price of a second pass over the decays (the exponentials are most of the work) and of joining the pieces.
 int64_t scan_piece(const psh_scan_desc* d) {
-    const int64_t ts = tile_steps(d->dtype);
-    return ((int64_t)d->rows + ts) / ts * ts;
+    const int64_t ts = tile_steps(d->dtype), blocks = channel_blocks(d), whole = ((int64_t)d->rows + ts) / ts * ts;
+    if (d->n_seqs * blocks >= 768) return whole;
+    int64_t L = (int64_t)d->rows * blocks / 1024 / ts * ts;
+    if (L < 64) L = 64;
+    return L < whole ? L : whole;
 }
 bool scan_split(const psh_scan_desc* d) { return scan_piece(d) < d->rows; }
+bool scan_ordered(const psh_scan_desc* d) { return !d->step && !scan_split(d) && d->n_seqs > 1 && d->n_seqs <= ORDER_MOST && d->rows > 64 * (int64_t)d->n_seqs; }
 
-struct ScanSpace { int64_t carry, carry_dt, part, mid, bc, total; };
+// (the order of the launch, if any, lies first)
+struct ScanSpace { int64_t order, carry, carry_dt, part, mid, bc, total; };
 ScanSpace scan_space(const psh_scan_desc* d, bool grad) {
     ScanSpace s{};
     const int64_t slots = parts_slots(d->rows, d->n_seqs, scan_piece(d)), w = wide_size(d->dtype), D = d->channels, N = d->states;
+    if (scan_ordered(d)) s.order = align256((int64_t)d->n_seqs * 4);
     if (scan_split(d)) {
         s.carry = align256(slots * D * N * w);
         s.carry_dt = align256(slots * D * w);
@@ -952,7 +1066,7 @@ ScanSpace scan_space(const psh_scan_desc* d, bool grad) {
         }
         if ((d->dB || d->dC) && channel_blocks(d) > 1) s.bc = align256((int64_t)channel_blocks(d) * d->rows * 2 * N * w);
     }
-    s.total = s.carry + s.carry_dt + s.part + s.mid + s.bc;
+    s.total = s.order + s.carry + s.carry_dt + s.part + s.mid + s.bc;
     return s;
 }
 
@@ -1004,6 +1118,10 @@ template <class T, int NP, int LPC> int scan_forward(psh_ctx* c, const psh_scan_
     hipStream_t st = (hipStream_t)d->stream;
     const long slots = parts_slots(d->rows, d->n_seqs, a.parts.L);
     const dim3 grid((unsigned)slots, (unsigned)channel_blocks(d));
+    if (a.order) {
+        hipLaunchKernelGGL(k_order, dim3(1), dim3(1024), 0, st, a.parts, const_cast<int*>(a.order));
+        PSH_HIP(c, hipGetLastError());
+    }
     if (a.carry) {
         hipLaunchKernelGGL((k_scan<T, NP, LPC, true>), grid, dim3(THREADS), 0, st, a);
         PSH_HIP(c, hipGetLastError());
@@ -1018,6 +1136,10 @@ template <class T, int NP, int LPC> int scan_backward(psh_ctx* c, const psh_scan
     hipStream_t st = (hipStream_t)d->stream;
     const long slots = parts_slots(d->rows, d->n_seqs, a.parts.L);
     const dim3 grid((unsigned)slots, (unsigned)channel_blocks(d));
+    if (a.order) {
+        hipLaunchKernelGGL(k_order, dim3(1), dim3(1024), 0, st, a.parts, const_cast<int*>(a.order));
+        PSH_HIP(c, hipGetLastError());
+    }
     if (a.carry) {
         hipLaunchKernelGGL((k_scan_grad<T, NP, LPC, true>), grid, dim3(THREADS), 0, st, a);
         PSH_HIP(c, hipGetLastError());
@@ -1046,9 +1168,11 @@ template <class T> int run_scan(psh_ctx* c, const psh_scan_desc* d) {
         return PSH_OK;
     }
     const ScanSpace s = scan_space(d, false);
+    unsigned char* const at = (unsigned char*)d->workspace + s.order;
+    if (s.order) a.order = (const int*)d->workspace;
     if (s.carry) {
-        a.carry = (W*)d->workspace;
-        a.carry_dt = (W*)((unsigned char*)d->workspace + s.carry);
+        a.carry = (W*)at;
+        a.carry_dt = (W*)(at + s.carry);
     }
     scan_alignment(a, false);
 #define PSH_CALL(NP, LPC) scan_forward<T, NP, LPC>(c, d, a)
@@ -1060,7 +1184,8 @@ template <class T> int run_scan_grad(psh_ctx* c, const psh_scan_desc* d) {
     hipStream_t st = (hipStream_t)d->stream;
     ScanArgs<T> a = scan_args<T>(d);
     const ScanSpace s = scan_space(d, true);
-    unsigned char* at = (unsigned char*)d->workspace;
+    unsigned char* at = (unsigned char*)d->workspace + s.order;
+    if (s.order) a.order = (const int*)d->workspace;
     if (s.carry) {
         a.carry = (W*)at;
         a.carry_dt = (W*)(at + s.carry);
@@ -1128,10 +1253,12 @@ int lanes_for(int D, int V) {
     while (n < 64 && n * V < D) n *= 2;
     return n;
 }
+// channels of a lane: 16 bytes, for bf16 gradients 8 (8 channels' windows, sums and weights take 174 registers, 4 channels' 98)
+constexpr int conv_wide(int elem, bool grad) { return grad && elem == 2 ? 4 : 16 / elem; }
 int conv_vec(const psh_conv_desc* d, bool grad) {
-    const int e = elem_size(d->dtype), V = 16 / e;
-    const bool ok = d->channels % V == 0 && aligned(d->x, 16, d->ld_x * e) &&
-                    (grad ? aligned(d->dy, 16, d->ld_dy * e) && aligned(d->dx, 16, 0) : aligned(d->y, 16, 0));
+    const int e = elem_size(d->dtype), V = conv_wide(e, grad);
+    const bool ok = d->channels % V == 0 && aligned(d->x, V * e, d->ld_x * e) &&
+                    (grad ? aligned(d->dy, V * e, d->ld_dy * e) && aligned(d->dx, V * e, 0) : aligned(d->y, V * e, 0));
     return ok ? V : 1;
 }
 int64_t conv_piece(const psh_conv_desc* d, int V, bool grad) {
@@ -1143,7 +1270,7 @@ ConvSpace conv_space(const psh_conv_desc* d) {
     if (d->dweight || d->dbias) {
         // the wide and the one-element lane layouts cut pieces of different lengths: room for either
         for (int k = 0; k < 2; ++k) {
-            const int64_t slots = parts_slots(d->rows, d->n_seqs, conv_piece(d, k ? 1 : 16 / elem_size(d->dtype), true));
+            const int64_t slots = parts_slots(d->rows, d->n_seqs, conv_piece(d, k ? 1 : conv_wide(elem_size(d->dtype), true), true));
             const int64_t cols = (int64_t)d->channels * (d->taps + 1) * wide_size(d->dtype);
             const int64_t part = align256(slots * cols), mid = align256(join_segs(slots, d->n_policies) * cols);
             if (part > s.part) s.part = part;
@@ -1156,7 +1283,7 @@ ConvSpace conv_space(const psh_conv_desc* d) {
 
 template <class T, int K> int run_conv(psh_ctx* c, const psh_conv_desc* d, bool grad) {
     typedef typename Wide<T>::type W;
-    constexpr int VW = 16 / sizeof(T);
+    constexpr int VW = conv_wide(sizeof(T), false), VG = conv_wide(sizeof(T), true);
     hipStream_t st = (hipStream_t)d->stream;
     ConvArgs<T> a{};
     a.pol = Policies{d->groups, d->groups ? d->n_policies : 1, d->n_seqs};
@@ -1192,7 +1319,7 @@ template <class T, int K> int run_conv(psh_ctx* c, const psh_conv_desc* d, bool 
     a.dx = (T*)d->dx; a.dstate = K > 1 ? (T*)d->dstate : nullptr;
     const ConvSpace s = conv_space(d);
     if (s.part) a.part = (W*)d->workspace;
-    if (V > 1) hipLaunchKernelGGL((k_conv_grad<T, VW, K>), grid, dim3(256), 0, st, a, slots);
+    if (V > 1) hipLaunchKernelGGL((k_conv_grad<T, VG, K>), grid, dim3(256), 0, st, a, slots);
     else hipLaunchKernelGGL((k_conv_grad<T, 1, K>), grid, dim3(256), 0, st, a, slots);
     PSH_HIP(c, hipGetLastError());
     if (a.part) {

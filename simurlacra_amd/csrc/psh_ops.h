@@ -47,8 +47,18 @@ template <class W> PSH_OP W silu_w(W x) { return x * sigmoid_w(x); }
 // d/dx of x sigmoid(x) from s = sigmoid(x)
 template <class W> PSH_OP W silu_slope_w(W x, W s) { return s * (W(1) + x * (W(1) - s)); }
 // log(1 + e^x) = max(x, 0) + log1p(e^-|x|).  log1p keeps the digits of a small e, where the step sizes of a slow memory are.
-PSH_OP float softplus_w(float x) { return fmaxf(x, 0.f) + (x != x ? x : log1pf(exp_w(-fabsf(x)))); }
-PSH_OP double softplus_w(double x) { return fmax(x, 0.) + (x != x ? x : log1p(psh_exp(-fabs(x)))); }
+// By hand: w = 1 + e rounds, and e - (w - 1) is what that lost, exactly; it goes back in front of log's slope
+// 1 / w, which is 1 where it matters (for e near 1 the lost part is below half a ulp of the result anyway).
+PSH_OP float softplus_w(float x) {
+    const float e = exp_w(-fabsf(x)), w = 1.f + e;
+    const float l = __builtin_amdgcn_logf(w) * (float)PSH_LN2 + (e - (w - 1.f));
+    return x != x ? x : fmaxf(x, 0.f) + l;
+}
+PSH_OP double softplus_w(double x) {
+    const double e = psh_exp(-fabs(x)), w = 1. + e;
+    const double l = psh_log_normal(x != x ? 1. : w) + (e - (w - 1.));
+    return x != x ? x : fmax(x, 0.) + l;
+}
 PSH_OP float tanh_w(float x) { return tanhf(x); }
 PSH_OP double tanh_w(double x) { return psh_tanh(x); }
 
