@@ -52,8 +52,14 @@ template <class T> struct Operand {
     const T* p;
     long ld;
     int n, nc;      // valid indices and valid c
-    bool wide;      // 16-byte loads are aligned
 };
+
+// 16 bytes at any element: the hardware takes unaligned global loads
+template <class T> PSH_OP v4u load16(const T* p) {
+    v4u v;
+    __builtin_memcpy(&v, p, 16);
+    return v;
+}
 
 template <class T> PSH_OP int unit_of(int i, int u) { return u ^ ((i ^ (i >> 3)) & 7); }
 
@@ -69,7 +75,7 @@ template <class T, int N, int THREADS, bool TR> struct Stager {
     static PSH_OP v4u load(const Operand<T>& o, const T* q, int first, int limit) {
         // elements [first, first + V) of a line with `limit` valid ones
         if (first >= limit) return v4u{0, 0, 0, 0};
-        if (o.wide && first + V <= limit) return *reinterpret_cast<const v4u*>(q + first);
+        if (first + V <= limit) return load16(q + first);
         T e[V];
 #pragma unroll
         for (int k = 0; k < V; ++k) e[k] = first + k < limit ? q[first + k] : T(0);
@@ -115,6 +121,68 @@ template <class T, int N, int THREADS, bool TR> struct Stager {
                     *reinterpret_cast<v4u*>(lds + i * 128 + unit_of<T>(i, u) * 16) = __builtin_bit_cast(v4u, e);
                 }
             }
+        }
+    }
+};
+
+// A bf16 operand's tiles by loads that go to LDS directly: no registers, no transposing on the way in.  The tile lies as it is in memory, [index][64 c]
+// or, for a transposed operand, [64 c][index], where ds_read_b64_tr_b16 does the transposing: 16 lanes, four to a row of 16 indices, read 4
+// rows, and lane i gets column i.  The loads go to LDS in lane order, so the permutation that spreads the banks is applied
+// to the addresses they read from: 16-byte units by the index as in Stager, or 32-byte chunks of a row by (c ^ c / 8) & 7.
+// Rows past the operand's end are read as its last one (their results are not stored); only whole tiles of c come this way.
+template <int N, int THREADS, bool TR> struct Direct {
+    static constexpr int WAVES = THREADS / 64, PER = N * 128 / 1024 / WAVES;   // 1-KiB loads of a wave
+    static constexpr int ROW = N * 2, SWZ = N >= 128 ? 7 : 3;                  // transposed: bytes and permutation of a row
+    static PSH_OP int swz(int c) { return (c ^ (c >> 3)) & SWZ; }
+    static PSH_OP void fetch(const Operand<bf16_t>& o, int c0, unsigned lds) {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            const int chunk = __builtin_amdgcn_readfirstlane(wave + k * WAVES);
+            const bf16_t* g;
+            if constexpr (!TR) {
+                const int i = chunk * 8 + (lane >> 3), u = (lane & 7) ^ ((i ^ (i >> 3)) & 7);
+                g = o.p + (long)min(i, o.n - 1) * o.ld + c0 + u * 8;
+            } else {
+                const int at = chunk * 1024 + lane * 16, c = at / ROW, u = (at % ROW / 16) ^ (swz(c) << 1);
+                g = o.p + (long)(c0 + c) * o.ld + min(u * 8, o.n - 8);
+            }
+            // (by hand, because the compiler would wait for a builtin's load before the next read of any part of LDS; the
+            // wait is in front of the barrier that ends the tile)
+            asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds + chunk * 1024), "v"(g) : "memory");
+        }
+    }
+    // the last, partial tile of c through registers, zero where there is none
+    static PSH_OP void fetch_tail(const Operand<bf16_t>& o, int c0, unsigned char* lds) {
+        if constexpr (!TR) {
+            Stager<bf16_t, N, THREADS, false> st;
+            st.fetch(o, c0);
+            st.store(lds);
+        } else {
+            for (int at = threadIdx.x * 16; at < N * 128; at += THREADS * 16) {
+                const int c = at / ROW, u = (at % ROW / 16) ^ (swz(c) << 1);
+                *reinterpret_cast<v4u*>(lds + at) =
+                    c0 + c < o.nc ? load16(o.p + (long)(c0 + c) * o.ld + min(u * 8, o.n - 8)) : v4u{0, 0, 0, 0};
+            }
+        }
+    }
+    // 16 bytes along c for the index i0 + (lane & 15): c from s * 32 + (lane / 16) * 8
+    static PSH_OP v4u fragment(unsigned char* lds, int i0, int s) {
+        const int l = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
+        if constexpr (!TR) {
+            const int i = i0 + l;
+            return *reinterpret_cast<const v4u*>(lds + i * 128 + (((s * 4 + g) ^ (i ^ (i >> 3))) & 7) * 16);
+        } else {
+            typedef short v4s __attribute__((ext_vector_type(4)));
+            typedef __attribute__((address_space(3))) v4s* at_t;
+            uint2 h[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int c = s * 32 + g * 8 + k * 4 + (l >> 2);
+                unsigned char* const at = lds + c * ROW + (((i0 >> 4) ^ swz(c)) * 32) + (l & 3) * 8;
+                h[k] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((at_t)at));
+            }
+            return v4u{h[0].x, h[0].y, h[1].x, h[1].y};
         }
     }
 };
@@ -188,6 +256,57 @@ template <class T, int BI, int BJ, int WI, int WJ> struct Tile {
         }
     }
 
+    // the same for bf16 by direct loads
+    template <bool TP, bool TQ, bool SUMS> PSH_OP void multiply_direct(const Operand<bf16_t>& p, const Operand<bf16_t>& q, unsigned char* lds) {
+        typedef Direct<BI, THREADS, TP> DP;
+        typedef Direct<BJ, THREADS, TQ> DQ;
+        const int wave = threadIdx.x >> 6;
+        const int wi = (wave % WI) * (BI / WI), wj = (wave / WI) * (BJ / WJ);
+#pragma unroll
+        for (int a = 0; a < MI; ++a) {
+            ones[a] = acc_t{0, 0, 0, 0};
+#pragma unroll
+            for (int b = 0; b < MJ; ++b) acc[a][b] = acc_t{0, 0, 0, 0};
+        }
+        v4u unit = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};   // eight ones
+        const int nc = p.nc, tiles = (nc + 63) / 64, whole = nc / 64;
+        if (tiles <= 0) return;
+        const unsigned base = (unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)lds;
+        constexpr unsigned BUF = (BI + BJ) * 128;
+        const auto bring = [&](int t, unsigned buf) {
+            if (t < whole) {
+                DP::fetch(p, t * 64, base + buf);
+                DQ::fetch(q, t * 64, base + buf + BI * 128);
+            } else {
+                DP::fetch_tail(p, t * 64, lds + buf);
+                DQ::fetch_tail(q, t * 64, lds + buf + BI * 128);
+            }
+        };
+        bring(0, 0);
+        asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+        __syncthreads();
+        for (int t = 0; t < tiles; ++t) {
+            const unsigned cur = (t & 1) * BUF, nxt = BUF - cur;
+            if (t + 1 < tiles) bring(t + 1, nxt);
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                v4u fp[MI], fq[MJ];
+#pragma unroll
+                for (int a = 0; a < MI; ++a) fp[a] = DP::fragment(lds + cur, wi + a * 16, s);
+#pragma unroll
+                for (int b = 0; b < MJ; ++b) fq[b] = DQ::fragment(lds + cur + BI * 128, wj + b * 16, s);
+#pragma unroll
+                for (int a = 0; a < MI; ++a) {
+#pragma unroll
+                    for (int b = 0; b < MJ; ++b) Mfma<T>::step(fp[a], fq[b], acc[a][b]);
+                    if constexpr (SUMS) Mfma<T>::step(fp[a], unit, ones[a]);
+                }
+            }
+            asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+            __syncthreads();
+        }
+    }
+
     // f(i, j, v[4]) for the results of this lane: units i .. i + 3 of row j for fp32 accumulators; for fp64 ones the
     // four units are i, i + 4, i + 8, i + 12
     template <class F> PSH_OP void each(F f) {
@@ -215,7 +334,7 @@ template <class T> struct RowsArgs {   // forward and dx
     T* out;                            // [rows, n_out] contiguous
     int n_in, n_out, nonlin;
     long slots, tiles_i;
-    bool wide_in, wide_w, wide_out;
+    bool wide_out;
 };
 
 // store up to four units of one row
@@ -237,7 +356,7 @@ template <class T, class A> PSH_OP void store_units(T* row, int i, int n, const 
     }
 }
 
-template <class T, int BI, int BJ, int WI, int WJ, bool TW>
+template <class T, int BI, int BJ, int WI, int WJ, bool TW, bool DIRECT>
 __global__ __launch_bounds__(64 * WI * WJ) void k_rows(const RowsArgs<T> a) {
     extern __shared__ __align__(16) unsigned char lds[];
     const long id = xcd_order(blockIdx.x, a.slots * a.tiles_i);
@@ -251,10 +370,11 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_rows(const RowsArgs<T> a) {
         return;
     }
     const T* const w = a.weight + (long)q.part * a.stride_w;
-    const Operand<T> p{TW ? w + i0 : w + (long)i0 * a.ld_w, a.ld_w, ni, a.n_in, a.wide_w};
-    const Operand<T> x{a.rows_in + (long)q.begin * a.ld_in, a.ld_in, nj, a.n_in, a.wide_in};
+    const Operand<T> p{TW ? w + i0 : w + (long)i0 * a.ld_w, a.ld_w, ni, a.n_in};
+    const Operand<T> x{a.rows_in + (long)q.begin * a.ld_in, a.ld_in, nj, a.n_in};
     Tile<T, BI, BJ, WI, WJ> tile;
-    tile.template multiply<TW, false, false>(p, x, lds);
+    if constexpr (DIRECT) tile.template multiply_direct<TW, false, false>(p, x, lds);
+    else tile.template multiply<TW, false, false>(p, x, lds);
     typedef typename Wide<T>::type W;
     const T* const b = a.bias ? a.bias + (long)q.part * a.stride_b + i0 : nullptr;
     tile.each([&](int i, int j, auto v) {
@@ -288,10 +408,9 @@ template <class T> struct GradArgs {   // dW, db
     typename Wide<T>::type* part_b;
     int n, k;
     long slots, tiles_i, tiles_j;
-    bool wide_dp, wide_x, wide_out;
 };
 
-template <class T, int BI, int BJ, int WI, int WJ>
+template <class T, int BI, int BJ, int WI, int WJ, bool DIRECT>
 __global__ __launch_bounds__(64 * WI * WJ) void k_weights(const GradArgs<T> a) {
     extern __shared__ __align__(16) unsigned char lds[];
     const long tiles = a.tiles_i * a.tiles_j, total = a.slots * tiles;
@@ -302,13 +421,18 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_weights(const GradArgs<T> a) {
     if (q.part >= a.parts.n || (q.j > 0 && q.begin >= q.end)) return;
     const int i0 = (int)(id % tiles / a.tiles_j) * BI, j0 = (int)(id % a.tiles_j) * BJ;
     const int ni = min(BI, a.n - i0), nj = min(BJ, a.k - j0), rows = max(0, q.end - q.begin);
-    const Operand<T> p{a.dp + (long)q.begin * a.ld_dp + i0, a.ld_dp, ni, rows, a.wide_dp};
-    const Operand<T> x{a.x + (long)q.begin * a.ld_x + j0, a.ld_x, nj, rows, a.wide_x};
+    const Operand<T> p{a.dp + (long)q.begin * a.ld_dp + i0, a.ld_dp, ni, rows};
+    const Operand<T> x{a.x + (long)q.begin * a.ld_x + j0, a.ld_x, nj, rows};
     Tile<T, BI, BJ, WI, WJ> tile;
     const bool whole = q.part_end - q.part_begin <= a.parts.L;   // no other piece: the result itself
     const bool sums = j0 == 0 && a.db;
-    if (sums) tile.template multiply<true, true, true>(p, x, lds);
-    else tile.template multiply<true, true, false>(p, x, lds);
+    if constexpr (DIRECT) {
+        if (sums) tile.template multiply_direct<true, true, true>(p, x, lds);
+        else tile.template multiply_direct<true, true, false>(p, x, lds);
+    } else {
+        if (sums) tile.template multiply<true, true, true>(p, x, lds);
+        else tile.template multiply<true, true, false>(p, x, lds);
+    }
     constexpr int step = sizeof(T) == 8 ? 4 : 1;
     const long at = (long)(whole ? q.part : slot) * a.n;
     if (a.dw) tile.each([&](int i, int j, auto v) {
@@ -354,7 +478,7 @@ template <class T> __global__ __launch_bounds__(256) void k_join(const GradArgs<
     }
 }
 
-inline bool wide_ok(const void* p, int size, int64_t ld, int64_t stride = 0) {
+inline bool aligned16(const void* p, int size, int64_t ld, int64_t stride = 0) {
     return ((uintptr_t)p & 15) == 0 && (ld * size) % 16 == 0 && (stride * size) % 16 == 0;
 }
 
@@ -363,14 +487,14 @@ template <class K> int allow_lds(psh_ctx* c, K kernel, int bytes) {
     return PSH_OK;
 }
 
-template <class T, int BI, int BJ, int WI, int WJ, bool TW> int launch_rows(psh_ctx* c, RowsArgs<T>& a, int rows, hipStream_t st) {
+template <class T, int BI, int BJ, int WI, int WJ, bool TW, bool DIRECT> int launch_rows(psh_ctx* c, RowsArgs<T>& a, int rows, hipStream_t st) {
     a.parts.L = BJ;
     a.slots = parts_slots(rows, a.parts.n, BJ);
     a.tiles_i = (a.n_out + BI - 1) / BI;
     const long total = (a.slots * a.tiles_i + 7) / 8 * 8;
     if (total > 0x7fffffffL) { set_err(c, "grouped_linear: too many tiles for one launch"); return PSH_ERR_UNSUPPORTED; }
     constexpr int lds = 2 * (BI + BJ) * 128;
-    const auto kernel = k_rows<T, BI, BJ, WI, WJ, TW>;
+    const auto kernel = k_rows<T, BI, BJ, WI, WJ, TW, DIRECT>;
     const int rc = allow_lds(c, kernel, lds);
     if (rc != PSH_OK) return rc;
     hipLaunchKernelGGL(kernel, dim3((unsigned)total), dim3(64 * WI * WJ), lds, st, a);
@@ -378,13 +502,34 @@ template <class T, int BI, int BJ, int WI, int WJ, bool TW> int launch_rows(psh_
     return PSH_OK;
 }
 
+// Tiles [units][rows].  Large ones re-read the operands less often, small ones waste less where a group has few rows or a layer few
+// units, and there are more of them to fill the CUs.
 template <class T, bool TW> int run_rows(psh_ctx* c, RowsArgs<T>& a, int rows, hipStream_t st) {
-    return launch_rows<T, 64, 64, 2, 2, TW>(c, a, rows, st);
+    const long mean = rows / a.parts.n;
+    if (mean <= 24) return launch_rows<T, 64, 16, 4, 1, TW, false>(c, a, rows, st);
+    if constexpr (sizeof(T) < 8) {
+        const long large = ((long)rows / 128 + a.parts.n / 2) * ((a.n_out + 127) / 128);
+        if (mean >= 96 && a.n_out > 64 && large >= 192) {
+            if constexpr (sizeof(T) == 2) {
+                const bool direct = aligned16(a.rows_in, 2, a.ld_in) && aligned16(a.weight, 2, a.ld_w, a.stride_w) && (!TW || a.n_out % 8 == 0);
+                if (direct) return launch_rows<T, 128, 128, 2, 2, TW, true>(c, a, rows, st);
+            }
+            return launch_rows<T, 128, 128, 2, 2, TW, false>(c, a, rows, st);
+        }
+    }
+    return launch_rows<T, 64, 64, 2, 2, TW, false>(c, a, rows, st);
 }
 
-// rows of one piece of the weight gradient's contraction
+// the weight gradient's tile: [out units][in units]
+int grad_tile(const psh_linear_desc* d) {
+    if (d->dtype == PSH_F64 || d->out_dim <= 64 || d->in_dim <= 64) return 64;
+    const int64_t tiles = (int64_t)((d->out_dim + 127) / 128) * ((d->in_dim + 127) / 128);
+    return tiles * (d->rows / 2048 + d->n_groups) >= 192 ? 128 : 64;
+}
+// rows of one piece of the weight gradient's contraction: enough pieces for about four workgroups a CU
 int64_t grad_piece(const psh_linear_desc* d) {
-    const int64_t tiles = (int64_t)((d->out_dim + 63) / 64) * ((d->in_dim + 63) / 64);
+    const int t = grad_tile(d);
+    const int64_t tiles = (int64_t)((d->out_dim + t - 1) / t) * ((d->in_dim + t - 1) / t);
     const int64_t whole = ((int64_t)d->rows + 64) / 64 * 64;
     if (tiles >= 512) return whole;
     int64_t L = ((int64_t)d->rows * tiles / 1024 + 63) / 64 * 64;
@@ -432,6 +577,21 @@ int check(psh_ctx* c, const psh_linear_desc* d, bool grad) {
     return PSH_OK;
 }
 
+template <class T, int B, int WI, int WJ, bool DIRECT> int launch_weights(psh_ctx* c, GradArgs<T>& a, int rows, hipStream_t st) {
+    a.slots = parts_slots(rows, a.parts.n, a.parts.L);
+    a.tiles_i = (a.n + B - 1) / B;
+    a.tiles_j = a.dw ? (a.k + B - 1) / B : 1;
+    const long total = (a.slots * a.tiles_i * a.tiles_j + 7) / 8 * 8;
+    if (total > 0x7fffffffL) { set_err(c, "grouped_linear_grad: too many tiles for one launch"); return PSH_ERR_UNSUPPORTED; }
+    constexpr int lds = 4 * B * 128;
+    const auto kernel = k_weights<T, B, B, WI, WJ, DIRECT>;
+    const int rc = allow_lds(c, kernel, lds);
+    if (rc != PSH_OK) return rc;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)total), dim3(64 * WI * WJ), lds, st, a);
+    PSH_HIP(c, hipGetLastError());
+    return PSH_OK;
+}
+
 template <class T> int forward(psh_ctx* c, const psh_linear_desc* d) {
     RowsArgs<T> a{};
     a.parts = Parts{d->offsets, d->n_groups, d->rows, 0};
@@ -440,9 +600,7 @@ template <class T> int forward(psh_ctx* c, const psh_linear_desc* d) {
     a.bias = (const T*)d->bias; a.stride_b = d->stride_b;
     a.out = (T*)d->y;
     a.n_in = d->in_dim; a.n_out = d->out_dim; a.nonlin = d->nonlin;
-    a.wide_in = wide_ok(d->x, sizeof(T), d->ld_x);
-    a.wide_w = wide_ok(d->weight, sizeof(T), d->ld_w, d->stride_w);
-    a.wide_out = wide_ok(d->y, sizeof(T), 4) && d->out_dim % 4 == 0;
+    a.wide_out = aligned16(d->y, sizeof(T), 4) && d->out_dim % 4 == 0;
     return run_rows<T, false>(c, a, d->rows, (hipStream_t)d->stream);
 }
 
@@ -469,9 +627,7 @@ template <class T> int backward(psh_ctx* c, const psh_linear_desc* d) {
         a.weight = (const T*)d->weight; a.ld_w = d->ld_w; a.stride_w = d->stride_w;
         a.out = (T*)d->dx;
         a.n_in = d->out_dim; a.n_out = d->in_dim; a.nonlin = PSH_NL_NONE;
-        a.wide_in = wide_ok(dp, sizeof(T), ld_dp);
-        a.wide_w = wide_ok(d->weight, sizeof(T), d->ld_w, d->stride_w);
-        a.wide_out = wide_ok(d->dx, sizeof(T), 4) && d->in_dim % 4 == 0;
+        a.wide_out = aligned16(d->dx, sizeof(T), 4) && d->in_dim % 4 == 0;
         const int rc = run_rows<T, true>(c, a, d->rows, st);
         if (rc != PSH_OK) return rc;
     }
@@ -483,15 +639,18 @@ template <class T> int backward(psh_ctx* c, const psh_linear_desc* d) {
         a.dw = (T*)d->dweight; a.db = (T*)d->dbias;
         a.part_w = (W*)(space + s.dp); a.part_b = (W*)(space + s.dp + s.part_w);
         a.n = d->out_dim; a.k = d->in_dim;
-        a.wide_dp = wide_ok(dp, sizeof(T), ld_dp);
-        a.wide_x = wide_ok(d->x, sizeof(T), d->ld_x);
-        a.slots = parts_slots(d->rows, d->n_groups, a.parts.L);
-        a.tiles_i = (a.n + 63) / 64;
-        a.tiles_j = d->dweight ? (a.k + 63) / 64 : 1;
-        const long total = (a.slots * a.tiles_i * a.tiles_j + 7) / 8 * 8;
-        if (total > 0x7fffffffL) { set_err(c, "grouped_linear_grad: too many tiles for one launch"); return PSH_ERR_UNSUPPORTED; }
-        hipLaunchKernelGGL((k_weights<T, 64, 64, 2, 2>), dim3((unsigned)total), dim3(256), 2 * 128 * 128, st, a);
-        PSH_HIP(c, hipGetLastError());
+        int rc;
+        if constexpr (sizeof(T) == 8) {
+            rc = launch_weights<T, 64, 2, 2, false>(c, a, d->rows, st);
+        } else if (grad_tile(d) == 64) {
+            rc = launch_weights<T, 64, 2, 2, false>(c, a, d->rows, st);
+        } else if constexpr (sizeof(T) == 2) {
+            const bool direct = aligned16(dp, 2, ld_dp) && aligned16(d->x, 2, d->ld_x) && a.n % 8 == 0 && a.k % 8 == 0;
+            rc = direct ? launch_weights<T, 128, 2, 2, true>(c, a, d->rows, st) : launch_weights<T, 128, 2, 2, false>(c, a, d->rows, st);
+        } else {
+            rc = launch_weights<T, 128, 2, 2, false>(c, a, d->rows, st);
+        }
+        if (rc != PSH_OK) return rc;
         if (s.part_w + s.part_b > 0) {
             const long n = (long)a.n * (a.k + 1);
             const unsigned bx = (unsigned)((n + 255) / 256 < 1024 ? (n + 255) / 256 : 1024);

@@ -315,7 +315,7 @@ template <class W> struct JoinArgs {
     const W* part; W* mid;
     W *out0, *out1, *out2;    // columns [0, n0) -> out0, then n1 -> out1, then n2 -> out2 (NULL: not wanted)
     long n0, n1, n2, split;   // split: column layout [.., split + 1] with the last of each row going to out1 (0: plain)
-    int seg;
+    int seg;                  // 0: few enough slots for one pass over `part`
     PSH_OP int slot_of(int p) const { return p >= pol.n ? parts.first_slot(parts.n) : parts.first_slot(pol.at(p)); }
     PSH_OP int seg_of(int p) const { return slot_of(p) / seg + p; }
 };
@@ -329,17 +329,34 @@ template <class W> __global__ __launch_bounds__(256) void k_join_mid(const JoinA
     const long stop = begin + a.seg < end ? begin + a.seg : end;
     if (begin >= end && seg != a.seg_of(p)) return;
     W s = 0;
-    for (long k = begin; k < stop; ++k) s += a.part[k * cols + m];
+    long k = begin;
+    for (; k + 8 <= stop; k += 8) {
+        W v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = a.part[(k + i) * cols + m];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s += v[i];
+    }
+    for (; k < stop; ++k) s += a.part[k * cols + m];
     a.mid[(long)seg * cols + m] = s;
 }
 template <class W> __global__ __launch_bounds__(256) void k_join_out(const JoinArgs<W> a) {
     const int p = blockIdx.x;
     const long m = (long)blockIdx.y * 256 + threadIdx.x, cols = a.n0 + a.n1 + a.n2;
     if (m >= cols) return;
-    const int slots = a.slot_of(p + 1) - a.slot_of(p), first = a.seg_of(p);
-    const int n = slots <= 0 ? 0 : (slots + a.seg - 1) / a.seg;
+    const int slots = max(0, a.slot_of(p + 1) - a.slot_of(p)), first = a.seg ? a.seg_of(p) : a.slot_of(p);
+    const int n = a.seg ? (slots + a.seg - 1) / a.seg : slots;
+    const W* const mid = a.seg ? a.mid : a.part;
     W s = 0;
-    for (int k = 0; k < n; ++k) s += a.mid[(long)(first + k) * cols + m];
+    int k0 = 0;
+    for (; k0 + 8 <= n; k0 += 8) {
+        W v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = mid[(long)(first + k0 + i) * cols + m];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s += v[i];
+    }
+    for (; k0 < n; ++k0) s += mid[(long)(first + k0) * cols + m];
     if (a.split) {   // convolution: [D, K + 1] rows of weights and a bias
         const long d = m / (a.split + 1), k = m - d * (a.split + 1);
         if (k < a.split) { if (a.out0) a.out0[(long)p * (cols / (a.split + 1)) * a.split + d * a.split + k] = s; }
@@ -359,8 +376,14 @@ int join_seg(long slots) {
 }
 long join_segs(long slots, int policies) { return slots / join_seg(slots) + policies + 1; }
 template <class W> int run_join(psh_ctx* c, JoinArgs<W>& a, long slots, hipStream_t st) {
-    a.seg = join_seg(slots);
     const unsigned by = (unsigned)((a.n0 + a.n1 + a.n2 + 255) / 256);
+    a.seg = 0;
+    if (slots <= 96 * (long)a.pol.n) {   // one pass of a few dozen loads, eight in flight, is done before a second launch would begin
+        hipLaunchKernelGGL(k_join_out<W>, dim3((unsigned)a.pol.n, by), dim3(256), 0, st, a);
+        PSH_HIP(c, hipGetLastError());
+        return PSH_OK;
+    }
+    a.seg = join_seg(slots);
     hipLaunchKernelGGL(k_join_mid<W>, dim3((unsigned)join_segs(slots, a.pol.n), by), dim3(256), 0, st, a);
     PSH_HIP(c, hipGetLastError());
     hipLaunchKernelGGL(k_join_out<W>, dim3((unsigned)a.pol.n, by), dim3(256), 0, st, a);
@@ -397,7 +420,8 @@ template <class T> struct ScanArgs {
     W* check;                // [rows / TS + n + 1, D, N] states before every tile
     W* carry;                // [slots, D, N]: states (adjoint states) at the pieces' beginnings (ends), NULL: pieces are whole sequences
     W* carry_dt;             // [slots, D]
-    const int* order;        // slot of every workgroup, NULL: its number
+    const int* order;        // sequences from the longest to the shortest, NULL: as they come
+    int blocks;              // channel blocks
     bool vec_d, vec_n;       // wide loads of channel rows / of states
     // gradients
     const T* dy; long ld_dy;
@@ -569,6 +593,23 @@ __global__ __launch_bounds__(1024) void k_order(const Parts p, int* order) {
     for (int s = tid; s < p.n; s += 1024) order[atomicAdd(&count[255 - min(255, (int)((float)max(0, p.at(s + 1) - p.at(s)) * scale))], 1)] = s;
 }
 
+// Which slot and channel block a workgroup works on.  In an ordered launch work item k is channel block k % blocks of the (k / blocks)-th
+// longest sequence, and workgroup i takes item i in even, the mirrored one in odd runs of 256: workgroups go round the
+// CUs, so a CU that got the longest of one run gets the shortest of the next.
+template <class T> PSH_OP void work_of(const ScanArgs<T>& a, int& slot, int& block) {
+    const int blocks = a.blocks;
+    unsigned i = blockIdx.x;
+    const unsigned ordered = (unsigned)a.parts.n * blocks;
+    if (a.order && i < ordered) {
+        const unsigned run = i / 256, r = i % 256, len = min(256u, ordered - run * 256);
+        i = run & 1 ? run * 256 + len - 1 - r : i;
+        slot = a.order[i / blocks];
+    } else {
+        slot = (int)(i / blocks);
+    }
+    block = (int)(i % blocks);
+}
+
 // h_t along a piece.  CARRY: only the state at the piece's end from zero and the sum of its step sizes, for the joining
 // of pieces; otherwise y as well, from the state at the piece's beginning.
 template <class T, int NP, int LPC, bool CARRY> __global__ __launch_bounds__(THREADS) void k_scan(const ScanArgs<T> a) {
@@ -579,7 +620,9 @@ template <class T, int NP, int LPC, bool CARRY> __global__ __launch_bounds__(THR
     __shared__ __align__(16) W s_b[TS * NL];
     __shared__ __align__(16) W s_c[CARRY ? 1 : TS * NL];
     __shared__ __align__(16) W s_y[CARRY ? 1 : TS][CB];
-    const int slot = a.order && (int)blockIdx.x < a.parts.n ? a.order[blockIdx.x] : (int)blockIdx.x, c0 = (int)blockIdx.y * CB;
+    int slot, block;
+    work_of(a, slot, block);
+    const int c0 = block * CB;
     const Piece q = find_piece(a.parts, slot);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int ql = lane % LPC, cl = wave * (64 / LPC) + lane / LPC;     // lane of the channel, channel of the block
@@ -727,13 +770,16 @@ template <class T, int NP, int LPC, bool CARRY> __global__ __launch_bounds__(THR
     typedef Shape<W, NP, LPC> SH;
     constexpr int TS = SH::TS, CB = SH::CB, E = SH::E, NL = SH::NL;
     constexpr int NV = 2 * NP < 4 ? 4 : 2 * NP;     // gradients of B and C of a step and lane, padded
+    constexpr int GS = LPC < TS ? LPC : TS;         // steps whose sums the lanes of a channel collect, one each
     __shared__ Pair<W> s_dt[TS][CB];
     __shared__ __align__(16) W s_dy[TS][CB];
     __shared__ __align__(16) W s_sz[CARRY ? 1 : TS][CB], s_sd[CARRY ? 1 : TS][CB];   // sigmoids of z and of delta + bias
     __shared__ __align__(16) W s_b[TS * NL], s_c[TS * NL];
     __shared__ __align__(16) W s_1[CARRY ? 1 : TS][CB], s_2[CARRY ? 1 : TS][CB], s_y[CARRY ? 1 : TS][CB];
     __shared__ __align__(16) W s_bc[CARRY ? 1 : 4 * TS * 2 * NL];
-    const int slot = a.order && (int)blockIdx.x < a.parts.n ? a.order[blockIdx.x] : (int)blockIdx.x, c0 = (int)blockIdx.y * CB;
+    int slot, block;
+    work_of(a, slot, block);
+    const int c0 = block * CB;
     const Piece q = find_piece(a.parts, slot);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int ql = lane % LPC, cl = wave * (64 / LPC) + lane / LPC;
@@ -747,7 +793,7 @@ template <class T, int NP, int LPC, bool CARRY> __global__ __launch_bounds__(THR
                     if (a.ddelta) a.ddelta[(long)r * a.D + c] = T(0);
                     if (a.dz) a.dz[(long)r * a.D + c] = T(0);
                 }
-                for (int n = threadIdx.x; n < a.N && blockIdx.y == 0; n += THREADS) {
+                for (int n = threadIdx.x; n < a.N && block == 0; n += THREADS) {
                     if (a.dB) a.dB[(long)r * a.N + n] = T(0);
                     if (a.dC) a.dC[(long)r * a.N + n] = T(0);
                 }
@@ -829,10 +875,10 @@ template <class T, int NP, int LPC, bool CARRY> __global__ __launch_bounds__(THR
         } else {
             W av[TS][NP], hv[TS][NP];   // a_t and h_{t-1}
 #pragma unroll
-            for (int t1 = 0; t1 < TS; t1 += LPC < TS ? LPC : TS) {
+            for (int t1 = 0; t1 < TS; t1 += GS) {
                 W keep = 0;
 #pragma unroll
-                for (int t2 = 0; t2 < (LPC < TS ? LPC : TS); ++t2) {
+                for (int t2 = 0; t2 < GS; ++t2) {
                     const int t = t1 + t2;
                     const Pair<W> x = s_dt[t][cl];
                     W y = 0;
@@ -848,15 +894,15 @@ template <class T, int NP, int LPC, bool CARRY> __global__ __launch_bounds__(THR
                         keep = ql == t2 ? y : keep;
                     }
                     step_fence<W>();
+                    if (t2 % 4 == 3) __builtin_amdgcn_sched_barrier(0);   // (else every LDS read of the tile is hoisted to its top, into registers that it has not got)
                 }
-                if (a.z && ql < TS) s_y[t1 + ql][cl] = keep;
-                __builtin_amdgcn_sched_barrier(0);   // (else every LDS read of the tile is hoisted to its top, into registers that it has not got)
+                if (a.z && ql < GS) s_y[t1 + ql][cl] = keep;
             }
 #pragma unroll
-            for (int t1 = TS - (LPC < TS ? LPC : TS); t1 >= 0; t1 -= LPC < TS ? LPC : TS) {
+            for (int t1 = TS - GS; t1 >= 0; t1 -= GS) {
                 W keep1 = 0, keep2 = 0;
 #pragma unroll
-                for (int t2 = (LPC < TS ? LPC : TS) - 1; t2 >= 0; --t2) {
+                for (int t2 = GS - 1; t2 >= 0; --t2) {
                     const int t = t1 + t2;
                     const Pair<W> x = s_dt[t][cl];
                     const W dy = s_dy[t][cl];
@@ -894,12 +940,12 @@ template <class T, int NP, int LPC, bool CARRY> __global__ __launch_bounds__(THR
                             s_bc[((wave * TS + t) * 2 + k / NP) * NL + n0 + k % NP] = s;
                     }
                     step_fence<W>();
+                    if (t2 % 4 == 0) __builtin_amdgcn_sched_barrier(0);
                 }
-                if (ql < TS) {
+                if (ql < GS) {
                     s_1[t1 + ql][cl] = keep1;
                     s_2[t1 + ql][cl] = keep2;
                 }
-                __builtin_amdgcn_sched_barrier(0);
             }
             __syncthreads();
             const long row = r0 + ld.t;
@@ -931,7 +977,7 @@ template <class T, int NP, int LPC, bool CARRY> __global__ __launch_bounds__(THR
                     W s = 0;
 #pragma unroll
                     for (int w = 0; w < 4; ++w) s += s_bc[w * TS * 2 * NL + k];
-                    if (a.part_bc) a.part_bc[((long)blockIdx.y * a.parts.rows + r) * 2 * a.N + which * a.N + n] = s;
+                    if (a.part_bc) a.part_bc[((long)block * a.parts.rows + r) * 2 * a.N + which * a.N + n] = s;
                     else if (which ? a.dC : a.dB) (which ? a.dC : a.dB)[r * a.N + n] = to_elem<T>(s);
                 }
             }
@@ -1031,31 +1077,36 @@ template <class T> __global__ __launch_bounds__(256) void k_scan_step(const Scan
 
 // ====================================================================================================== host side
 int64_t tile_steps(int dtype) { return dtype == PSH_F64 ? 8 : 16; }
-int lanes_per_channel(int N) { return N <= 16 ? 4 : N <= 32 ? 8 : 16; }
-int channel_blocks(const psh_scan_desc* d) {
-    const int cb = THREADS / lanes_per_channel(d->states);
+// The gradient's registers hold a tile's decays and states, in fp64 twice as many: two states a lane there.
+int lanes_per_channel(const psh_scan_desc* d, bool grad) {
+    const int n = grad && d->dtype == PSH_F64 ? d->states * 2 : d->states;
+    return d->states <= 8 || n <= 16 ? 4 : n <= 32 ? 8 : 16;
+}
+int channel_blocks(const psh_scan_desc* d, bool grad) {
+    const int cb = THREADS / lanes_per_channel(d, grad);
     return (d->channels + cb - 1) / cb;
 }
 // Rows of a piece.  A step of the recurrence takes a wave about 200 cycles however many waves there are, so a launch wants 4 workgroups
 // for every CU before its steps are throughput and not latency.  Sequences that are too few for that are cut, down to 64
-// rows, at the price of a second pass over the decays (the exponentials are most of the work) and of joining the pieces.
-int64_t scan_piece(const psh_scan_desc* d) {
-    const int64_t ts = tile_steps(d->dtype), blocks = channel_blocks(d), whole = ((int64_t)d->rows + ts) / ts * ts;
-    if (d->n_seqs * blocks >= 768) return whole;
+// rows, at the price of a second pass over the decays (the exponentials are most of the work) and of joining the pieces;
+// short sequences (192 steps are 16 us) are not worth the two launches.
+int64_t scan_piece(const psh_scan_desc* d, bool grad) {
+    const int64_t ts = tile_steps(d->dtype), blocks = channel_blocks(d, grad), whole = ((int64_t)d->rows + ts) / ts * ts;
+    if (d->n_seqs * blocks >= 768 || d->rows <= 192 * (int64_t)d->n_seqs) return whole;
     int64_t L = (int64_t)d->rows * blocks / 1024 / ts * ts;
     if (L < 64) L = 64;
     return L < whole ? L : whole;
 }
-bool scan_split(const psh_scan_desc* d) { return scan_piece(d) < d->rows; }
-bool scan_ordered(const psh_scan_desc* d) { return !d->step && !scan_split(d) && d->n_seqs > 1 && d->n_seqs <= ORDER_MOST && d->rows > 64 * (int64_t)d->n_seqs; }
+bool scan_split(const psh_scan_desc* d, bool grad) { return scan_piece(d, grad) < d->rows; }
+bool scan_ordered(const psh_scan_desc* d, bool grad) { return !d->step && !scan_split(d, grad) && d->n_seqs > 1 && d->n_seqs <= ORDER_MOST && d->rows > 64 * (int64_t)d->n_seqs; }
 
 // (the order of the launch, if any, lies first)
 struct ScanSpace { int64_t order, carry, carry_dt, part, mid, bc, total; };
 ScanSpace scan_space(const psh_scan_desc* d, bool grad) {
     ScanSpace s{};
-    const int64_t slots = parts_slots(d->rows, d->n_seqs, scan_piece(d)), w = wide_size(d->dtype), D = d->channels, N = d->states;
-    if (scan_ordered(d)) s.order = align256((int64_t)d->n_seqs * 4);
-    if (scan_split(d)) {
+    const int64_t slots = parts_slots(d->rows, d->n_seqs, scan_piece(d, grad)), w = wide_size(d->dtype), D = d->channels, N = d->states;
+    if (scan_ordered(d, grad)) s.order = align256((int64_t)d->n_seqs * 4);
+    if (scan_split(d, grad)) {
         s.carry = align256(slots * D * N * w);
         s.carry_dt = align256(slots * D * w);
     }
@@ -1064,7 +1115,7 @@ ScanSpace scan_space(const psh_scan_desc* d, bool grad) {
             s.part = align256(slots * (D * N + 2 * D) * w);
             s.mid = align256(join_segs(slots, d->n_policies) * (D * N + 2 * D) * w);
         }
-        if ((d->dB || d->dC) && channel_blocks(d) > 1) s.bc = align256((int64_t)channel_blocks(d) * d->rows * 2 * N * w);
+        if ((d->dB || d->dC) && channel_blocks(d, true) > 1) s.bc = align256((int64_t)channel_blocks(d, true) * d->rows * 2 * N * w);
     }
     s.total = s.order + s.carry + s.carry_dt + s.part + s.mid + s.bc;
     return s;
@@ -1082,10 +1133,10 @@ int too_large(psh_ctx* c, const char* what) {
     return PSH_ERR_UNSUPPORTED;
 }
 
-template <class T> ScanArgs<T> scan_args(const psh_scan_desc* d) {
+template <class T> ScanArgs<T> scan_args(const psh_scan_desc* d, bool grad) {
     typedef typename Wide<T>::type W;
     ScanArgs<T> a{};
-    a.parts = Parts{d->offsets, d->n_seqs, d->rows, (int)scan_piece(d)};
+    a.parts = Parts{d->offsets, d->n_seqs, d->rows, (int)scan_piece(d, grad)};
     a.pol = Policies{d->groups, d->groups ? d->n_policies : 1, d->n_seqs};
     a.D = d->channels; a.N = d->states;
     a.u = (const T*)d->u; a.delta = (const T*)d->delta; a.z = (const T*)d->z; a.B = (const T*)d->B; a.C = (const T*)d->C;
@@ -1117,7 +1168,8 @@ template <class T> void scan_alignment(ScanArgs<T>& a, bool grad) {
 template <class T, int NP, int LPC> int scan_forward(psh_ctx* c, const psh_scan_desc* d, ScanArgs<T>& a) {
     hipStream_t st = (hipStream_t)d->stream;
     const long slots = parts_slots(d->rows, d->n_seqs, a.parts.L);
-    const dim3 grid((unsigned)slots, (unsigned)channel_blocks(d));
+    a.blocks = channel_blocks(d, false);
+    const dim3 grid((unsigned)(slots * a.blocks));
     if (a.order) {
         hipLaunchKernelGGL(k_order, dim3(1), dim3(1024), 0, st, a.parts, const_cast<int*>(a.order));
         PSH_HIP(c, hipGetLastError());
@@ -1135,7 +1187,8 @@ template <class T, int NP, int LPC> int scan_forward(psh_ctx* c, const psh_scan_
 template <class T, int NP, int LPC> int scan_backward(psh_ctx* c, const psh_scan_desc* d, ScanArgs<T>& a) {
     hipStream_t st = (hipStream_t)d->stream;
     const long slots = parts_slots(d->rows, d->n_seqs, a.parts.L);
-    const dim3 grid((unsigned)slots, (unsigned)channel_blocks(d));
+    a.blocks = channel_blocks(d, true);
+    const dim3 grid((unsigned)(slots * a.blocks));
     if (a.order) {
         hipLaunchKernelGGL(k_order, dim3(1), dim3(1024), 0, st, a.parts, const_cast<int*>(a.order));
         PSH_HIP(c, hipGetLastError());
@@ -1156,7 +1209,7 @@ template <class T, int NP, int LPC> int scan_backward(psh_ctx* c, const psh_scan
 template <class T> int run_scan(psh_ctx* c, const psh_scan_desc* d) {
     typedef typename Wide<T>::type W;
     hipStream_t st = (hipStream_t)d->stream;
-    ScanArgs<T> a = scan_args<T>(d);
+    ScanArgs<T> a = scan_args<T>(d, false);
     if (d->step) {
         a.check = nullptr;
         scan_alignment(a, false);
@@ -1182,7 +1235,7 @@ template <class T> int run_scan(psh_ctx* c, const psh_scan_desc* d) {
 template <class T> int run_scan_grad(psh_ctx* c, const psh_scan_desc* d) {
     typedef typename Wide<T>::type W;
     hipStream_t st = (hipStream_t)d->stream;
-    ScanArgs<T> a = scan_args<T>(d);
+    ScanArgs<T> a = scan_args<T>(d, true);
     const ScanSpace s = scan_space(d, true);
     unsigned char* at = (unsigned char*)d->workspace + s.order;
     if (s.order) a.order = (const int*)d->workspace;
@@ -1197,14 +1250,18 @@ template <class T> int run_scan_grad(psh_ctx* c, const psh_scan_desc* d) {
     at += s.mid;
     if (s.bc) a.part_bc = (W*)at;
     scan_alignment(a, true);
+    int rc;
 #define PSH_CALL(NP, LPC) scan_backward<T, NP, LPC>(c, d, a)
-    const int rc = PSH_FOR_STATES(a.N, PSH_CALL);
+    if constexpr (sizeof(T) == 8)
+        rc = a.N <= 4 ? PSH_CALL(1, 4) : a.N <= 8 ? PSH_CALL(2, 4) : a.N <= 16 ? PSH_CALL(2, 8) : a.N <= 32 ? PSH_CALL(2, 16) : PSH_CALL(4, 16);
+    else
+        rc = PSH_FOR_STATES(a.N, PSH_CALL);
 #undef PSH_CALL
     if (rc != PSH_OK) return rc;
     if (a.part_bc && d->rows > 0) {
         const long n = ((long)d->rows * 2 * a.N + 255) / 256;
         hipLaunchKernelGGL(k_sum_bc<T>, dim3((unsigned)(n < 4096 ? n : 4096)), dim3(256), 0, st, (const W*)a.part_bc, (long)d->rows,
-                           d->offsets, (int)d->n_seqs, channel_blocks(d), (int)a.N, a.dB, a.dC);
+                           d->offsets, (int)d->n_seqs, a.blocks, (int)a.N, a.dB, a.dC);
         PSH_HIP(c, hipGetLastError());
         // rows behind the last sequence: the grad kernel's first channel block has written their zeros
     }
@@ -1224,7 +1281,7 @@ int check_scan(psh_ctx* c, const psh_scan_desc* d, bool grad) {
     if (d->dtype < PSH_F64 || d->dtype > PSH_BF16) return bad(c, "selective_scan: unknown dtype");
     if (d->n_policies < 1 || d->n_seqs < 0 || d->rows < 0 || d->channels < 1 || d->states < 1 || d->states > PSH_MAX_MEM_STATES)
         return bad(c, "selective_scan: invalid sizes (1..PSH_MAX_MEM_STATES states)");
-    if (d->rows > (1 << 30) || d->n_seqs > (1 << 30) || channel_blocks(d) > 65535 || ((int64_t)d->channels * d->states + 2 * (int64_t)d->channels + 255) / 256 > 65535)
+    if (d->rows > (1 << 30) || d->n_seqs > (1 << 30) || (d->rows + (int64_t)d->n_seqs + 2) * channel_blocks(d, true) > 0x7fffffffLL || ((int64_t)d->channels * d->states + 2 * (int64_t)d->channels + 255) / 256 > 65535)
         return too_large(c, "selective_scan");
     if (d->n_policies > 1 && !d->groups) return bad(c, "selective_scan: several policies need groups");
     if (d->step ? d->rows != d->n_seqs : !d->offsets) return bad(c, "selective_scan: offsets are NULL, or a step call has not one row per sequence");

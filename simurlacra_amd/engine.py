@@ -81,7 +81,7 @@ class Engine:
                 raise EngineError(f'{what} failed ({rc}): {msg.decode() if msg else ""}')
 
     def _stream(self):
-        return torch.cuda.current_stream(self.device).cuda_stream
+        return torch._C._cuda_getCurrentRawStream(self.device.index)   # what current_stream() wraps, at a tenth of its cost
 
     def f64(self, a, shape=None):
         t = torch.as_tensor(np.asarray(a, dtype=np.float64) if not torch.is_tensor(a) else a, dtype=torch.float64)

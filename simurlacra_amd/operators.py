@@ -38,39 +38,58 @@ def wide_dtype(dtype: torch.dtype) -> torch.dtype:
 
 
 # --------------------------------------------------------------------------------------------------------- checks
-def _rows_arg(name, t, dtype=None, device=None, cols=None, rows=None):
-    """ A [rows, cols] tensor whose columns are neighbours (copied if they are not): (tensor, row stride). """
-    if not torch.is_tensor(t):
-        raise TypeErr(given=t, given_name=name, expected_type=torch.Tensor)
+# (These run before every call, and a small call takes a few microseconds on the GPU: each check is one expression on the
+# common path, and what is wrong is only worked out once something is.)
+_Tensor = torch.Tensor
+
+
+def _refuse(name, t, dtype, device, shape):
+    """ Raises for the first thing about t that is not as the call wants it (None in shape: any size). """
+    if not isinstance(t, _Tensor):
+        raise TypeErr(given=t, given_name=name, expected_type=_Tensor)
     if t.dtype not in _DTYPES or (dtype is not None and t.dtype != dtype):
         raise TypeErr(msg=f'{name} must be of type {"float64, float32 or bfloat16" if dtype is None else dtype}, but is {t.dtype}!')
-    if not t.is_cuda or (device is not None and t.device != device):
-        raise ValueErr(msg=f'{name} must be on {"a GPU" if device is None else device}, but is on {t.device}! There is no CPU fallback.')
-    if t.dim() != 2 or (cols is not None and t.shape[1] != cols) or (rows is not None and t.shape[0] != rows):
-        raise ShapeErr(msg=f'{name} must have the shape [{"rows" if rows is None else rows}, '
-                           f'{"columns" if cols is None else cols}], but has {list(t.shape)}!')
-    n, m = t.shape
-    if m > 1 and t.stride(1) != 1 or n > 1 and t.stride(0) < m:
+    if not t.is_cuda and device is None:
+        raise ValueErr(msg=f'{name} must be on a GPU, but is on {t.device}! There is no CPU fallback.')
+    if device is not None and t.device != device:
+        raise ValueErr(msg=f'{name} must be on {device}, but is on {t.device}!')
+    raise ShapeErr(msg=f'{name} must have the shape [{", ".join("any" if n is None else str(n) for n in shape)}], but has {list(t.shape)}!')
+
+
+def _rows_arg(name, t, dtype, device, rows, cols):
+    """ A [rows, cols] tensor whose columns are neighbours (copied if they are not): (tensor, row stride). """
+    if not isinstance(t, _Tensor) or t.dtype != dtype or t.device != device or t.shape != (rows, cols):
+        _refuse(name, t, dtype, device, (rows, cols))
+    ld, step = t.stride()
+    if (step != 1 and cols > 1) or (ld < cols and rows > 1):
         t = t.contiguous()
-    return t, (t.stride(0) if n > 1 else m)
+        ld = cols
+    return t, (ld if rows > 1 else cols)
+
+
+def _first_rows_arg(name, t):
+    """ The same for the tensor that decides about type, device and size, and the engine of its GPU. """
+    if not isinstance(t, _Tensor) or t.dtype not in _DTYPES or not t.is_cuda or t.dim() != 2:
+        _refuse(name, t, None, None, (None, None))
+    rows, cols = t.shape
+    ld, step = t.stride()
+    if (step != 1 and cols > 1) or (ld < cols and rows > 1):
+        t = t.contiguous()
+        ld = cols
+    device = t.device
+    return t, (ld if rows > 1 else cols), rows, cols, t.dtype, device, get_engine(device.index)
 
 
 def _param(name, t, dtype, device, shape):
     """ A parameter or state of the given shape, contiguous. """
-    if not torch.is_tensor(t):
-        raise TypeErr(given=t, given_name=name, expected_type=torch.Tensor)
-    if t.dtype != dtype:
-        raise TypeErr(msg=f'{name} must be of type {dtype}, but is {t.dtype}!')
-    if t.device != device:
-        raise ValueErr(msg=f'{name} must be on {device}, but is on {t.device}!')
-    if tuple(t.shape) != tuple(shape):
-        raise ShapeErr(msg=f'{name} must have the shape {list(shape)}, but has {list(t.shape)}!')
+    if not isinstance(t, _Tensor) or t.dtype != dtype or t.device != device or t.shape != shape:
+        _refuse(name, t, dtype, device, shape)
     return t.contiguous()
 
 
 def _offsets(name, t, device):
-    if not torch.is_tensor(t):
-        raise TypeErr(given=t, given_name=name, expected_type=torch.Tensor)
+    if not isinstance(t, _Tensor):
+        raise TypeErr(given=t, given_name=name, expected_type=_Tensor)
     if t.dtype != torch.int32:
         raise TypeErr(msg=f'{name} must be of type torch.int32, but is {t.dtype}!')
     if t.device != device:
@@ -80,8 +99,15 @@ def _offsets(name, t, device):
     return t.contiguous()
 
 
+def _any_requires_grad(*tensors):
+    for t in tensors:
+        if isinstance(t, _Tensor) and t.requires_grad:
+            return True
+    return False
+
+
 def _no_grad_args(what, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if torch.is_grad_enabled() and _any_requires_grad(*tensors):
         raise ValueErr(msg=f'{what} updates its state in place and has no gradient: call it under torch.no_grad(), and the '
                            f'form for whole sequences for training!')
 
@@ -90,15 +116,30 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _workspace(bytes_, device):
-    return torch.empty(bytes_, dtype=torch.uint8, device=device) if bytes_ > 0 else None
-
-
 def _size(eng, name, desc):
     n = getattr(eng.lib, name)(C.byref(desc))
     if n < 0:
         raise ValueErr(msg=f'{name}: invalid sizes')
-    return int(n)
+    return n
+
+
+def _workspace(n, device):
+    return torch.empty(n, dtype=torch.uint8, device=device) if n > 0 else None
+
+
+def _give_workspace(eng, desc, name, device):
+    """ The scratch memory of a call, written into its descriptor; it has to outlive the call. """
+    n = _size(eng, name, desc)
+    if n == 0:
+        return None
+    space = torch.empty(n, dtype=torch.uint8, device=device)
+    desc.workspace, desc.workspace_bytes = space.data_ptr(), n
+    return space
+
+
+def _first_derivative_only():
+    if torch.is_grad_enabled():   # as it is in a backward pass with create_graph=True
+        raise ValueErr(msg='the policy operators have no second derivatives!')
 
 
 def _grad_tensor(t, like_dtype):
@@ -107,49 +148,39 @@ def _grad_tensor(t, like_dtype):
 
 
 # ------------------------------------------------------------------------------------------------- grouped_linear
-def _linear_desc(eng, x, weight, bias, offsets, nonlin):
-    x, ld_x = _rows_arg('x', x)
-    dev, dt = x.device, x.dtype
+def _linear_desc(x, weight, bias, offsets, nonlin):
+    x, ld_x, R, K, dt, dev, eng = _first_rows_arg('x', x)
     offsets = _offsets('offsets', offsets, dev)
     if nonlin not in _NONLINS:
         raise ValueErr(msg=f'nonlin must be one of {list(_NONLINS)}, but is {nonlin!r}!')
-    G, K = offsets.shape[0] - 1, x.shape[1]
-    if not torch.is_tensor(weight):
-        raise TypeErr(given=weight, given_name='weight', expected_type=torch.Tensor)
-    if weight.dim() != 3 or weight.shape[0] != G or weight.shape[2] != K or weight.shape[1] < 1 or K < 1:
+    G = offsets.shape[0] - 1
+    if not isinstance(weight, _Tensor) or weight.dtype != dt or weight.device != dev or weight.dim() != 3:
+        _refuse('weight', weight, dt, dev, (G, None, K))
+    groups, N, cols = weight.shape
+    if groups != G or cols != K or N < 1 or K < 1:
         raise ShapeErr(msg=f'weight must have the shape [{G}, outputs, {K}] with at least one input and output, but has {list(weight.shape)}!')
-    N = weight.shape[1]
-    for name, t in (('weight', weight), ('bias', bias)):
-        if t is not None and (t.dtype != dt or t.device != dev):
-            raise TypeErr(msg=f'{name} must be of type {dt} on {dev}, but is {t.dtype} on {t.device}!')
-    if K > 1 and weight.stride(2) != 1 or N > 1 and weight.stride(1) < K:
+    stride_w, ld_w, step = weight.stride()
+    if (step != 1 and K > 1) or (ld_w < K and N > 1):
         weight = weight.contiguous()
+        stride_w, ld_w = N*K, K
+    stride_b, b = 0, None
     if bias is not None:
-        if tuple(bias.shape) != (G, N):
-            raise ShapeErr(msg=f'bias must have the shape {[G, N]}, but has {list(bias.shape)}!')
-        if N > 1 and bias.stride(1) != 1:
+        if not isinstance(bias, _Tensor) or bias.dtype != dt or bias.device != dev or bias.shape != (G, N):
+            _refuse('bias', bias, dt, dev, (G, N))
+        stride_b, step = bias.stride()
+        if step != 1 and N > 1:
             bias = bias.contiguous()
-    d = abi.PshLinearDesc()
-    d.dtype, d.nonlin, d.n_groups, d.rows, d.in_dim, d.out_dim = _DTYPES[dt], _NONLINS[nonlin], G, x.shape[0], K, N
-    d.offsets, d.x, d.weight, d.bias = offsets.data_ptr(), x.data_ptr(), weight.data_ptr(), _ptr(bias)
-    d.ld_x, d.ld_w, d.stride_w = ld_x, (weight.stride(1) if N > 1 else K), (weight.stride(0) if G > 1 else 0)
-    d.stride_b = 0 if bias is None or G == 1 else bias.stride(0)
+            stride_b = N
+        b = bias.data_ptr()
+    d = abi.PshLinearDesc(_DTYPES[dt], _NONLINS[nonlin], G, R, K, N, offsets.data_ptr(), x.data_ptr(), weight.data_ptr(), b, None, ld_x,
+                          ld_w if N > 1 else K, stride_w if G > 1 else 0, stride_b if G > 1 else 0)
     d.stream = eng._stream()
-    return d, (x, weight, bias, offsets)    # the tensors have to outlive the call
-
-
-def _engine_of(x, name='x'):
-    if not torch.is_tensor(x):
-        raise TypeErr(given=x, given_name=name, expected_type=torch.Tensor)
-    if not x.is_cuda:
-        raise ValueErr(msg=f'{name} must be on a GPU, but is on {x.device}! There is no CPU fallback.')
-    return get_engine(x.device.index)
+    return eng, d, (x, weight, bias, offsets), R, K, G, N, dt, dev    # the tensors have to outlive the call
 
 
 def _linear_forward(x, weight, bias, offsets, nonlin):
-    eng = _engine_of(x)
-    d, keep = _linear_desc(eng, x, weight, bias, offsets, nonlin)
-    y = torch.empty((x.shape[0], weight.shape[1]), dtype=x.dtype, device=x.device)
+    eng, d, keep, R, K, G, N, dt, dev = _linear_desc(x, weight, bias, offsets, nonlin)
+    y = torch.empty((R, N), dtype=dt, device=dev)
     d.y = y.data_ptr()
     eng._call('psh_grouped_linear', C.byref(d))
     del keep
@@ -159,23 +190,25 @@ def _linear_forward(x, weight, bias, offsets, nonlin):
 def grouped_linear_grad(dy, y, x, weight, offsets, nonlin=None, want=(True, True, True)):
     """ The gradients (dx, dweight, dbias) of grouped_linear for the gradient dy of its result y; None where `want` is false.
     y is only read with a nonlinearity (its slope is taken from the value, in y's type). """
-    eng = _engine_of(x)
-    d, keep = _linear_desc(eng, x, weight, None, offsets, nonlin)
-    (G, N, K), R, dev = weight.shape, x.shape[0], x.device
-    dy, d.ld_dy = _rows_arg('dy', dy, x.dtype, dev, N, R)
+    eng, d, keep, R, K, G, N, dt, dev = _linear_desc(x, weight, None, offsets, nonlin)
+    dy, d.ld_dy = _rows_arg('dy', dy, dt, dev, R, N)
     d.dy = dy.data_ptr()
     if nonlin is not None:
-        y = _param('y', y, x.dtype, dev, (R, N))
+        y = _param('y', y, dt, dev, (R, N))
         d.y = y.data_ptr()
-    dx = torch.empty((R, K), dtype=x.dtype, device=dev) if want[0] else None
-    dw = torch.empty((G, N, K), dtype=x.dtype, device=dev) if want[1] else None
-    db = torch.empty((G, N), dtype=x.dtype, device=dev) if want[2] else None
-    d.dx, d.dweight, d.dbias = _ptr(dx), _ptr(dw), _ptr(db)
-    d.workspace_bytes = _size(eng, 'psh_grouped_linear_grad_workspace', d)
-    space = _workspace(d.workspace_bytes, dev)
-    d.workspace = _ptr(space)
+    dx = dw = db = None
+    if want[0]:
+        dx = torch.empty((R, K), dtype=dt, device=dev)
+        d.dx = dx.data_ptr()
+    if want[1]:
+        dw = torch.empty((G, N, K), dtype=dt, device=dev)
+        d.dweight = dw.data_ptr()
+    if want[2]:
+        db = torch.empty((G, N), dtype=dt, device=dev)
+        d.dbias = db.data_ptr()
+    space = _give_workspace(eng, d, 'psh_grouped_linear_grad_workspace', dev)
     eng._call('psh_grouped_linear_grad', C.byref(d))
-    del keep
+    del keep, space
     return dx, dw, db
 
 
@@ -188,8 +221,8 @@ class _GroupedLinear(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        _first_derivative_only()
         x, weight, offsets, y = ctx.saved_tensors
         return grouped_linear_grad(dy, y, x, weight, offsets, ctx.nonlin, ctx.needs_input_grad[:3]) + (None, None)
 
@@ -199,7 +232,7 @@ def grouped_linear(x, weight, bias, offsets, nonlin: str = None):
 
     x [R, K]; weight [G, N, K] and bias [G, N] (or None) of x's type, views into a matrix of whole parameter vectors
     included; nonlin None, 'tanh', 'relu' or 'sigmoid'.  Returns y [R, N]. """
-    if torch.is_grad_enabled() and any(torch.is_tensor(t) and t.requires_grad for t in (x, weight, bias)):
+    if torch.is_grad_enabled() and _any_requires_grad(x, weight, bias):
         return _GroupedLinear.apply(x, weight, bias, offsets, nonlin)
     return _linear_forward(x, weight, bias, offsets, nonlin)
 
@@ -221,8 +254,8 @@ def _state_arg(name, t, dtype, dev, shape):
     """ A [sequences, ...] state whose sequences may be apart: (tensor, stride). """
     if t is None:
         return None, 0
-    if not torch.is_tensor(t):
-        raise TypeErr(given=t, given_name=name, expected_type=torch.Tensor)
+    if not isinstance(t, _Tensor):
+        raise TypeErr(given=t, given_name=name, expected_type=_Tensor)
     if t.dtype != dtype or t.device != dev:
         raise TypeErr(msg=f'{name} must be of type {dtype} on {dev}, but is {t.dtype} on {t.device}!')
     if tuple(t.shape) != tuple(shape):
@@ -233,12 +266,10 @@ def _state_arg(name, t, dtype, dev, shape):
     return t, (t.stride(0) if shape[0] > 1 else size)
 
 
-def _conv_desc(eng, x, weight, bias, offsets, groups, state, silu, step):
-    x, ld_x = _rows_arg('x', x)
-    dev, dt = x.device, x.dtype
+def _conv_desc(x, weight, bias, offsets, groups, state, silu, step):
+    x, ld_x, R, D, dt, dev, eng = _first_rows_arg('x', x)
     W = wide_dtype(dt)
-    R, D = x.shape
-    if not torch.is_tensor(weight) or weight.dim() != 3:
+    if not isinstance(weight, _Tensor) or weight.dim() != 3:
         raise ShapeErr(msg='weight must be a tensor of shape [policies, channels, taps]!')
     P, K = weight.shape[0], weight.shape[2]
     if not 1 <= K <= abi.PSH_MAX_TAPS or P < 1 or D < 1:
@@ -248,23 +279,21 @@ def _conv_desc(eng, x, weight, bias, offsets, groups, state, silu, step):
     groups = _policies(groups, dev, P)
     offsets = None if step else _offsets('offsets', offsets, dev)
     S = R if step else offsets.shape[0] - 1
-    d = abi.PshConvDesc()
-    d.dtype, d.silu, d.step, d.n_policies, d.n_seqs, d.rows, d.channels, d.taps = _DTYPES[dt], int(bool(silu)), int(step), P, S, R, D, K
-    d.offsets, d.groups, d.x, d.weight, d.bias = _ptr(offsets), _ptr(groups), x.data_ptr(), weight.data_ptr(), _ptr(bias)
+    d = abi.PshConvDesc(_DTYPES[dt], 1 if silu else 0, 1 if step else 0, P, S, R, D, K, _ptr(offsets), _ptr(groups), x.data_ptr(), weight.data_ptr(),
+                        _ptr(bias))
     d.ld_x = ld_x
     if state is not None:
         state, d.stride_state = _state_arg('state', state, dt, dev, (S, D, K - 1))
         d.state = state.data_ptr()
     d.stream = eng._stream()
-    return d, (x, weight, bias, offsets, groups, state), S
+    return eng, d, (x, weight, bias, offsets, groups, state), S, R, D, P, K, dt, dev
 
 
 def _conv_forward(x, weight, bias, offsets, groups, state, silu):
-    eng = _engine_of(x)
-    d, keep, S = _conv_desc(eng, x, weight, bias, offsets, groups, state, silu, False)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    last = torch.empty((S, x.shape[1], weight.shape[2] - 1), dtype=x.dtype, device=x.device)
-    d.y, d.last, d.stride_last = y.data_ptr(), last.data_ptr(), last.shape[1]*last.shape[2]
+    eng, d, keep, S, R, D, P, K, dt, dev = _conv_desc(x, weight, bias, offsets, groups, state, silu, False)
+    y = torch.empty((R, D), dtype=dt, device=dev)
+    last = torch.empty((S, D, K - 1), dtype=dt, device=dev)
+    d.y, d.last, d.stride_last = y.data_ptr(), last.data_ptr(), D*(K - 1)
     eng._call('psh_causal_conv', C.byref(d))
     del keep
     return y, last
@@ -273,24 +302,21 @@ def _conv_forward(x, weight, bias, offsets, groups, state, silu):
 def causal_conv_grad(dy, dlast, x, weight, bias, offsets, groups=None, state=None, silu: bool = True, want=(True,)*4):
     """ The gradients (dx, dweight, dbias, dstate) of causal_conv for those of its results (dlast may be None); None
     where `want` is false. """
-    eng = _engine_of(x)
-    d, keep, S = _conv_desc(eng, x, weight, bias, offsets, groups, state, silu, False)
-    (R, D), (P, _, K), dev = x.shape, weight.shape, x.device
-    dy, d.ld_dy = _rows_arg('dy', dy, x.dtype, dev, D, R)
+    eng, d, keep, S, R, D, P, K, dt, dev = _conv_desc(x, weight, bias, offsets, groups, state, silu, False)
+    dy, d.ld_dy = _rows_arg('dy', dy, dt, dev, R, D)
     d.dy = dy.data_ptr()
     if dlast is not None:
-        dlast = _param('dlast', dlast, x.dtype, dev, (S, D, K - 1))
+        dlast = _param('dlast', dlast, dt, dev, (S, D, K - 1))
         d.dlast = dlast.data_ptr()
-    dx = torch.empty((R, D), dtype=x.dtype, device=dev) if want[0] else None
-    dw = torch.empty((P, D, K), dtype=weight.dtype, device=dev) if want[1] else None
-    db = torch.empty((P, D), dtype=weight.dtype, device=dev) if want[2] else None
-    ds = torch.empty((S, D, K - 1), dtype=x.dtype, device=dev) if want[3] else None
+    W = wide_dtype(dt)
+    dx = torch.empty((R, D), dtype=dt, device=dev) if want[0] else None
+    dw = torch.empty((P, D, K), dtype=W, device=dev) if want[1] else None
+    db = torch.empty((P, D), dtype=W, device=dev) if want[2] else None
+    ds = torch.empty((S, D, K - 1), dtype=dt, device=dev) if want[3] else None
     d.dx, d.dweight, d.dbias, d.dstate = _ptr(dx), _ptr(dw), _ptr(db), _ptr(ds)
-    d.workspace_bytes = _size(eng, 'psh_causal_conv_grad_workspace', d)
-    space = _workspace(d.workspace_bytes, dev)
-    d.workspace = _ptr(space)
+    space = _give_workspace(eng, d, 'psh_causal_conv_grad_workspace', dev)
     eng._call('psh_causal_conv_grad', C.byref(d))
-    del keep
+    del keep, space
     return dx, dw, db, ds
 
 
@@ -303,8 +329,8 @@ class _CausalConv(torch.autograd.Function):
         return _conv_forward(x, weight, bias, offsets, groups, state, silu)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dlast):
+        _first_derivative_only()
         x, weight, bias, state, offsets, groups = ctx.saved_tensors
         if dy is None:
             dy = torch.zeros_like(x)
@@ -320,7 +346,7 @@ def causal_conv(x, weight, bias, offsets, groups=None, state=None, silu: bool = 
     x [R, D]; weight [P, D, K] and bias [P, D] (or None) of policy p, whose sequences `groups` name; state [S, D, K - 1] the inputs
     before each sequence's first step, oldest first (None: zeros).  Returns y [R, D], with return_state also the state
     after each sequence's last step. """
-    if torch.is_grad_enabled() and any(torch.is_tensor(t) and t.requires_grad for t in (x, weight, bias, state)):
+    if torch.is_grad_enabled() and _any_requires_grad(x, weight, bias, state):
         y, last = _CausalConv.apply(x, weight, bias, state, offsets, groups, silu)
     else:
         y, last = _conv_forward(x, weight, bias, offsets, groups, state, silu)
@@ -329,14 +355,13 @@ def causal_conv(x, weight, bias, offsets, groups=None, state=None, silu: bool = 
 
 def causal_conv_step(x, state, weight, bias, groups=None, silu: bool = True):
     """ causal_conv for one step of every sequence: x [S, D]; state [S, D, K - 1] is updated in place.  Returns y [S, D]. """
-    _no_grad_args('causal_conv_step', *(t for t in (x, state, weight, bias) if torch.is_tensor(t)))
-    eng = _engine_of(x)
+    _no_grad_args('causal_conv_step', x, state, weight, bias)
     if state is None:
-        raise TypeErr(given=state, given_name='state', expected_type=torch.Tensor)
-    d, keep, S = _conv_desc(eng, x, weight, bias, None, groups, state, silu, True)
-    if S and weight.shape[2] > 1 and keep[5] is not state:
+        raise TypeErr(given=state, given_name='state', expected_type=_Tensor)
+    eng, d, keep, S, R, D, P, K, dt, dev = _conv_desc(x, weight, bias, None, groups, state, silu, True)
+    if S and K > 1 and keep[5] is not state:
         raise ValueErr(msg='state is updated in place: the values of each sequence have to be contiguous!')
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = torch.empty((R, D), dtype=dt, device=dev)
     d.y, d.last, d.stride_last = y.data_ptr(), state.data_ptr(), d.stride_state
     eng._call('psh_causal_conv', C.byref(d))
     del keep
@@ -344,55 +369,47 @@ def causal_conv_step(x, state, weight, bias, groups=None, silu: bool = True):
 
 
 # ------------------------------------------------------------------------------------------------- selective_scan
-def _scan_desc(eng, u, delta, A, B, Cm, D, z, delta_bias, offsets, groups, state, step):
-    u, ld_u = _rows_arg('u', u)
-    dev, dt = u.device, u.dtype
+def _scan_desc(u, delta, A, B, Cm, D, z, delta_bias, offsets, groups, state, step):
+    u, ld_u, R, ch, dt, dev, eng = _first_rows_arg('u', u)
     W = wide_dtype(dt)
-    R, ch = u.shape
-    if not torch.is_tensor(A) or A.dim() != 3:
+    if not isinstance(A, _Tensor) or A.dim() != 3:
         raise ShapeErr(msg='A must be a tensor of shape [policies, channels, states]!')
-    P, N = A.shape[0], A.shape[2]
+    P, _, N = A.shape
     if not 1 <= N <= abi.PSH_MAX_MEM_STATES or P < 1 or ch < 1:
         raise ValueErr(msg=f'selective_scan takes 1 to {abi.PSH_MAX_MEM_STATES} states and at least one policy and channel, but A is {list(A.shape)}!')
-    delta, ld_delta = _rows_arg('delta', delta, dt, dev, ch, R)
-    B, ld_B = _rows_arg('B', B, dt, dev, N, R)
-    Cm, ld_C = _rows_arg('C', Cm, dt, dev, N, R)
+    delta, ld_delta = _rows_arg('delta', delta, dt, dev, R, ch)
+    B, ld_B = _rows_arg('B', B, dt, dev, R, N)
+    Cm, ld_C = _rows_arg('C', Cm, dt, dev, R, N)
+    ld_z = 0
+    if z is not None:
+        z, ld_z = _rows_arg('z', z, dt, dev, R, ch)
     A = _param('A', A, W, dev, (P, ch, N))
     D = None if D is None else _param('D', D, W, dev, (P, ch))
     delta_bias = None if delta_bias is None else _param('delta_bias', delta_bias, W, dev, (P, ch))
     groups = _policies(groups, dev, P)
     offsets = None if step else _offsets('offsets', offsets, dev)
     S = R if step else offsets.shape[0] - 1
-    d = abi.PshScanDesc()
-    d.dtype, d.step, d.n_policies, d.n_seqs, d.rows, d.channels, d.states = _DTYPES[dt], int(step), P, S, R, ch, N
-    d.offsets, d.groups = _ptr(offsets), _ptr(groups)
-    d.u, d.delta, d.B, d.C = u.data_ptr(), delta.data_ptr(), B.data_ptr(), Cm.data_ptr()
-    d.ld_u, d.ld_delta, d.ld_B, d.ld_C = ld_u, ld_delta, ld_B, ld_C
-    if z is not None:
-        z, d.ld_z = _rows_arg('z', z, dt, dev, ch, R)
-        d.z = z.data_ptr()
-    d.A, d.D, d.delta_bias = A.data_ptr(), _ptr(D), _ptr(delta_bias)
+    stride = 0
     if state is not None:
-        state, d.stride_state = _state_arg('state', state, W, dev, (S, ch, N))
-        d.state = state.data_ptr()
+        state, stride = _state_arg('state', state, W, dev, (S, ch, N))
+    d = abi.PshScanDesc(_DTYPES[dt], 1 if step else 0, P, S, R, ch, N, 0, _ptr(offsets), _ptr(groups), u.data_ptr(), delta.data_ptr(), _ptr(z), B.data_ptr(),
+                        Cm.data_ptr(), A.data_ptr(), _ptr(D), _ptr(delta_bias), _ptr(state), None, None, ld_u, ld_delta, ld_z, ld_B, ld_C, stride)
     d.stream = eng._stream()
-    return d, (u, delta, A, B, Cm, D, z, delta_bias, offsets, groups, state), S
+    return eng, d, (u, delta, A, B, Cm, D, z, delta_bias, offsets, groups, state), S, R, ch, P, N, dt, W, dev
 
 
 def _scan_forward(u, delta, A, B, Cm, D, z, delta_bias, offsets, groups, state, keep_check):
-    eng = _engine_of(u, 'u')
-    d, keep, S = _scan_desc(eng, u, delta, A, B, Cm, D, z, delta_bias, offsets, groups, state, False)
-    dev = u.device
-    y = torch.empty(u.shape, dtype=u.dtype, device=dev)
-    last = torch.empty((S,) + tuple(A.shape[1:]), dtype=A.dtype, device=dev)
-    d.y, d.last, d.stride_last = y.data_ptr(), last.data_ptr(), A.shape[1]*A.shape[2]
-    check = _workspace(_size(eng, 'psh_selective_scan_check', d), dev) if keep_check else None
-    d.check = _ptr(check)
-    d.workspace_bytes = _size(eng, 'psh_selective_scan_workspace', d)
-    space = _workspace(d.workspace_bytes, dev)
-    d.workspace = _ptr(space)
+    eng, d, keep, S, R, ch, P, N, dt, W, dev = _scan_desc(u, delta, A, B, Cm, D, z, delta_bias, offsets, groups, state, False)
+    y = torch.empty((R, ch), dtype=dt, device=dev)
+    last = torch.empty((S, ch, N), dtype=W, device=dev)
+    d.y, d.last, d.stride_last = y.data_ptr(), last.data_ptr(), ch*N
+    check = None
+    if keep_check:
+        check = _workspace(_size(eng, 'psh_selective_scan_check', d), dev)
+        d.check = check.data_ptr()
+    space = _give_workspace(eng, d, 'psh_selective_scan_workspace', dev)
     eng._call('psh_selective_scan', C.byref(d))
-    del keep
+    del keep, space
     return y, last, check
 
 
@@ -409,10 +426,8 @@ def selective_scan_grad(dy, dlast, check, u, delta, A, B, C, D, z, delta_bias, o
 
 
 def _scan_grad(dy, dlast, check, u, delta, A, B, Cm, D, z, delta_bias, offsets, groups, state, want):
-    eng = _engine_of(u, 'u')
-    d, keep, S = _scan_desc(eng, u, delta, A, B, Cm, D, z, delta_bias, offsets, groups, state, False)
-    (R, ch), (P, _, N), dev, dt, W = u.shape, A.shape, u.device, u.dtype, A.dtype
-    dy, d.ld_dy = _rows_arg('dy', dy, dt, dev, ch, R)
+    eng, d, keep, S, R, ch, P, N, dt, W, dev = _scan_desc(u, delta, A, B, Cm, D, z, delta_bias, offsets, groups, state, False)
+    dy, d.ld_dy = _rows_arg('dy', dy, dt, dev, R, ch)
     d.dy = dy.data_ptr()
     if dlast is not None:
         dlast = _param('dlast', dlast, W, dev, (S, ch, N))
@@ -429,11 +444,9 @@ def _scan_grad(dy, dlast, check, u, delta, A, B, Cm, D, z, delta_bias, offsets, 
     dD, dz = out(5, D is not None, (P, ch), W), out(6, z is not None, (R, ch), dt)
     dbias, dstate = out(7, delta_bias is not None, (P, ch), W), out(8, state is not None, (S, ch, N), W)
     d.du, d.ddelta, d.dA, d.dB, d.dC, d.dD, d.dz, d.ddelta_bias, d.dstate = (_ptr(t) for t in (du, ddelta, dA, dB, dC, dD, dz, dbias, dstate))
-    d.workspace_bytes = _size(eng, 'psh_selective_scan_grad_workspace', d)
-    space = _workspace(d.workspace_bytes, dev)
-    d.workspace = _ptr(space)
+    space = _give_workspace(eng, d, 'psh_selective_scan_grad_workspace', dev)
     eng._call('psh_selective_scan_grad', C.byref(d))
-    del keep
+    del keep, space
     return du, ddelta, dA, dB, dC, dD, dz, dbias, dstate
 
 
@@ -446,8 +459,8 @@ class _SelectiveScan(torch.autograd.Function):
         return y, last
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dlast):
+        _first_derivative_only()
         u, delta, A, B, Cm, D, z, delta_bias, state, offsets, groups, check = ctx.saved_tensors
         if dy is None:
             dy = torch.zeros_like(u)
@@ -466,7 +479,7 @@ def selective_scan(u, delta, A, B, C, D, z, delta_bias, offsets, groups=None, st
     before each sequence's first step (None: zeros).  D, z and delta_bias may be None.  Returns y [R, D], with return_state
     also the state after each sequence's last step. """
     args = (u, delta, A, B, C, D, z, delta_bias, state)
-    if torch.is_grad_enabled() and any(torch.is_tensor(t) and t.requires_grad for t in args):
+    if torch.is_grad_enabled() and _any_requires_grad(*args):
         y, last = _SelectiveScan.apply(*args, offsets, groups)
     else:
         y, last, _ = _scan_forward(u, delta, A, B, C, D, z, delta_bias, offsets, groups, state, False)
@@ -480,14 +493,13 @@ def selective_scan_step(u, delta, state, A, B, C, D, z, delta_bias, groups=None)
 
 
 def _scan_step(u, delta, state, A, B, Cm, D, z, delta_bias, groups):
-    _no_grad_args('selective_scan_step', *(t for t in (u, delta, state, A, B, Cm, D, z, delta_bias) if torch.is_tensor(t)))
-    eng = _engine_of(u, 'u')
+    _no_grad_args('selective_scan_step', u, delta, state, A, B, Cm, D, z, delta_bias)
     if state is None:
-        raise TypeErr(given=state, given_name='state', expected_type=torch.Tensor)
-    d, keep, S = _scan_desc(eng, u, delta, A, B, Cm, D, z, delta_bias, None, groups, state, True)
+        raise TypeErr(given=state, given_name='state', expected_type=_Tensor)
+    eng, d, keep, S, R, ch, P, N, dt, W, dev = _scan_desc(u, delta, A, B, Cm, D, z, delta_bias, None, groups, state, True)
     if S and keep[10] is not state:
         raise ValueErr(msg='state is updated in place: the values of each sequence have to be contiguous!')
-    y = torch.empty(u.shape, dtype=u.dtype, device=u.device)
+    y = torch.empty((R, ch), dtype=dt, device=dev)
     d.y, d.last, d.stride_last = y.data_ptr(), state.data_ptr(), d.stride_state
     eng._call('psh_selective_scan', C.byref(d))
     del keep

@@ -296,3 +296,56 @@ def test_selective_scan_far_values(ops):
         n = 24*(4 + 3 + 3)*2 + 44
         close('y', y, want['y'], M['y'], n, T)
         close('last', last, want['last'], M['last'], n, T)
+
+
+@pytest.mark.parametrize('T', TYPES, ids=IDS)
+@pytest.mark.parametrize('lengths,K,N,shift', [
+    # rows and sizes of the large tiles: whole and partial ones of every dimension, aligned and not
+    ([9000, 0, 130, 17000], 72, 200, 0), ([12800, 12800], 264, 136, 0), ([20000, 5001], 100, 129, 0), ([16000], 256, 328, 1), ([6000, 127, 4001], 129, 520, 0),
+    ([8192, 8193], 512, 264, 0), ([200]*40, 136, 1032, 0)])
+def test_grouped_linear_large(ops, T, lengths, K, N, shift):
+    """ as above, elements off their 16-byte places by `shift` """
+    gen = torch.Generator().manual_seed(K)
+    off, R, G = offs(lengths), sum(lengths) + 2, len(lengths)
+    x, dy = rnd(gen, R, K + 8, T=T)[:, shift:shift + K], rnd(gen, R, N, T=T)
+    w, b = rnd(gen, G, N, K + 8, T=T, scale=K**-.5)[:, :, shift:shift + K], rnd(gen, G, N, T=T)
+    y = ops.grouped_linear(x, w, b, off)
+    got = ops.grouped_linear_grad(dy, None, x, w, off)
+    want, M = (ref.linear(x, w, b, off, None, dy, mag=m) for m in (False, True))
+    close('y', y, want['y'], M['y'], K + 8, T)
+    # a sum over n rows that is cut into pieces has fewer roundings than n on any chain
+    for name, g, n in zip(('dx', 'dw', 'db'), got, (N + 8, max(lengths) + 8, max(lengths) + 8)):
+        close(name, g, want[name], M[name], n, T)
+    again = ops.grouped_linear_grad(dy, None, x, w, off)
+    assert all(torch.equal(a, b) for a, b in zip(got, again)) and torch.equal(y, ops.grouped_linear(x, w, b, off))
+
+
+@pytest.mark.parametrize('T', TYPES, ids=IDS)
+@pytest.mark.parametrize('lengths,D,N,groups', [([1500, 0, 700, 3], 40, 16, None), ([4000], 70, 5, None), ([900, 1, 64, 65, 1000], 12, 40, [1, 0, 4]),
+                                                ([130]*9, 200, 16, [3, 6]), ([3 + i % 90 for i in range(400)], 24, 16, None)])
+def test_long_sequences(ops, T, lengths, D, N, groups):
+    """ The recurrence cut into pieces and joined, and the convolution over many runs of rows """
+    gen = torch.Generator().manual_seed(sum(lengths))
+    W, K = ops.wide_dtype(T), 4
+    v, off, grp = scan_inputs(gen, ops, T, lengths, D, N, groups)
+    S, R, P = len(lengths), v['u'].shape[0], len(groups) if groups else 1
+    dy, dlast = rnd(gen, R, D, T=T), rnd(gen, S, D, N, T=W)
+    args = (v['u'], v['delta'], v['A'], v['B'], v['C'], v['D'], v['z'], v['delta_bias'], off, grp, v['state'])
+    y, last, check = ops.selective_scan_check(*args)
+    got = dict(zip(('u', 'delta', 'A', 'B', 'C', 'D', 'z', 'bias', 'state'), ops.selective_scan_grad(dy, dlast, check, *args)))
+    want, M = (ref.scan(*args, dy, dlast, mag=m) for m in (False, True))
+    n = roundings(v, lengths, N, D)
+    close('y', y, want['y'], M['y'], n, T)
+    close('last', last, want['last'], M['last'], n, W)
+    for k in ('u', 'delta', 'z', 'B', 'C'):
+        close('d' + k, got[k], want['d' + k], M['d' + k], 2*n + D, T)
+    for k in ('A', 'D', 'bias'):
+        close('d' + k, got[k], want['d' + k], M['d' + k], 2*n + sum(lengths), W)
+    close('dstate', got['state'], want['dstate'], M['dstate'], 2*n, W)
+    x, cy, cs = rnd(gen, R, D, T=T), rnd(gen, R, D, T=T), rnd(gen, S, D, K - 1, T=T)
+    w, b = rnd(gen, P, D, K, T=W, scale=.5), rnd(gen, P, D, T=W)
+    g = ops.causal_conv_grad(cy, cs, x, w, b, off, grp, cs)
+    want, M = (ref.conv(x, w, b, off, grp, cs, True, cy, cs, mag=m) for m in (False, True))
+    for name, t, k, T_ in zip(('dx', 'dw', 'db', 'dstate'), g, (2*(K + 12), K + 12 + sum(lengths), K + 12 + sum(lengths), 2*(K + 12)), (T, W, W, T)):
+        close(name, t, want[name], M[name], k, T_)
+    close('conv', ops.causal_conv(x, w, b, off, grp, cs), want['y'], M['y'], K + 12, T)
