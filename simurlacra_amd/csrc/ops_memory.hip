@@ -435,13 +435,7 @@ template <class T> struct ScanArgs {
 PSH_OP float decay_rate(float a) { return a * (float)PSH_LOG2E; }
 PSH_OP double decay_rate(double a) { return a; }
 PSH_OP float decay(float dt, float rate) { return exp2_w(dt * rate); }
-// (psh_exp without its branch, which would keep the states of a step from running side by side: the core is right, and over- or
-// underflows, for every |x| < 2^30, so only the high word of what lies beyond is replaced; a NaN stays one)
-PSH_OP double decay(double dt, double rate) {
-    const double x = dt * rate;
-    const int hi = __double2hiint(x);
-    return psh_exp_core(__hiloint2double(fabs(x) > 1e9 ? (hi & (int)0x80000000) | 0x41cdcd65 : hi, __double2loint(x)));
-}
+PSH_OP double decay(double dt, double rate) { return exp_w(dt * rate); }
 // sum of g a h' A from a sum with prepared rates
 PSH_OP float rate_unit(float) { return (float)PSH_LN2; }
 PSH_OP double rate_unit(double) { return 1.; }
@@ -661,9 +655,10 @@ template <class T, int NP, int LPC, bool CARRY> __global__ __launch_bounds__(THR
     for (int r0 = q.begin, tile = 0; r0 < q.end; r0 += TS, ++tile) {
         now = next;
         if (ld.on) {
+            const int live = r0 + ld.t < q.end ? -1 : 0;   // (a step size of 0 leaves the state as it is)
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                const W dt = r0 + ld.t < q.end ? softplus_w(to_wide((T)now.delta[e]) + ld.bias[e]) : W(0);
+                const W dt = masked(softplus_w(to_wide((T)now.delta[e]) + ld.bias[e]), live);
                 s_dt[ld.t][ld.c + e] = Pair<W>{dt, dt * to_wide((T)now.u[e])};
             }
         }
@@ -862,10 +857,11 @@ template <class T, int NP, int LPC, bool CARRY> __global__ __launch_bounds__(THR
         now = next;
         W dt[E];
         if (ld.on) {
+            const int live = r0 + ld.t < q.end ? -1 : 0;
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                const W raw = to_wide((T)now.delta[e]) + ld.bias[e];
-                dt[e] = r0 + ld.t < q.end ? softplus_w(raw) : W(0);
+                W slope;
+                dt[e] = masked(softplus_w(to_wide((T)now.delta[e]) + ld.bias[e], slope), live);
                 s_dt[ld.t][ld.c + e] = Pair<W>{dt[e], dt[e] * to_wide((T)now.u[e])};
                 W dy = to_wide((T)now.dy[e]);
                 if (a.z) {
@@ -874,7 +870,7 @@ template <class T, int NP, int LPC, bool CARRY> __global__ __launch_bounds__(THR
                     if constexpr (!CARRY) s_sz[ld.t][ld.c + e] = sz;
                 }
                 s_dy[ld.t][ld.c + e] = dy;
-                if constexpr (!CARRY) s_sd[ld.t][ld.c + e] = sigmoid_w(raw);
+                if constexpr (!CARRY) s_sd[ld.t][ld.c + e] = slope;
             }
         }
         bc.template store<true>(s_b, s_c);

@@ -33,32 +33,53 @@ template <> PSH_OP bf16_t to_elem<bf16_t>(float x) {
 }
 
 // ------------------------------------------------------------------------------------------ elementary functions
+// Without branches, so that the elements a lane works on run side by side; NaN arguments give NaNs by themselves.
 // fp32: v_exp_f32 / v_log_f32 / v_rcp_f32 are within 1 ulp of the power, logarithm and reciprocal; what the argument's
 // scaling by log2(e) adds is |x| 2^-24 relative, which an exponential of a negative argument shrinks again.
+// fp64: psh_exp's core, which is right, and over- or underflows, for every |x| < 2^30; only the high word of what lies
+// beyond is replaced (a NaN compares false and stays one).
 #define PSH_LOG2E 1.4426950408889634
 #define PSH_LN2 0.6931471805599453
 PSH_OP float exp2_w(float x) { return __builtin_amdgcn_exp2f(x); }
 PSH_OP float exp_w(float x) { return __builtin_amdgcn_exp2f(x * (float)PSH_LOG2E); }
-PSH_OP double exp_w(double x) { return psh_exp(x); }
+PSH_OP double exp_w(double x) {
+    const int hi = __double2hiint(x);
+    return psh_exp_core(__hiloint2double(fabs(x) > 1e9 ? (hi & (int)0x80000000) | 0x41cdcd65 : hi, __double2loint(x)));
+}
 PSH_OP float rcp_w(float x) { return __builtin_amdgcn_rcpf(x); }
 PSH_OP float sigmoid_w(float x) { return rcp_w(1.f + exp_w(-x)); }
-PSH_OP double sigmoid_w(double x) { return psh_sigmoid(x); }
+PSH_OP double sigmoid_w(double x) {
+    const double e = exp_w(-fabs(x)), r = psh_rcp_refined(1. + e);   // (the denominator lies in [1, 2])
+    return x >= 0. ? r : e * r;
+}
 template <class W> PSH_OP W silu_w(W x) { return x * sigmoid_w(x); }
 // d/dx of x sigmoid(x) from s = sigmoid(x)
 template <class W> PSH_OP W silu_slope_w(W x, W s) { return s * (W(1) + x * (W(1) - s)); }
-// log(1 + e^x) = max(x, 0) + log1p(e^-|x|).  log1p keeps the digits of a small e, where the step sizes of a slow memory are.
-// By hand: w = 1 + e rounds, and e - (w - 1) is what that lost, exactly; it goes back in front of log's slope
-// 1 / w, which is 1 where it matters (for e near 1 the lost part is below half a ulp of the result anyway).
+// log(1 + e^x) = max(x, 0) + log1p(e^-|x|).  log1p keeps the digits of a small e, where the step sizes of a slow memory are:
+// w = 1 + e rounds, and e - (w - 1) is what that lost, exactly; it goes back in front of log's slope 1 / w, which is 1 where
+// it matters (for e near 1 the lost part is below half a ulp of the result anyway).
 PSH_OP float softplus_w(float x) {
     const float e = exp_w(-fabsf(x)), w = 1.f + e;
-    const float l = __builtin_amdgcn_logf(w) * (float)PSH_LN2 + (e - (w - 1.f));
-    return x != x ? x : fmaxf(x, 0.f) + l;
+    return fmaxf(x, 0.f) + (__builtin_amdgcn_logf(w) * (float)PSH_LN2 + (e - (w - 1.f)));
 }
 PSH_OP double softplus_w(double x) {
-    const double e = psh_exp(-fabs(x)), w = 1. + e;
-    const double l = psh_log_normal(x != x ? 1. : w) + (e - (w - 1.));
-    return x != x ? x : fmax(x, 0.) + l;
+    const double e = exp_w(-fabs(x)), w = 1. + e;
+    return fmax(x, 0.) + (psh_log_normal(w) + (e - (w - 1.)));
 }
+// the same and its derivative, sigmoid(x), from one exponential
+PSH_OP float softplus_w(float x, float& slope) {
+    const float e = exp_w(-fabsf(x)), w = 1.f + e, r = rcp_w(w);
+    slope = x >= 0.f ? r : e * r;
+    return fmaxf(x, 0.f) + (__builtin_amdgcn_logf(w) * (float)PSH_LN2 + (e - (w - 1.f)));
+}
+PSH_OP double softplus_w(double x, double& slope) {
+    const double e = exp_w(-fabs(x)), w = 1. + e, r = psh_rcp_refined(w);
+    slope = x >= 0. ? r : e * r;
+    return fmax(x, 0.) + (psh_log_normal(w) + (e - (w - 1.)));
+}
+// x where the mask is all ones, 0 where it is 0, whatever x is
+PSH_OP float masked(float x, int mask) { return __int_as_float(__float_as_int(x) & mask); }
+PSH_OP double masked(double x, int mask) { return __hiloint2double(__double2hiint(x) & mask, __double2loint(x) & mask); }
 PSH_OP float tanh_w(float x) { return tanhf(x); }
 PSH_OP double tanh_w(double x) { return psh_tanh(x); }
 
