@@ -15,35 +15,38 @@
 // indices (fragment reads) and 8 indices 8 apart (transposing writes) lie in different banks.
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "psh_ops.h"
 
 namespace {
 
+// Part k of the product of two fragments.  The parts of one fragment pair all add to the same accumulator, so the parts are the outer
+// loop: an instruction that waits for the one before it would leave the matrix pipe idle.
 template <class T> struct Mfma;
 template <> struct Mfma<bf16_t> {
     typedef v4f acc;
+    static constexpr int PARTS = 1;
     static constexpr int row(int q, int r) { return 4 * q + r; }   // index i of accumulator register r in lane group q
-    static PSH_OP void step(const v4u& p, const v4u& q, acc& d) {
+    template <int> static PSH_OP void step(const v4u& p, const v4u& q, acc& d) {
         d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, p), __builtin_bit_cast(v8bf, q), d, 0, 0, 0);
     }
 };
 template <> struct Mfma<float> {
     typedef v4f acc;
+    static constexpr int PARTS = 4;
     static constexpr int row(int q, int r) { return 4 * q + r; }
-    static PSH_OP void step(const v4u& p, const v4u& q, acc& d) {
-        const v4f a = __builtin_bit_cast(v4f, p), b = __builtin_bit_cast(v4f, q);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) d = __builtin_amdgcn_mfma_f32_16x16x4f32(a[k], b[k], d, 0, 0, 0);
+    template <int K> static PSH_OP void step(const v4u& p, const v4u& q, acc& d) {
+        d = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(p[K]), __uint_as_float(q[K]), d, 0, 0, 0);
     }
 };
 template <> struct Mfma<double> {
     typedef v4d acc;
+    static constexpr int PARTS = 2;
     static constexpr int row(int q, int r) { return 4 * r + q; }
-    static PSH_OP void step(const v4u& p, const v4u& q, acc& d) {
-        typedef double v2d __attribute__((ext_vector_type(2)));
-        const v2d a = __builtin_bit_cast(v2d, p), b = __builtin_bit_cast(v2d, q);
-#pragma unroll
-        for (int k = 0; k < 2; ++k) d = __builtin_amdgcn_mfma_f64_16x16x4f64(a[k], b[k], d, 0, 0, 0);
+    template <int K> static PSH_OP void step(const v4u& p, const v4u& q, acc& d) {
+        d = __builtin_amdgcn_mfma_f64_16x16x4f64(__hiloint2double((int)p[2 * K + 1], (int)p[2 * K]),
+                                                 __hiloint2double((int)q[2 * K + 1], (int)q[2 * K]), d, 0, 0, 0);
     }
 };
 
@@ -193,6 +196,15 @@ template <class T, int BI, int BJ, int WI, int WJ> struct Tile {
     acc_t acc[MI][MJ];
     acc_t ones[MI];   // sums of P over c, in every column (the bias gradient), if asked for
 
+    template <int K, bool SUMS> PSH_OP void part(const v4u (&fp)[MI], const v4u (&fq)[MJ], const v4u& unit) {
+#pragma unroll
+        for (int a = 0; a < MI; ++a) {
+#pragma unroll
+            for (int b = 0; b < MJ; ++b) Mfma<T>::template step<K>(fp[a], fq[b], acc[a][b]);
+            if constexpr (SUMS) Mfma<T>::template step<K>(fp[a], unit, ones[a]);
+        }
+    }
+
     // D += P Q^T over all c.  LDS: two buffers of (BI + BJ) * 128 bytes.
     template <bool TP, bool TQ, bool SUMS> PSH_OP void multiply(const Operand<T>& p, const Operand<T>& q, unsigned char* lds) {
         constexpr int KC = 128 / (int)sizeof(T);
@@ -205,7 +217,7 @@ template <class T, int BI, int BJ, int WI, int WJ> struct Tile {
 #pragma unroll
             for (int b = 0; b < MJ; ++b) acc[a][b] = acc_t{0, 0, 0, 0};
         }
-        v4u unit;
+        v4u unit = {0, 0, 0, 0};
         if constexpr (SUMS) {
             T e[16 / sizeof(T)];
 #pragma unroll
@@ -241,11 +253,11 @@ template <class T, int BI, int BJ, int WI, int WJ> struct Tile {
                     const int j = wj + b * 16 + l;
                     fq[b] = *reinterpret_cast<const v4u*>(cur + BI * 128 + j * 128 + unit_of<T>(j, s * 4 + g) * 16);
                 }
-#pragma unroll
-                for (int a = 0; a < MI; ++a) {
-#pragma unroll
-                    for (int b = 0; b < MJ; ++b) Mfma<T>::step(fp[a], fq[b], acc[a][b]);
-                    if constexpr (SUMS) Mfma<T>::step(fp[a], unit, ones[a]);
+                part<0, SUMS>(fp, fq, unit);
+                if constexpr (Mfma<T>::PARTS > 1) part<1, SUMS>(fp, fq, unit);
+                if constexpr (Mfma<T>::PARTS > 2) {
+                    part<2, SUMS>(fp, fq, unit);
+                    part<3, SUMS>(fp, fq, unit);
                 }
             }
             if (t + 1 < tiles) {
@@ -295,11 +307,11 @@ template <class T, int BI, int BJ, int WI, int WJ> struct Tile {
                 for (int a = 0; a < MI; ++a) fp[a] = DP::fragment(lds + cur, wi + a * 16, s);
 #pragma unroll
                 for (int b = 0; b < MJ; ++b) fq[b] = DQ::fragment(lds + cur + BI * 128, wj + b * 16, s);
-#pragma unroll
-                for (int a = 0; a < MI; ++a) {
-#pragma unroll
-                    for (int b = 0; b < MJ; ++b) Mfma<T>::step(fp[a], fq[b], acc[a][b]);
-                    if constexpr (SUMS) Mfma<T>::step(fp[a], unit, ones[a]);
+                part<0, SUMS>(fp, fq, unit);
+                if constexpr (Mfma<T>::PARTS > 1) part<1, SUMS>(fp, fq, unit);
+                if constexpr (Mfma<T>::PARTS > 2) {
+                    part<2, SUMS>(fp, fq, unit);
+                    part<3, SUMS>(fp, fq, unit);
                 }
             }
             asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
@@ -334,30 +346,35 @@ template <class T> struct RowsArgs {   // forward and dx
     T* out;                            // [rows, n_out] contiguous
     int n_in, n_out, nonlin;
     long slots, tiles_i;
-    bool wide_out;
 };
 
-// store up to four units of one row
-template <class T, class A> PSH_OP void store_units(T* row, int i, int n, const A& v, bool wide) {
-    if constexpr (sizeof(T) == 8) {
+// A result tile goes to memory through LDS (a lane holds four units of one row, and neighbouring lanes neighbouring rows, so stores
+// from registers would be pieces of 8 to 32 bytes): rows of COLS elements, 16-byte units permuted within a row by XOR with swz(row).
+template <class T, int COLS> PSH_OP T* tile_at(unsigned char* lds, int row, int col, int swz) {
+    const int byte = col * (int)sizeof(T);
+    return reinterpret_cast<T*>(lds + row * COLS * (int)sizeof(T) + (((byte >> 4) ^ swz) << 4) + (byte & 15));
+}
+template <class T, int COLS, class S> PSH_OP void store_tile(unsigned char* lds, T* out, long ld, int rows, int cols, S swz) {
+    constexpr int V = 16 / (int)sizeof(T), UNITS = COLS / V;
+    for (int id = threadIdx.x; id < rows * UNITS; id += blockDim.x) {
+        const int r = id / UNITS, c = id % UNITS * V;
+        if (c >= cols) continue;
+        const v4u v = *reinterpret_cast<const v4u*>(tile_at<T, COLS>(lds, r, c, swz(r)));
+        T* const o = out + r * ld + c;
+        if (c + V <= cols) {
+            __builtin_memcpy(o, &v, 16);
+        } else {
+            T e[V];
+            __builtin_memcpy(e, &v, 16);
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-            if (i + 4 * r < n) row[i + 4 * r] = v[r];
-    } else if (wide && i + 4 <= n) {
-        T e[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) e[r] = to_elem<T>(v[r]);
-        if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(row + i) = __builtin_bit_cast(uint2, e);
-        else *reinterpret_cast<v4u*>(row + i) = __builtin_bit_cast(v4u, e);
-    } else {
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-            if (i + r < n) row[i + r] = to_elem<T>(v[r]);
+            for (int k = 0; k < V; ++k)
+                if (c + k < cols) o[k] = e[k];
+        }
     }
 }
 
 template <class T, int BI, int BJ, int WI, int WJ, bool TW, bool DIRECT>
-__global__ __launch_bounds__(64 * WI * WJ) void k_rows(const RowsArgs<T> a) {
+__global__ __launch_bounds__(64 * WI * WJ, BI * BJ > 4096 ? 2 : 4) void k_rows(const RowsArgs<T> a) {
     extern __shared__ __align__(16) unsigned char lds[];
     const long id = xcd_order(blockIdx.x, a.slots * a.tiles_i);
     if (id >= a.slots * a.tiles_i) return;
@@ -377,17 +394,25 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_rows(const RowsArgs<T> a) {
     else tile.template multiply<TW, false, false>(p, x, lds);
     typedef typename Wide<T>::type W;
     const T* const b = a.bias ? a.bias + (long)q.part * a.stride_b + i0 : nullptr;
+    const auto swz = [](int j) { return j & (BI * (int)sizeof(T) / 16 - 1) & 15; };
     tile.each([&](int i, int j, auto v) {
-        if (j >= nj) return;
         constexpr int step = sizeof(T) == 8 ? 4 : 1;
+        T e[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             W s = v[r];
             if (b && i + step * r < ni) s += to_wide(b[i + step * r]);
-            v[r] = nonlin_w(a.nonlin, s);
+            e[r] = to_elem<T>(nonlin_w(a.nonlin, s));
         }
-        store_units(a.out + (long)(q.begin + j) * a.n_out + i0, i, ni, v, a.wide_out);
+        if constexpr (sizeof(T) == 8) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) *tile_at<T, BI>(lds, j, i + 4 * r, swz(j)) = e[r];
+        } else {
+            __builtin_memcpy(__builtin_assume_aligned(tile_at<T, BI>(lds, j, i, swz(j)), 4 * sizeof(T)), e, 4 * sizeof(T));
+        }
     });
+    __syncthreads();
+    store_tile<T, BI>(lds, a.out + (long)q.begin * a.n_out + i0, a.n_out, nj, ni, swz);
 }
 
 // dp = dy f'(y), rounded to the element type as the gradient that reaches a layer's product in any composition of
@@ -411,7 +436,7 @@ template <class T> struct GradArgs {   // dW, db
 };
 
 template <class T, int BI, int BJ, int WI, int WJ, bool DIRECT>
-__global__ __launch_bounds__(64 * WI * WJ) void k_weights(const GradArgs<T> a) {
+__global__ __launch_bounds__(64 * WI * WJ, BI * BJ > 4096 ? 2 : sizeof(T) == 2 ? 2 : 4) void k_weights(const GradArgs<T> a) {
     extern __shared__ __align__(16) unsigned char lds[];
     const long tiles = a.tiles_i * a.tiles_j, total = a.slots * tiles;
     const long id = xcd_order(blockIdx.x, total);
@@ -435,16 +460,21 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_weights(const GradArgs<T> a) {
     }
     constexpr int step = sizeof(T) == 8 ? 4 : 1;
     const long at = (long)(whole ? q.part : slot) * a.n;
-    if (a.dw) tile.each([&](int i, int j, auto v) {
-        if (j >= nj) return;
+    if (a.dw) {
+        // rows of the tile are output units here
+        const auto put = [&](auto* out) {
+            typedef typename std::remove_pointer<decltype(out)>::type O;
+            const auto swz = [](int i) { return ((i >> 2) & 3) * (int)sizeof(O); };
+            tile.each([&](int i, int j, auto v) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            if (i + step * r >= ni) continue;
-            const long o = (at + i0 + i + step * r) * a.k + j0 + j;
-            if (whole) a.dw[o] = to_elem<T>(v[r]);
-            else a.part_w[o] = v[r];
-        }
-    });
+                for (int r = 0; r < 4; ++r) *tile_at<O, BJ>(lds, i + step * r, j, swz(i + step * r)) = to_elem<O>(v[r]);
+            });
+            __syncthreads();
+            store_tile<O, BJ>(lds, out + (at + i0) * a.k + j0, a.k, ni, nj, swz);
+        };
+        if (whole) put(a.dw);
+        else put(a.part_w);
+    }
     if (sums && (threadIdx.x & 15) == 0 && (threadIdx.x >> 6) / WI == 0) {
         const int wi = ((threadIdx.x >> 6) % WI) * (BI / WI);
 #pragma unroll
@@ -533,6 +563,8 @@ int64_t grad_piece(const psh_linear_desc* d) {
     const int64_t whole = ((int64_t)d->rows + 64) / 64 * 64;
     if (tiles >= 512) return whole;
     int64_t L = ((int64_t)d->rows * tiles / 1024 + 63) / 64 * 64;
+    // (with enough groups to fill the CUs only those of twice the mean size are cut)
+    if (tiles * d->n_groups >= 512 && L < 2 * (int64_t)d->rows / d->n_groups) L = (2 * (int64_t)d->rows / d->n_groups + 63) / 64 * 64;
     if (L < 256) L = 256;
     return L < whole ? L : whole;
 }
@@ -600,7 +632,6 @@ template <class T> int forward(psh_ctx* c, const psh_linear_desc* d) {
     a.bias = (const T*)d->bias; a.stride_b = d->stride_b;
     a.out = (T*)d->y;
     a.n_in = d->in_dim; a.n_out = d->out_dim; a.nonlin = d->nonlin;
-    a.wide_out = aligned16(d->y, sizeof(T), 4) && d->out_dim % 4 == 0;
     return run_rows<T, false>(c, a, d->rows, (hipStream_t)d->stream);
 }
 
@@ -627,8 +658,7 @@ template <class T> int backward(psh_ctx* c, const psh_linear_desc* d) {
         a.weight = (const T*)d->weight; a.ld_w = d->ld_w; a.stride_w = d->stride_w;
         a.out = (T*)d->dx;
         a.n_in = d->out_dim; a.n_out = d->in_dim; a.nonlin = PSH_NL_NONE;
-        a.wide_out = aligned16(d->dx, sizeof(T), 4) && d->in_dim % 4 == 0;
-        const int rc = run_rows<T, true>(c, a, d->rows, st);
+            const int rc = run_rows<T, true>(c, a, d->rows, st);
         if (rc != PSH_OK) return rc;
     }
     if (d->dweight || d->dbias) {

@@ -157,28 +157,40 @@ template <class T, int V, int K> __global__ __launch_bounds__(256) void k_conv(c
     }
 }
 
-// one row per sequence; a thread reads its carried inputs before it writes the new ones, which may be in the same place
-template <class T, int K> __global__ __launch_bounds__(256) void k_conv_step(const ConvArgs<T> a, int n_seqs, int per_row) {
+// One row per sequence.  A wave takes step_seqs() neighbouring sequences and 64 channels: with one policy (ONE) their parameters are read
+// once.  A thread reads its carried inputs before it writes the new ones, which may be in the same place.
+template <class T> constexpr int step_seqs() { return sizeof(T) == 8 ? 2 : 4; }
+template <class T, int K, bool ONE> __global__ __launch_bounds__(256) void k_conv_step(const ConvArgs<T> a, int n_seqs, int per_row) {
     typedef typename Wide<T>::type W;
-    // 4 waves: consecutive (sequence, 64 channels) pairs
+    constexpr int STEP_SEQS = step_seqs<T>();
     const long id = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int s = (int)(id / per_row), c = (int)(id % per_row) * 64 + (threadIdx.x & 63);
-    if (s >= n_seqs) return;
-    const int p = a.pol.of(s);
-    if (c >= a.D) return;
+    const int s0 = (int)(id / per_row) * STEP_SEQS, c = (int)(id % per_row) * 64 + (threadIdx.x & 63);
+    if (s0 >= n_seqs) return;
+    const int live = min(STEP_SEQS, n_seqs - s0), cc = min(c, a.D - 1);
     W w[K], b;
-    conv_params<T, K>(w, b, a, p, c);
-    T in[K];
+    if constexpr (ONE) conv_params<T, K>(w, b, a, 0, cc);
+    T in[STEP_SEQS][K];
 #pragma unroll
-    for (int k = 0; k < K - 1; ++k) in[k] = a.state ? a.state[s * a.stride_state + (long)c * (K - 1) + k] : T(0);
-    in[K - 1] = a.x[s * a.ld_x + c];
-    W sum = b;
+    for (int i = 0; i < STEP_SEQS; ++i) {
+        const long s = s0 + min(i, live - 1);
 #pragma unroll
-    for (int k = 0; k < K; ++k) sum += w[k] * to_wide(in[k]);
-    a.y[(long)s * a.D + c] = to_elem<T>(a.silu ? silu_w(sum) : sum);
-    if (a.last)
+        for (int k = 0; k < K - 1; ++k) in[i][k] = a.state ? a.state[s * a.stride_state + (long)cc * (K - 1) + k] : T(0);
+        in[i][K - 1] = a.x[s * a.ld_x + cc];
+    }
 #pragma unroll
-        for (int k = 0; k < K - 1; ++k) a.last[s * a.stride_last + (long)c * (K - 1) + k] = in[k + 1];
+    for (int i = 0; i < STEP_SEQS; ++i) {
+        if (i >= live) break;
+        const long s = s0 + i;
+        if constexpr (!ONE) conv_params<T, K>(w, b, a, a.pol.of((int)s), cc);
+        if (c >= a.D) continue;
+        W sum = b;
+#pragma unroll
+        for (int k = 0; k < K; ++k) sum += w[k] * to_wide(in[i][k]);
+        a.y[s * a.D + c] = to_elem<T>(a.silu ? silu_w(sum) : sum);
+        if (a.last)
+#pragma unroll
+            for (int k = 0; k < K - 1; ++k) a.last[s * a.stride_last + (long)c * (K - 1) + k] = in[i][k + 1];
+    }
 }
 
 // dx[t] = sum_k w[k] dpre[t + K-1-k],  dw[k] = sum_t dpre[t] x[t - (K-1) + k],  db = sum_t dpre[t],  dpre = dy f'(pre).
@@ -422,6 +434,7 @@ template <class T> struct ScanArgs {
     const int* order;        // sequences from the longest to the shortest, NULL: as they come
     int blocks;              // channel blocks
     bool vec_d, vec_n;       // wide loads of channel rows / of states
+    bool vec_bc;             // and of rows of B and C (single steps)
     // gradients
     const T* dy; long ld_dy;
     const W* dlast;
@@ -1056,44 +1069,70 @@ template <class T> __global__ __launch_bounds__(256) void k_sum_bc(const typenam
 }
 
 // One step of every sequence: states read and written once, 4 lanes per channel with 4 neighbouring states each, 16
-// states per turn of the loop.  `last` may be `state`.
-template <class T> __global__ __launch_bounds__(256) void k_scan_step(const ScanArgs<T> a, int n_seqs, int per_row) {
+// states per turn of the loop, step_seqs() neighbouring sequences a wave, whose loads are in flight together.  `last` may be `state`.
+template <class T, bool ONE> __global__ __launch_bounds__(256) void k_scan_step(const ScanArgs<T> a, int n_seqs, int per_row) {
     typedef typename Wide<T>::type W;
+    constexpr int STEP_SEQS = step_seqs<T>();
     const long id = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int s = (int)(id / per_row);
-    if (s >= n_seqs) return;
-    const int lane = threadIdx.x & 63, ql = lane & 3;
+    const int s0 = (int)(id / per_row) * STEP_SEQS;
+    if (s0 >= n_seqs) return;
+    const int lane = threadIdx.x & 63, ql = lane & 3, live = min(STEP_SEQS, n_seqs - s0);
     const int d = (int)(id % per_row) * 16 + lane / 4;
-    const int p = a.pol.of(s);
-    if (d >= a.D) return;   // (whole quads)
-    const long pd = (long)p * a.D + d;
-    const W u = to_wide(a.u[s * a.ld_u + d]);
-    const W dt = softplus_w(to_wide(a.delta[s * a.ld_delta + d]) + (a.bias ? a.bias[pd] : W(0)));
-    const W dtu = dt * u;
-    W y = 0;
-    for (int n = ql * 4; n < a.N; n += 16) {
-        W h[4], A[4], b[4], c[4];
+    const bool in = d < a.D;
+    const int dd = min(d, a.D - 1);
+    long pd[STEP_SEQS];      // the parameters' row
+    W u[STEP_SEQS], dt[STEP_SEQS], y[STEP_SEQS];
+    T raw_u[STEP_SEQS], raw_dt[STEP_SEQS], raw_z[STEP_SEQS];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) h[i] = 0;
-        if (a.state) load_line<4>(h, a.state + s * a.stride_state + (long)d * a.N, n, a.N, a.vec_n);
-        load_line<4>(A, a.A + pd * a.N, n, a.N, a.vec_n);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            b[i] = n + i < a.N ? to_wide(a.B[s * a.ld_B + n + i]) : W(0);
-            c[i] = n + i < a.N ? to_wide(a.C[s * a.ld_C + n + i]) : W(0);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            h[i] = decay(dt, decay_rate(A[i])) * h[i] + dtu * b[i];
-            y += c[i] * h[i];
-        }
-        if (a.last) store_line<4>(a.last + s * a.stride_last + (long)d * a.N, h, n, a.N, a.vec_n);
+    for (int i = 0; i < STEP_SEQS; ++i) {
+        const long s = s0 + min(i, live - 1);
+        pd[i] = (ONE ? 0L : (long)a.pol.of((int)s) * a.D) + dd;
+        raw_u[i] = a.u[s * a.ld_u + dd];
+        raw_dt[i] = a.delta[s * a.ld_delta + dd];
+        raw_z[i] = a.z ? a.z[s * a.ld_z + dd] : T(0);
+        y[i] = 0;
     }
-    y = sum_states<4>(y);
-    if (ql == 0) {
-        if (a.skip) y += a.skip[pd] * u;
-        if (a.z) y *= silu_w(to_wide(a.z[s * a.ld_z + d]));
-        a.y[(long)s * a.D + d] = to_elem<T>(y);
+    for (int n = ql * 4; n < a.N; n += 16) {
+        W h[STEP_SEQS][4], A[4], b[STEP_SEQS][4], c[STEP_SEQS][4];
+#pragma unroll
+        for (int i = 0; i < STEP_SEQS; ++i) {
+            const long s = s0 + min(i, live - 1);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) h[i][k] = 0;
+            if (a.state) load_line<4>(h[i], a.state + s * a.stride_state + (long)dd * a.N, n, a.N, a.vec_n);
+            load_line<4>(b[i], a.B + s * a.ld_B, n, a.N, a.vec_bc);
+            load_line<4>(c[i], a.C + s * a.ld_C, n, a.N, a.vec_bc);
+        }
+        if constexpr (ONE) load_line<4>(A, a.A + (long)dd * a.N, n, a.N, a.vec_n);
+        if (n < 16) {
+#pragma unroll
+            for (int i = 0; i < STEP_SEQS; ++i) {
+                u[i] = to_wide(raw_u[i]);
+                dt[i] = softplus_w(to_wide(raw_dt[i]) + (a.bias ? a.bias[pd[i]] : W(0)));
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < STEP_SEQS; ++i) {
+            if constexpr (!ONE) load_line<4>(A, a.A + pd[i] * a.N, n, a.N, a.vec_n);
+            const W dtu = dt[i] * u[i];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                h[i][k] = decay(dt[i], decay_rate(A[k])) * h[i][k] + dtu * b[i][k];
+                y[i] += c[i][k] * h[i][k];
+            }
+            step_fence<W, 4>();
+            if (a.last && in && i < live) store_line<4>(a.last + (s0 + i) * a.stride_last + (long)d * a.N, h[i], n, a.N, a.vec_n);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < STEP_SEQS; ++i) {
+        if (i >= live) break;
+        W v = sum_states<4>(y[i]);
+        if (ql == i % 4 && in) {
+            if (a.skip) v += a.skip[pd[i]] * to_wide(raw_u[i]);
+            if (a.z) v *= silu_w(to_wide(raw_z[i]));
+            a.y[(long)(s0 + i) * a.D + d] = to_elem<T>(v);
+        }
     }
 }
 
@@ -1127,7 +1166,7 @@ ScanPlan scan_plan(const psh_scan_desc* d, bool grad) {
     if (with(least) < 512) {
         if (d->rows > 192 * (int64_t)d->n_seqs) {
             p.piece = (int64_t)d->rows * p.blocks / 1024 / ts * ts;
-            if (p.piece < 64) p.piece = 64;
+            if (p.piece < 32) p.piece = 32;
             if (p.piece > whole) p.piece = whole;
         } else {
             while (lpc < widest && with(lpc) < 512) lpc *= 2;
@@ -1260,9 +1299,12 @@ template <class T> int run_scan(psh_ctx* c, const psh_scan_desc* d) {
         a.check = nullptr;
         scan_alignment(a, false);
         const int per_row = (a.D + 15) / 16;
-        const long blocks = ((long)d->n_seqs * per_row + 3) / 4;
+        const int64_t e = 4 * sizeof(T);
+        a.vec_bc = a.N % 4 == 0 && aligned(a.B, e, a.ld_B * sizeof(T)) && aligned(a.C, e, a.ld_C * sizeof(T));
+        const long blocks = (((long)d->n_seqs + step_seqs<T>() - 1) / step_seqs<T>() * per_row + 3) / 4;
         if (blocks > 0x7fffffffL) return too_large(c, "selective_scan");
-        hipLaunchKernelGGL(k_scan_step<T>, dim3((unsigned)blocks), dim3(256), 0, st, a, (int)d->n_seqs, per_row);
+        if (a.pol.n == 1) hipLaunchKernelGGL((k_scan_step<T, true>), dim3((unsigned)blocks), dim3(256), 0, st, a, (int)d->n_seqs, per_row);
+        else hipLaunchKernelGGL((k_scan_step<T, false>), dim3((unsigned)blocks), dim3(256), 0, st, a, (int)d->n_seqs, per_row);
         PSH_HIP(c, hipGetLastError());
         return PSH_OK;
     }
@@ -1405,9 +1447,10 @@ template <class T, int K> int run_conv(psh_ctx* c, const psh_conv_desc* d, bool 
     a.D = d->channels; a.silu = d->silu;
     if (d->step) {
         const int per_row = (a.D + 63) / 64;
-        const long blocks = ((long)d->n_seqs * per_row + 3) / 4;
+        const long blocks = (((long)d->n_seqs + step_seqs<T>() - 1) / step_seqs<T>() * per_row + 3) / 4;
         if (blocks > 0x7fffffffL) return too_large(c, "causal_conv");
-        hipLaunchKernelGGL((k_conv_step<T, K>), dim3((unsigned)blocks), dim3(256), 0, st, a, (int)d->n_seqs, per_row);
+        if (a.pol.n == 1) hipLaunchKernelGGL((k_conv_step<T, K, true>), dim3((unsigned)blocks), dim3(256), 0, st, a, (int)d->n_seqs, per_row);
+        else hipLaunchKernelGGL((k_conv_step<T, K, false>), dim3((unsigned)blocks), dim3(256), 0, st, a, (int)d->n_seqs, per_row);
         PSH_HIP(c, hipGetLastError());
         return PSH_OK;
     }
