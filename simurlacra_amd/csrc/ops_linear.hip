@@ -11,8 +11,7 @@
 // In LDS both operands lie as [index][128 bytes of c], whichever way they are laid out in memory; a lane's fragment is 16
 // bytes along c, so 8 bf16 are one operand of v_mfma_f32_16x16x32_bf16, 4 floats those of four v_mfma_f32_16x16x4_f32 and 2
 // doubles those of two v_mfma_f64_16x16x4_f64 (c is summed over, so which c meets in which instruction is free as long as
-// P and Q agree).  The 16-byte units of an index are permuted by XOR with (index ^ index / 8) & 7: 8 neighbouring
-// indices (fragment reads) and 8 indices 8 apart (transposing writes) lie in different banks.
+// P and Q agree).  The 16-byte units of an index are permuted, see unit_of.
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
@@ -64,51 +63,79 @@ template <class T> PSH_OP v4u load16(const T* p) {
     return v;
 }
 
-template <class T> PSH_OP int unit_of(int i, int u) { return u ^ ((i ^ (i >> 3)) & 7); }
+// The 16-byte units of an index are permuted: 16 neighbouring indices, which a fragment read takes at a time, lie two to a row of 64 banks
+// in 8 different units, and so do indices V apart, which the transposing writes take.
+PSH_OP int unit_of(int i, int u) { return u ^ (((i >> 1) ^ (i >> 4)) & 7); }
 
 // One thread's part of a tile of N indices x 8 units of 16 bytes: loaded into registers while the previous tile is being
-// multiplied, stored to LDS afterwards.
+// multiplied, stored to LDS afterwards.  Indices past the operand's end are read as whatever lies there within the operand (their results
+// are not stored); c past its end are zeros.
 template <class T, int N, int THREADS, bool TR> struct Stager {
-    static constexpr int V = 16 / (int)sizeof(T);
+    static constexpr int V = 16 / (int)sizeof(T), KC = 128 / (int)sizeof(T);
     static constexpr int WORK = TR ? (N / V) * 8 : N * 8;                 // V x V blocks, or units
     static constexpr int PER = (WORK + THREADS - 1) / THREADS;
     static constexpr int REGS = TR ? PER * V : PER;
     v4u r[REGS];
+    const T* at[PER];   // line (block) of c = 0
 
-    static PSH_OP v4u load(const Operand<T>& o, const T* q, int first, int limit) {
-        // elements [first, first + V) of a line with `limit` valid ones
-        if (first >= limit) return v4u{0, 0, 0, 0};
-        if (first + V <= limit) return load16(q + first);
-        T e[V];
+    PSH_OP explicit Stager(const Operand<T>& o) {
 #pragma unroll
-        for (int k = 0; k < V; ++k) e[k] = first + k < limit ? q[first + k] : T(0);
-        return __builtin_bit_cast(v4u, e);
+        for (int k = 0; k < PER; ++k) {
+            const int id = (int)threadIdx.x + k * THREADS;
+            if constexpr (!TR) at[k] = o.p + (long)min(id >> 3, o.n - 1) * o.ld + (id & 7) * V;
+            else at[k] = o.p + (long)(id / (N / V) * V) * o.ld + min(id % (N / V) * V, (o.n - 1) / V * V);
+        }
+    }
+    // whether the tile from c0 can be read in whole units.  A transposed operand's last unit may run over its line's end, by up to V - 1
+    // elements: that many have to follow in the operand.
+    static PSH_OP bool whole(const Operand<T>& o, int c0) {
+        return c0 + KC <= o.nc && (!TR || o.n % V == 0 || (long)(o.nc - c0 - KC) * o.ld >= V - 1);
     }
     PSH_OP void fetch(const Operand<T>& o, int c0) {
+        if (whole(o, c0)) {
+#pragma unroll
+            for (int k = 0; k < PER; ++k) {
+                if (WORK % THREADS != 0 && (int)threadIdx.x + k * THREADS >= WORK) break;
+                if constexpr (!TR) {
+                    r[k] = load16(at[k] + c0);
+                } else {
+                    const T* const q = at[k] + (long)c0 * o.ld;
+#pragma unroll
+                    for (int j = 0; j < V; ++j) r[k * V + j] = load16(q + j * o.ld);
+                }
+            }
+            return;
+        }
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
             const int id = (int)threadIdx.x + k * THREADS;
             if constexpr (!TR) {
-                const int i = id >> 3, u = id & 7;
-                r[k] = i < o.n && id < WORK ? load(o, o.p + i * o.ld, c0 + u * V, o.nc) : v4u{0, 0, 0, 0};
+                r[k] = piece(o.p + (long)min(id >> 3, o.n - 1) * o.ld, c0 + (id & 7) * V, o.nc);
             } else {
                 const int ib = id % (N / V), u = id / (N / V);
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
                     const int c = c0 + u * V + j;
-                    r[k * V + j] = c < o.nc && id < WORK ? load(o, o.p + (long)c * o.ld, ib * V, o.n) : v4u{0, 0, 0, 0};
+                    r[k * V + j] = c < o.nc && id < WORK ? piece(o.p + (long)c * o.ld, ib * V, o.n) : v4u{0, 0, 0, 0};
                 }
             }
         }
+    }
+    // elements [first, first + V) of a line with `limit` valid ones
+    static PSH_OP v4u piece(const T* line, int first, int limit) {
+        T e[V];
+#pragma unroll
+        for (int k = 0; k < V; ++k) e[k] = first + k < limit ? line[first + k] : T(0);
+        return __builtin_bit_cast(v4u, e);
     }
     PSH_OP void store(unsigned char* lds) const {
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
             const int id = (int)threadIdx.x + k * THREADS;
-            if (id >= WORK) continue;
+            if (WORK % THREADS != 0 && id >= WORK) break;
             if constexpr (!TR) {
                 const int i = id >> 3, u = id & 7;
-                *reinterpret_cast<v4u*>(lds + i * 128 + unit_of<T>(i, u) * 16) = r[k];
+                *reinterpret_cast<v4u*>(lds + i * 128 + unit_of(i, u) * 16) = r[k];
             } else {
                 const int ib = id % (N / V), u = id / (N / V);
 #pragma unroll
@@ -121,7 +148,7 @@ template <class T, int N, int THREADS, bool TR> struct Stager {
                         e[m] = line[j];
                     }
                     const int i = ib * V + j;
-                    *reinterpret_cast<v4u*>(lds + i * 128 + unit_of<T>(i, u) * 16) = __builtin_bit_cast(v4u, e);
+                    *reinterpret_cast<v4u*>(lds + i * 128 + unit_of(i, u) * 16) = __builtin_bit_cast(v4u, e);
                 }
             }
         }
@@ -131,12 +158,13 @@ template <class T, int N, int THREADS, bool TR> struct Stager {
 // A bf16 operand's tiles by loads that go to LDS directly: no registers, no transposing on the way in.  The tile lies as it is in memory, [index][64 c]
 // or, for a transposed operand, [64 c][index], where ds_read_b64_tr_b16 does the transposing: 16 lanes, four to a row of 16 indices, read 4
 // rows, and lane i gets column i.  The loads go to LDS in lane order, so the permutation that spreads the banks is applied
-// to the addresses they read from: 16-byte units by the index as in Stager, or 32-byte chunks of a row by (c ^ c / 8) & 7.
+// to the addresses they read from: 16-byte units by the index as in Stager, or 32-byte chunks of a row by c, so that the 8
+// rows that half a wave reads at a time are in different banks.
 // Rows past the operand's end are read as its last one (their results are not stored); only whole tiles of c come this way.
 template <int N, int THREADS, bool TR> struct Direct {
     static constexpr int WAVES = THREADS / 64, PER = N * 128 / 1024 / WAVES;   // 1-KiB loads of a wave
-    static constexpr int ROW = N * 2, SWZ = N >= 128 ? 7 : 3;                  // transposed: bytes and permutation of a row
-    static PSH_OP int swz(int c) { return (c ^ (c >> 3)) & SWZ; }
+    static constexpr int ROW = N * 2;                                          // transposed: bytes of a row
+    static PSH_OP int swz(int c) { return (c & 3) | ((c >> 1) & 4); }
     static PSH_OP void fetch(const Operand<bf16_t>& o, int c0, unsigned lds) {
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
@@ -144,7 +172,7 @@ template <int N, int THREADS, bool TR> struct Direct {
             const int chunk = __builtin_amdgcn_readfirstlane(wave + k * WAVES);
             const bf16_t* g;
             if constexpr (!TR) {
-                const int i = chunk * 8 + (lane >> 3), u = (lane & 7) ^ ((i ^ (i >> 3)) & 7);
+                const int i = chunk * 8 + (lane >> 3), u = unit_of(i, lane & 7);
                 g = o.p + (long)min(i, o.n - 1) * o.ld + c0 + u * 8;
             } else {
                 const int at = chunk * 1024 + lane * 16, c = at / ROW, u = (at % ROW / 16) ^ (swz(c) << 1);
@@ -158,7 +186,7 @@ template <int N, int THREADS, bool TR> struct Direct {
     // the last, partial tile of c through registers, zero where there is none
     static PSH_OP void fetch_tail(const Operand<bf16_t>& o, int c0, unsigned char* lds) {
         if constexpr (!TR) {
-            Stager<bf16_t, N, THREADS, false> st;
+            Stager<bf16_t, N, THREADS, false> st(o);
             st.fetch(o, c0);
             st.store(lds);
         } else {
@@ -174,7 +202,7 @@ template <int N, int THREADS, bool TR> struct Direct {
         const int l = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
         if constexpr (!TR) {
             const int i = i0 + l;
-            return *reinterpret_cast<const v4u*>(lds + i * 128 + (((s * 4 + g) ^ (i ^ (i >> 3))) & 7) * 16);
+            return *reinterpret_cast<const v4u*>(lds + i * 128 + unit_of(i, s * 4 + g) * 16);
         } else {
             typedef short v4s __attribute__((ext_vector_type(4)));
             typedef __attribute__((address_space(3))) v4s* at_t;
@@ -224,10 +252,10 @@ template <class T, int BI, int BJ, int WI, int WJ> struct Tile {
             for (int k = 0; k < (int)(16 / sizeof(T)); ++k) e[k] = to_elem<T>(1);
             unit = __builtin_bit_cast(v4u, e);
         }
-        Stager<T, BI, THREADS, TP> sp;
-        Stager<T, BJ, THREADS, TQ> sq;
         const int nc = p.nc, tiles = (nc + KC - 1) / KC;
         if (tiles <= 0) return;
+        Stager<T, BI, THREADS, TP> sp(p);
+        Stager<T, BJ, THREADS, TQ> sq(q);
         sp.fetch(p, 0);
         sq.fetch(q, 0);
         sp.store(lds);
@@ -246,12 +274,12 @@ template <class T, int BI, int BJ, int WI, int WJ> struct Tile {
 #pragma unroll
                 for (int a = 0; a < MI; ++a) {
                     const int i = wi + a * 16 + l;
-                    fp[a] = *reinterpret_cast<const v4u*>(cur + i * 128 + unit_of<T>(i, s * 4 + g) * 16);
+                    fp[a] = *reinterpret_cast<const v4u*>(cur + i * 128 + unit_of(i, s * 4 + g) * 16);
                 }
 #pragma unroll
                 for (int b = 0; b < MJ; ++b) {
                     const int j = wj + b * 16 + l;
-                    fq[b] = *reinterpret_cast<const v4u*>(cur + BI * 128 + j * 128 + unit_of<T>(j, s * 4 + g) * 16);
+                    fq[b] = *reinterpret_cast<const v4u*>(cur + BI * 128 + j * 128 + unit_of(j, s * 4 + g) * 16);
                 }
                 part<0, SUMS>(fp, fq, unit);
                 if constexpr (Mfma<T>::PARTS > 1) part<1, SUMS>(fp, fq, unit);
@@ -374,7 +402,7 @@ template <class T, int COLS, class S> PSH_OP void store_tile(unsigned char* lds,
 }
 
 template <class T, int BI, int BJ, int WI, int WJ, bool TW, bool DIRECT>
-__global__ __launch_bounds__(64 * WI * WJ, BI * BJ > 4096 ? 2 : 4) void k_rows(const RowsArgs<T> a) {
+__global__ __launch_bounds__(64 * WI * WJ, BI * BJ > 4096 ? 2 : sizeof(T) == 2 && TW ? 3 : 4) void k_rows(const RowsArgs<T> a) {
     extern __shared__ __align__(16) unsigned char lds[];
     const long id = xcd_order(blockIdx.x, a.slots * a.tiles_i);
     if (id >= a.slots * a.tiles_i) return;
@@ -395,22 +423,31 @@ __global__ __launch_bounds__(64 * WI * WJ, BI * BJ > 4096 ? 2 : 4) void k_rows(c
     typedef typename Wide<T>::type W;
     const T* const b = a.bias ? a.bias + (long)q.part * a.stride_b + i0 : nullptr;
     const auto swz = [](int j) { return j & (BI * (int)sizeof(T) / 16 - 1) & 15; };
-    tile.each([&](int i, int j, auto v) {
-        constexpr int step = sizeof(T) == 8 ? 4 : 1;
-        T e[4];
+    constexpr int step = sizeof(T) == 8 ? 4 : 1;
+    const auto finish = [&](auto f) {
+        W bias[4];
+        int bias_of = -1;
+        tile.each([&](int i, int j, auto v) {
+            if (i != bias_of) {   // (the units change in the outer loop of each())
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            W s = v[r];
-            if (b && i + step * r < ni) s += to_wide(b[i + step * r]);
-            e[r] = to_elem<T>(nonlin_w(a.nonlin, s));
-        }
-        if constexpr (sizeof(T) == 8) {
+                for (int r = 0; r < 4; ++r) bias[r] = b ? to_wide(b[min(i + step * r, ni - 1)]) : W(0);
+                bias_of = i;
+            }
+            T e[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) *tile_at<T, BI>(lds, j, i + 4 * r, swz(j)) = e[r];
-        } else {
-            __builtin_memcpy(__builtin_assume_aligned(tile_at<T, BI>(lds, j, i, swz(j)), 4 * sizeof(T)), e, 4 * sizeof(T));
-        }
-    });
+            for (int r = 0; r < 4; ++r) e[r] = to_elem<T>(f((W)(v[r] + bias[r])));
+            if constexpr (sizeof(T) == 8) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) *tile_at<T, BI>(lds, j, i + 4 * r, swz(j)) = e[r];
+            } else {
+                __builtin_memcpy(__builtin_assume_aligned(tile_at<T, BI>(lds, j, i, swz(j)), 4 * sizeof(T)), e, 4 * sizeof(T));
+            }
+        });
+    };
+    if (a.nonlin == PSH_NL_TANH) finish([](W x) { return tanh_w(x); });
+    else if (a.nonlin == PSH_NL_SIGMOID) finish([](W x) { return sigmoid_w(x); });
+    else if (a.nonlin == PSH_NL_RELU) finish([](W x) { return x <= W(0) ? W(0) : x; });   // a NaN stays one
+    else finish([](W x) { return x; });
     __syncthreads();
     store_tile<T, BI>(lds, a.out + (long)q.begin * a.n_out + i0, a.n_out, nj, ni, swz);
 }
@@ -436,7 +473,7 @@ template <class T> struct GradArgs {   // dW, db
 };
 
 template <class T, int BI, int BJ, int WI, int WJ, bool DIRECT>
-__global__ __launch_bounds__(64 * WI * WJ, BI * BJ > 4096 ? 2 : sizeof(T) == 2 ? 2 : 4) void k_weights(const GradArgs<T> a) {
+__global__ __launch_bounds__(64 * WI * WJ, BI * BJ > 4096 || sizeof(T) == 2 ? 2 : sizeof(T) == 4 ? 3 : 4) void k_weights(const GradArgs<T> a) {
     extern __shared__ __align__(16) unsigned char lds[];
     const long tiles = a.tiles_i * a.tiles_j, total = a.slots * tiles;
     const long id = xcd_order(blockIdx.x, total);
@@ -465,12 +502,21 @@ __global__ __launch_bounds__(64 * WI * WJ, BI * BJ > 4096 ? 2 : sizeof(T) == 2 ?
         const auto put = [&](auto* out) {
             typedef typename std::remove_pointer<decltype(out)>::type O;
             const auto swz = [](int i) { return ((i >> 2) & 3) * (int)sizeof(O); };
-            tile.each([&](int i, int j, auto v) {
+            // as many rows at a time as the two buffers of operands hold
+            constexpr int ROOM = 2 * (BI + BJ) * 128 / (BJ * (int)sizeof(O)), ROWS = ROOM < BI ? ROOM : BI;
+            static_assert(BI % ROWS == 0 && ROWS % 16 == 0, "whole blocks of a matrix instruction's rows");
+            for (int first = 0; first < BI; first += ROWS) {
+                if (first > 0) __syncthreads();
+                tile.each([&](int i, int j, auto v) {
+                    if (ROWS < BI && (i < first || i >= first + ROWS)) return;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) *tile_at<O, BJ>(lds, i + step * r, j, swz(i + step * r)) = to_elem<O>(v[r]);
-            });
-            __syncthreads();
-            store_tile<O, BJ>(lds, out + (at + i0) * a.k + j0, a.k, ni, nj, swz);
+                    for (int r = 0; r < 4; ++r)
+                        *tile_at<O, BJ>(lds, i - first + step * r, j, swz(i + step * r)) = to_elem<O>(v[r]);
+                });
+                __syncthreads();
+                if (first < ni)
+                    store_tile<O, BJ>(lds, out + (at + i0 + first) * a.k + j0, a.k, min(ROWS, ni - first), nj, swz);
+            }
         };
         if (whole) put(a.dw);
         else put(a.part_w);
@@ -542,6 +588,8 @@ template <class T, bool TW> int run_rows(psh_ctx* c, RowsArgs<T>& a, int rows, h
         if (mean >= 96 && a.n_out > 64 && large >= 192) {
             if constexpr (sizeof(T) == 2) {
                 const bool direct = aligned16(a.rows_in, 2, a.ld_in) && aligned16(a.weight, 2, a.ld_w, a.stride_w) && (!TW || a.n_out % 8 == 0);
+                const long huge = ((long)rows / 256 + a.parts.n / 2) * ((a.n_out + 255) / 256);
+                if (direct && mean >= 512 && a.n_out > 128 && huge >= 384) return launch_rows<T, 256, 256, 2, 4, TW, true>(c, a, rows, st);
                 if (direct) return launch_rows<T, 128, 128, 2, 2, TW, true>(c, a, rows, st);
             }
             return launch_rows<T, 128, 128, 2, 2, TW, false>(c, a, rows, st);
@@ -550,10 +598,16 @@ template <class T, bool TW> int run_rows(psh_ctx* c, RowsArgs<T>& a, int rows, h
     return launch_rows<T, 64, 64, 2, 2, TW, false>(c, a, rows, st);
 }
 
+// whether the weight gradient's bf16 operands can come by direct loads (dp is the caller's dy, or contiguous in the workspace)
+bool grad_direct(const psh_linear_desc* d) {
+    return (d->nonlin != PSH_NL_NONE || aligned16(d->dy, 2, d->ld_dy)) && aligned16(d->x, 2, d->ld_x) && d->out_dim % 8 == 0 && d->in_dim % 8 == 0;
+}
 // the weight gradient's tile: [out units][in units]
 int grad_tile(const psh_linear_desc* d) {
     if (d->dtype == PSH_F64 || d->out_dim <= 64 || d->in_dim <= 64) return 64;
     const int64_t tiles = (int64_t)((d->out_dim + 127) / 128) * ((d->in_dim + 127) / 128);
+    const int64_t huge = (int64_t)((d->out_dim + 255) / 256) * ((d->in_dim + 255) / 256);
+    if (d->dtype == PSH_BF16 && grad_direct(d) && d->out_dim > 128 && d->in_dim > 128 && huge * (d->rows / 2048 + d->n_groups) >= 384) return 256;
     return tiles * (d->rows / 2048 + d->n_groups) >= 192 ? 128 : 64;
 }
 // rows of one piece of the weight gradient's contraction: enough pieces for about four workgroups a CU
@@ -561,10 +615,9 @@ int64_t grad_piece(const psh_linear_desc* d) {
     const int t = grad_tile(d);
     const int64_t tiles = (int64_t)((d->out_dim + t - 1) / t) * ((d->in_dim + t - 1) / t);
     const int64_t whole = ((int64_t)d->rows + 64) / 64 * 64;
-    if (tiles >= 512) return whole;
-    int64_t L = ((int64_t)d->rows * tiles / 1024 + 63) / 64 * 64;
-    // (with enough groups to fill the CUs only those of twice the mean size are cut)
-    if (tiles * d->n_groups >= 512 && L < 2 * (int64_t)d->rows / d->n_groups) L = (2 * (int64_t)d->rows / d->n_groups + 63) / 64 * 64;
+    const int64_t wanted = t == 256 ? 512 : 1024;
+    if (tiles >= wanted / 2) return whole;
+    int64_t L = ((int64_t)d->rows * tiles / wanted + 63) / 64 * 64;
     if (L < 256) L = 256;
     return L < whole ? L : whole;
 }
@@ -675,8 +728,9 @@ template <class T> int backward(psh_ctx* c, const psh_linear_desc* d) {
         } else if (grad_tile(d) == 64) {
             rc = launch_weights<T, 64, 2, 2, false>(c, a, d->rows, st);
         } else if constexpr (sizeof(T) == 2) {
-            const bool direct = aligned16(dp, 2, ld_dp) && aligned16(d->x, 2, d->ld_x) && a.n % 8 == 0 && a.k % 8 == 0;
-            rc = direct ? launch_weights<T, 128, 2, 2, true>(c, a, d->rows, st) : launch_weights<T, 128, 2, 2, false>(c, a, d->rows, st);
+            if (!grad_direct(d)) rc = launch_weights<T, 128, 2, 2, false>(c, a, d->rows, st);
+            else if (grad_tile(d) == 128) rc = launch_weights<T, 128, 2, 2, true>(c, a, d->rows, st);
+            else rc = launch_weights<T, 256, 2, 4, true>(c, a, d->rows, st);
         } else {
             rc = launch_weights<T, 128, 2, 2, false>(c, a, d->rows, st);
         }

@@ -83,12 +83,6 @@ PSH_OP double masked(double x, int mask) { return __hiloint2double(__double2hiin
 PSH_OP float tanh_w(float x) { return tanhf(x); }
 PSH_OP double tanh_w(double x) { return psh_tanh(x); }
 
-template <class W> PSH_OP W nonlin_w(int kind, W x) {
-    if (kind == PSH_NL_TANH) return tanh_w(x);
-    if (kind == PSH_NL_SIGMOID) return sigmoid_w(x);
-    if (kind == PSH_NL_RELU) return x <= W(0) ? W(0) : x;  // a NaN stays one
-    return x;
-}
 // derivative of the nonlinearity from its value
 template <class W> PSH_OP W nonlin_slope_w(int kind, W y) {
     if (kind == PSH_NL_TANH) return W(1) - y * y;
