@@ -270,6 +270,7 @@ template <class T, int BI, int BJ, int WI, int WJ> struct Tile {
             }
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
+                if (s == 1 && nc - t * KC <= KC / 2) break;   // nothing but zeros in the second half
                 v4u fp[MI], fq[MJ];
 #pragma unroll
                 for (int a = 0; a < MI; ++a) {
@@ -583,15 +584,12 @@ template <class T, int BI, int BJ, int WI, int WJ, bool TW, bool DIRECT> int lau
 template <class T, bool TW> int run_rows(psh_ctx* c, RowsArgs<T>& a, int rows, hipStream_t st) {
     const long mean = rows / a.parts.n;
     if (mean <= 24) return launch_rows<T, 64, 16, 4, 1, TW, false>(c, a, rows, st);
-    if constexpr (sizeof(T) < 8) {
-        const long large = ((long)rows / 128 + a.parts.n / 2) * ((a.n_out + 127) / 128);
+    if constexpr (sizeof(T) == 2) {
+        const long large = ((long)rows / 128 + a.parts.n / 2) * ((a.n_out + 127) / 128), huge = ((long)rows / 256 + a.parts.n / 2) * ((a.n_out + 255) / 256);
         if (mean >= 96 && a.n_out > 64 && large >= 192) {
-            if constexpr (sizeof(T) == 2) {
-                const bool direct = aligned16(a.rows_in, 2, a.ld_in) && aligned16(a.weight, 2, a.ld_w, a.stride_w) && (!TW || a.n_out % 8 == 0);
-                const long huge = ((long)rows / 256 + a.parts.n / 2) * ((a.n_out + 255) / 256);
-                if (direct && mean >= 512 && a.n_out > 128 && huge >= 384) return launch_rows<T, 256, 256, 2, 4, TW, true>(c, a, rows, st);
-                if (direct) return launch_rows<T, 128, 128, 2, 2, TW, true>(c, a, rows, st);
-            }
+            const bool direct = aligned16(a.rows_in, 2, a.ld_in) && aligned16(a.weight, 2, a.ld_w, a.stride_w) && (!TW || a.n_out % 8 == 0);
+            if (direct && mean >= 512 && a.n_out > 128 && huge >= 384) return launch_rows<T, 256, 256, 2, 4, TW, true>(c, a, rows, st);
+            if (direct) return launch_rows<T, 128, 128, 2, 2, TW, true>(c, a, rows, st);
             return launch_rows<T, 128, 128, 2, 2, TW, false>(c, a, rows, st);
         }
     }
@@ -604,10 +602,10 @@ bool grad_direct(const psh_linear_desc* d) {
 }
 // the weight gradient's tile: [out units][in units]
 int grad_tile(const psh_linear_desc* d) {
-    if (d->dtype == PSH_F64 || d->out_dim <= 64 || d->in_dim <= 64) return 64;
+    if (d->dtype != PSH_BF16 || d->out_dim <= 64 || d->in_dim <= 64) return 64;
     const int64_t tiles = (int64_t)((d->out_dim + 127) / 128) * ((d->in_dim + 127) / 128);
     const int64_t huge = (int64_t)((d->out_dim + 255) / 256) * ((d->in_dim + 255) / 256);
-    if (d->dtype == PSH_BF16 && grad_direct(d) && d->out_dim > 128 && d->in_dim > 128 && huge * (d->rows / 2048 + d->n_groups) >= 384) return 256;
+    if (grad_direct(d) && d->out_dim > 128 && d->in_dim > 128 && huge * (d->rows / 2048 + d->n_groups) >= 384) return 256;
     return tiles * (d->rows / 2048 + d->n_groups) >= 192 ? 128 : 64;
 }
 // rows of one piece of the weight gradient's contraction: enough pieces for about four workgroups a CU
@@ -615,10 +613,10 @@ int64_t grad_piece(const psh_linear_desc* d) {
     const int t = grad_tile(d);
     const int64_t tiles = (int64_t)((d->out_dim + t - 1) / t) * ((d->in_dim + t - 1) / t);
     const int64_t whole = ((int64_t)d->rows + 64) / 64 * 64;
-    const int64_t wanted = t == 256 ? 512 : 1024;
+    const int64_t wanted = t == 256 ? 512 : t == 128 ? 1024 : 2048;
     if (tiles >= wanted / 2) return whole;
     int64_t L = ((int64_t)d->rows * tiles / wanted + 63) / 64 * 64;
-    if (L < 256) L = 256;
+    if (L < 128) L = 128;
     return L < whole ? L : whole;
 }
 
@@ -723,16 +721,14 @@ template <class T> int backward(psh_ctx* c, const psh_linear_desc* d) {
         a.part_w = (W*)(space + s.dp); a.part_b = (W*)(space + s.dp + s.part_w);
         a.n = d->out_dim; a.k = d->in_dim;
         int rc;
-        if constexpr (sizeof(T) == 8) {
-            rc = launch_weights<T, 64, 2, 2, false>(c, a, d->rows, st);
-        } else if (grad_tile(d) == 64) {
-            rc = launch_weights<T, 64, 2, 2, false>(c, a, d->rows, st);
-        } else if constexpr (sizeof(T) == 2) {
-            if (!grad_direct(d)) rc = launch_weights<T, 128, 2, 2, false>(c, a, d->rows, st);
-            else if (grad_tile(d) == 128) rc = launch_weights<T, 128, 2, 2, true>(c, a, d->rows, st);
+        if constexpr (sizeof(T) == 2) {
+            const int t = grad_tile(d);
+            if (t == 64) rc = launch_weights<T, 64, 2, 2, false>(c, a, d->rows, st);
+            else if (!grad_direct(d)) rc = launch_weights<T, 128, 2, 2, false>(c, a, d->rows, st);
+            else if (t == 128) rc = launch_weights<T, 128, 2, 2, true>(c, a, d->rows, st);
             else rc = launch_weights<T, 256, 2, 4, true>(c, a, d->rows, st);
         } else {
-            rc = launch_weights<T, 128, 2, 2, false>(c, a, d->rows, st);
+            rc = launch_weights<T, 64, 2, 2, false>(c, a, d->rows, st);
         }
         if (rc != PSH_OK) return rc;
         if (s.part_w + s.part_b > 0) {
