@@ -510,7 +510,9 @@ typedef struct psh_linear_desc {
     const void* x;           /* [dev] [R, in_dim], row stride ld_x */
     const void* weight;      /* [dev] */
     const void* bias;        /* [dev] [G, out_dim], group stride stride_b, or NULL */
-    void* y;                 /* [dev] [R, out_dim] contiguous; the _grad call reads it (may be NULL there with PSH_NL_NONE) */
+    void* y;                 /* [dev] [R, out_dim] contiguous; the _grad call reads it (may be NULL there with PSH_NL_NONE or y_wide) */
+    float* y_wide;           /* [dev] [R, out_dim] contiguous, PSH_BF16 only, or NULL: y before its rounding, written besides y; the _grad
+                              * call takes the slope of the nonlinearity from it instead of from y, which is more exact */
     int64_t ld_x, ld_w, stride_w, stride_b;
     /* psh_grouped_linear_grad: the loss gradient of y in, those of the inputs out (contiguous; NULL = not wanted) */
     const void* dy;          /* [dev] [R, out_dim], row stride ld_dy */

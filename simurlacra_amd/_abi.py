@@ -134,7 +134,8 @@ class PshLinearDesc(C.Structure):
     _fields_ = [
         ('dtype', C.c_int32), ('nonlin', C.c_int32), ('n_groups', C.c_int32), ('rows', C.c_int32),
         ('in_dim', C.c_int32), ('out_dim', C.c_int32), ('offsets', C.c_void_p), ('x', C.c_void_p),
-        ('weight', C.c_void_p), ('bias', C.c_void_p), ('y', C.c_void_p), ('ld_x', C.c_int64), ('ld_w', C.c_int64),
+        ('weight', C.c_void_p), ('bias', C.c_void_p), ('y', C.c_void_p), ('y_wide', C.c_void_p),
+        ('ld_x', C.c_int64), ('ld_w', C.c_int64),
         ('stride_w', C.c_int64), ('stride_b', C.c_int64), ('dy', C.c_void_p), ('ld_dy', C.c_int64),
         ('dx', C.c_void_p), ('dweight', C.c_void_p), ('dbias', C.c_void_p), ('workspace', C.c_void_p),
         ('workspace_bytes', C.c_int64), ('stream', C.c_void_p),

@@ -20,6 +20,8 @@
 
 namespace {
 
+PSH_OP int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+
 // Part k of the product of two fragments.  The parts of one fragment pair all add to the same accumulator, so the parts are the outer
 // loop: an instruction that waits for the one before it would leave the matrix pipe idle.
 template <class T> struct Mfma;
@@ -155,6 +157,13 @@ template <class T, int N, int THREADS, bool TR> struct Stager {
     }
 };
 
+// This lane's number, counted anew: what is computed from it is not kept in registers for a whole loop, where 128 accumulators and 96
+// registers of fragments leave room for little else.
+PSH_OP int lane_now() {
+    int lane;
+    asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=&v"(lane));
+    return lane;
+}
 // A bf16 operand's tiles by loads that go to LDS directly: no registers, no transposing on the way in.  The tile lies as it is in memory, [index][64 c]
 // or, for a transposed operand, [64 c][index], where ds_read_b64_tr_b16 does the transposing: 16 lanes, four to a row of 16 indices, read 4
 // rows, and lane i gets column i.  The loads go to LDS in lane order, so the permutation that spreads the banks is applied
@@ -162,189 +171,289 @@ template <class T, int N, int THREADS, bool TR> struct Stager {
 // rows that half a wave reads at a time are in different banks.
 // Rows past the operand's end are read as its last one (their results are not stored); only whole tiles of c come this way.
 template <int N, int THREADS, bool TR> struct Direct {
-    static constexpr int WAVES = THREADS / 64, PER = N * 128 / 1024 / WAVES;   // 1-KiB loads of a wave
-    static constexpr int ROW = N * 2;                                          // transposed: bytes of a row
-    static PSH_OP int swz(int c) { return (c & 3) | ((c >> 1) & 4); }
-    static PSH_OP void fetch(const Operand<bf16_t>& o, int c0, unsigned lds) {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-        for (int k = 0; k < PER; ++k) {
-            const int chunk = __builtin_amdgcn_readfirstlane(wave + k * WAVES);
+    static constexpr int KC = 32, BYTES = N * 2 * KC, WAVES = THREADS / 64, PER = BYTES / 1024 / WAVES;   // 1-KiB loads of a wave
+    static constexpr int ROW = N * 2, STEP = WAVES * 1024 / ROW;                                          // transposed: bytes of a row, rows between a thread's loads
+    static PSH_OP int swz_i(int i) { return (i >> 2) & 3; }
+    static PSH_OP int swz_c(int c) { return ((c & 3) | ((c >> 1) & 4)) << 1; }
+    // this wave's loads of the tile from c0 to the LDS address `lds`, one by one
+    struct Loads {
+        const bf16_t* line;
+        long ld;
+        unsigned lds;
+        int i0, last, unit;
+        PSH_OP Loads(const Operand<bf16_t>& o, int c0, unsigned to, int wave) : ld(o.ld), lds(to + wave * 1024) {
+            const int lane = lane_now(), at = wave * 1024 + lane * 16, c = at / ROW;
+            i0 = at >> 6;
+            last = o.n - 1;
+            unit = TR ? (at % ROW / 16) ^ swz_c(c) : (lane & 3) ^ swz_i(i0);
+            line = TR ? o.p + (long)(c0 + c) * ld : o.p + c0;
+        }
+        PSH_OP void issue(int k) const {
+            static_assert(STEP % 8 == 0, "the permutations of a thread's loads differ by constants");
             const bf16_t* g;
             if constexpr (!TR) {
-                const int i = chunk * 8 + (lane >> 3), u = unit_of(i, lane & 7);
-                g = o.p + (long)min(i, o.n - 1) * o.ld + c0 + u * 8;
+                g = line + (long)min(i0 + k * 16 * WAVES, last) * ld + unit * 8;
             } else {
-                const int at = chunk * 1024 + lane * 16, c = at / ROW, u = (at % ROW / 16) ^ (swz(c) << 1);
-                g = o.p + (long)(c0 + c) * o.ld + min(u * 8, o.n - 8);
+                g = line + (long)(k * STEP) * ld + min((unit ^ swz_c(k * STEP)) * 8, last - 7);
             }
             // (by hand, because the compiler would wait for a builtin's load before the next read of any part of LDS; the
-            // wait is in front of the barrier that ends the tile)
-            asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds + chunk * 1024), "v"(g) : "memory");
+            // waits are in front of the barriers)
+            asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds + k * WAVES * 1024), "v"(g) : "memory");
         }
-    }
+    };
     // the last, partial tile of c through registers, zero where there is none
-    static PSH_OP void fetch_tail(const Operand<bf16_t>& o, int c0, unsigned char* lds) {
-        if constexpr (!TR) {
-            Stager<bf16_t, N, THREADS, false> st(o);
-            st.fetch(o, c0);
-            st.store(lds);
-        } else {
-            for (int at = threadIdx.x * 16; at < N * 128; at += THREADS * 16) {
-                const int c = at / ROW, u = (at % ROW / 16) ^ (swz(c) << 1);
-                *reinterpret_cast<v4u*>(lds + at) =
-                    c0 + c < o.nc ? load16(o.p + (long)(c0 + c) * o.ld + min(u * 8, o.n - 8)) : v4u{0, 0, 0, 0};
+    static PSH_OP void fetch_tail(const Operand<bf16_t>& o, int c0, unsigned char* lds, int wave) {
+#pragma unroll 1
+        for (int at = (wave * 64 + lane_now()) * 16; at < BYTES; at += THREADS * 16) {
+            v4u v = {0, 0, 0, 0};
+            if constexpr (!TR) {
+                const int i = at >> 6;
+                v = Stager<bf16_t, N, THREADS, false>::piece(o.p + (long)min(i, o.n - 1) * o.ld, c0 + ((at >> 4 & 3) ^ swz_i(i)) * 8, o.nc);
+            } else {
+                const int c = at / ROW, u = (at % ROW / 16) ^ swz_c(c);
+                if (c0 + c < o.nc) v = load16(o.p + (long)(c0 + c) * o.ld + min(u * 8, o.n - 8));
             }
+            *reinterpret_cast<v4u*>(lds + at) = v;
         }
     }
-    // 16 bytes along c for the index i0 + (lane & 15): c from s * 32 + (lane / 16) * 8
-    static PSH_OP v4u fragment(unsigned char* lds, int i0, int s) {
-        const int l = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
-        if constexpr (!TR) {
-            const int i = i0 + l;
-            return *reinterpret_cast<const v4u*>(lds + i * 128 + unit_of(i, s * 4 + g) * 16);
-        } else {
+    // Fragments of blocks of 16 indices from i0 (a multiple of 16 times their number): 16 bytes along c for the index i0 + 16 m + (lane & 15),
+    // c from s * 32 + (lane / 16) * 8
+    struct Reads {
+        unsigned char* lds;
+        int at;
+        PSH_OP Reads(unsigned char* tile, int i0) : lds(tile) {
+            const int lane = lane_now(), l = lane & 15, g = lane >> 4, c = g * 8 + (l >> 2);
+            at = TR ? c * ROW + ((i0 >> 4) * 32 ^ swz_c(c) * 16) + (l & 3) * 8 : (i0 + l) * 64 + (g ^ swz_i(l)) * 16;
+        }
+        PSH_OP v4u block(int m) const {
+            if constexpr (!TR) return *reinterpret_cast<const v4u*>(lds + at + m * 1024);
             typedef short v4s __attribute__((ext_vector_type(4)));
             typedef __attribute__((address_space(3))) v4s* at_t;
-            uint2 h[2];
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const int c = s * 32 + g * 8 + k * 4 + (l >> 2);
-                unsigned char* const at = lds + c * ROW + (((i0 >> 4) ^ swz(c)) * 32) + (l & 3) * 8;
-                h[k] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((at_t)at));
-            }
-            return v4u{h[0].x, h[0].y, h[1].x, h[1].y};
+            unsigned char* const q = lds + (at ^ (m * 32));
+            const uint2 h0 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((at_t)q));
+            const uint2 h1 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((at_t)(q + 4 * ROW)));
+            return v4u{h0.x, h0.y, h1.x, h1.y};
         }
-    }
+    };
 };
 
 template <class T, int BI, int BJ, int WI, int WJ> struct Tile {
     static constexpr int THREADS = 64 * WI * WJ, MI = BI / WI / 16, MJ = BJ / WJ / 16;
     typedef typename Mfma<T>::acc acc_t;
     acc_t acc[MI][MJ];
-    acc_t ones[MI];   // sums of P over c, in every column (the bias gradient), if asked for
+    // sums of P over c, in every column (the bias gradient), if asked for: a block of 16 indices i is summed by one of the WJ waves that have it
+    static constexpr int OWN = MI / WJ > 0 ? MI / WJ : 1;
+    acc_t ones[OWN];
+    int wave_j;
 
     template <int K, bool SUMS> PSH_OP void part(const v4u (&fp)[MI], const v4u (&fq)[MJ], const v4u& unit) {
 #pragma unroll
         for (int a = 0; a < MI; ++a) {
 #pragma unroll
             for (int b = 0; b < MJ; ++b) Mfma<T>::template step<K>(fp[a], fq[b], acc[a][b]);
-            if constexpr (SUMS) Mfma<T>::template step<K>(fp[a], unit, ones[a]);
         }
+        if constexpr (SUMS) sums<K>(fp, unit);
+    }
+    template <int K> PSH_OP void sums(const v4u (&fp)[MI], const v4u& unit) {
+#pragma unroll
+        for (int w = 0; w < WJ; ++w)
+            if (w == wave_j)
+#pragma unroll
+                for (int k = 0; k < OWN; ++k) Mfma<T>::template step<K>(fp[w * OWN + k], unit, ones[k]);
     }
 
-    // D += P Q^T over all c.  LDS: two buffers of (BI + BJ) * 128 bytes.
-    template <bool TP, bool TQ, bool SUMS> PSH_OP void multiply(const Operand<T>& p, const Operand<T>& q, unsigned char* lds) {
-        constexpr int KC = 128 / (int)sizeof(T);
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-        const int wi = (wave % WI) * (BI / WI), wj = (wave / WI) * (BJ / WJ);
-        const int l = lane & 15, g = lane >> 4;
+    template <bool SUMS> PSH_OP void clear(v4u& unit) {
 #pragma unroll
-        for (int a = 0; a < MI; ++a) {
-            ones[a] = acc_t{0, 0, 0, 0};
+        for (int a = 0; a < MI; ++a)
 #pragma unroll
             for (int b = 0; b < MJ; ++b) acc[a][b] = acc_t{0, 0, 0, 0};
-        }
-        v4u unit = {0, 0, 0, 0};
         if constexpr (SUMS) {
+            static_assert(OWN * WJ == MI, "the waves share the blocks evenly");
+            wave_j = wave_id() / WI;
+#pragma unroll
+            for (int k = 0; k < OWN; ++k) ones[k] = acc_t{0, 0, 0, 0};
             T e[16 / sizeof(T)];
 #pragma unroll
             for (int k = 0; k < (int)(16 / sizeof(T)); ++k) e[k] = to_elem<T>(1);
             unit = __builtin_bit_cast(v4u, e);
         }
+    }
+    template <bool SUMS> PSH_OP void parts(const v4u (&fp)[MI], const v4u (&fq)[MJ], const v4u& unit) {
+        part<0, SUMS>(fp, fq, unit);
+        if constexpr (Mfma<T>::PARTS > 1) part<1, SUMS>(fp, fq, unit);
+        if constexpr (Mfma<T>::PARTS > 2) {
+            part<2, SUMS>(fp, fq, unit);
+            part<3, SUMS>(fp, fq, unit);
+        }
+    }
+
+    // D += P Q^T over all c, in steps of 128 bytes of c.  LDS: two buffers of (BI + BJ) * 128 bytes.
+    // A step's fragments are read in two halves, each while the half before it is being multiplied: the second half in front of the
+    // step's barrier, the next step's first one behind it.  The barrier says that the next step's tile is in LDS and that nobody
+    // reads this step's any more.
+    template <bool TP, bool TQ, bool SUMS> PSH_OP void multiply(const Operand<T>& p, const Operand<T>& q, unsigned char* lds) {
+        constexpr int KC = 128 / (int)sizeof(T);
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        const int wi = (wave % WI) * (BI / WI), wj = (wave / WI) * (BJ / WJ);
+        const int l = lane & 15, g = lane >> 4;
+        v4u unit = {0, 0, 0, 0};
+        clear<SUMS>(unit);
         const int nc = p.nc, tiles = (nc + KC - 1) / KC;
         if (tiles <= 0) return;
         Stager<T, BI, THREADS, TP> sp(p);
         Stager<T, BJ, THREADS, TQ> sq(q);
-        sp.fetch(p, 0);
-        sq.fetch(q, 0);
-        sp.store(lds);
-        sq.store(lds + BI * 128);
+        v4u fp[2][MI], fq[2][MJ];
+        const auto read = [&](int s, const unsigned char* at) {
+#pragma unroll
+            for (int a = 0; a < MI; ++a) {
+                const int i = wi + a * 16 + l;
+                fp[s][a] = *reinterpret_cast<const v4u*>(at + i * 128 + unit_of(i, s * 4 + g) * 16);
+            }
+#pragma unroll
+            for (int b = 0; b < MJ; ++b) {
+                const int j = wj + b * 16 + l;
+                fq[s][b] = *reinterpret_cast<const v4u*>(at + BI * 128 + j * 128 + unit_of(j, s * 4 + g) * 16);
+            }
+        };
+        const auto fetch = [&](int t) {
+            sp.fetch(p, t * KC);
+            sq.fetch(q, t * KC);
+        };
+        const auto store = [&](unsigned char* at) {
+            sp.store(at);
+            sq.store(at + BI * 128);
+        };
+        fetch(0);
+        store(lds);
+        if (tiles > 1) fetch(1);
         __syncthreads();
+        read(0, lds);
         for (int t = 0; t < tiles; ++t) {
             unsigned char* const cur = lds + (t & 1) * (BI + BJ) * 128;
             unsigned char* const nxt = lds + (~t & 1) * (BI + BJ) * 128;
-            if (t + 1 < tiles) {
-                sp.fetch(p, (t + 1) * KC);
-                sq.fetch(q, (t + 1) * KC);
-            }
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                if (s == 1 && nc - t * KC <= KC / 2) break;   // nothing but zeros in the second half
-                v4u fp[MI], fq[MJ];
-#pragma unroll
-                for (int a = 0; a < MI; ++a) {
-                    const int i = wi + a * 16 + l;
-                    fp[a] = *reinterpret_cast<const v4u*>(cur + i * 128 + unit_of(i, s * 4 + g) * 16);
-                }
-#pragma unroll
-                for (int b = 0; b < MJ; ++b) {
-                    const int j = wj + b * 16 + l;
-                    fq[b] = *reinterpret_cast<const v4u*>(cur + BI * 128 + j * 128 + unit_of(j, s * 4 + g) * 16);
-                }
-                part<0, SUMS>(fp, fq, unit);
-                if constexpr (Mfma<T>::PARTS > 1) part<1, SUMS>(fp, fq, unit);
-                if constexpr (Mfma<T>::PARTS > 2) {
-                    part<2, SUMS>(fp, fq, unit);
-                    part<3, SUMS>(fp, fq, unit);
-                }
-            }
-            if (t + 1 < tiles) {
-                sp.store(nxt);
-                sq.store(nxt + BI * 128);
-            }
+            const bool second = nc - t * KC > KC / 2;   // (else nothing but zeros there)
+            if (second) read(1, cur);
+            __builtin_amdgcn_sched_barrier(0);
+            parts<SUMS>(fp[0], fq[0], unit);
+            __builtin_amdgcn_sched_barrier(0);
+            if (t + 1 < tiles) store(nxt);
+            if (t + 2 < tiles) fetch(t + 2);
             __syncthreads();
+            if (t + 1 < tiles) read(0, nxt);
+            __builtin_amdgcn_sched_barrier(0);
+            if (second) parts<SUMS>(fp[1], fq[1], unit);
         }
     }
 
-    // the same for bf16 by direct loads
+    // The same for bf16 by direct loads, in steps of 64 bytes of c.  LDS: three buffers of (BI + BJ) * 64 bytes, so that the loads of two
+    // steps are in flight while one is being multiplied.  A step's fragments are read while the step before it is being multiplied; its
+    // barrier says that they are in everyone's registers, so that their buffer can be filled again, and that the next step's tile is in LDS.
+    // Reads of LDS and loads are issued between the matrix instructions, a few behind each block of rows: in one go they would hold the wave up
+    // until the queues have taken them, with its matrix instructions behind them.
     template <bool TP, bool TQ, bool SUMS> PSH_OP void multiply_direct(const Operand<bf16_t>& p, const Operand<bf16_t>& q, unsigned char* lds) {
         typedef Direct<BI, THREADS, TP> DP;
         typedef Direct<BJ, THREADS, TQ> DQ;
-        const int wave = threadIdx.x >> 6;
+        constexpr int KC = DP::KC, LOADS = DP::PER + DQ::PER;
+        constexpr unsigned BUF = DP::BYTES + DQ::BYTES;
+        const int wave = wave_id();
         const int wi = (wave % WI) * (BI / WI), wj = (wave / WI) * (BJ / WJ);
-#pragma unroll
-        for (int a = 0; a < MI; ++a) {
-            ones[a] = acc_t{0, 0, 0, 0};
-#pragma unroll
-            for (int b = 0; b < MJ; ++b) acc[a][b] = acc_t{0, 0, 0, 0};
-        }
-        v4u unit = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};   // eight ones
-        const int nc = p.nc, tiles = (nc + 63) / 64, whole = nc / 64;
+        v4u unit = {0, 0, 0, 0};
+        clear<SUMS>(unit);
+        const int nc = p.nc, tiles = (nc + KC - 1) / KC, whole = nc / KC;
         if (tiles <= 0) return;
         const unsigned base = (unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)lds;
-        constexpr unsigned BUF = (BI + BJ) * 128;
+        v4u fp[2][MI], fq[2][MJ];
+        // Rows of c are often powers of two apart, and then one step's reads of all rows lie in one or two of the 16 channels of an L2, 256
+        // bytes each.  So every workgroup of an XCD begins elsewhere, two steps from the one before it.
+        const int turn = whole > 0 ? (int)((blockIdx.x >> 3) * 2 % whole) : 0;
+        const auto at = [&](int t) { return (t + turn < whole ? t + turn : t + turn - whole) * KC; };
         const auto bring = [&](int t, unsigned buf) {
             if (t < whole) {
-                DP::fetch(p, t * 64, base + buf);
-                DQ::fetch(q, t * 64, base + buf + BI * 128);
-            } else {
-                DP::fetch_tail(p, t * 64, lds + buf);
-                DQ::fetch_tail(q, t * 64, lds + buf + BI * 128);
+                const typename DP::Loads lp(p, at(t), base + buf, wave);
+                const typename DQ::Loads lq(q, at(t), base + buf + DP::BYTES, wave);
+#pragma unroll
+                for (int k = 0; k < DP::PER; ++k) lp.issue(k);
+#pragma unroll
+                for (int k = 0; k < DQ::PER; ++k) lq.issue(k);
+            } else if (t < tiles) {
+                DP::fetch_tail(p, t * KC, lds + buf, wave);
+                DQ::fetch_tail(q, t * KC, lds + buf + DP::BYTES, wave);
             }
         };
-        bring(0, 0);
-        asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
-        __syncthreads();
-        for (int t = 0; t < tiles; ++t) {
-            const unsigned cur = (t & 1) * BUF, nxt = BUF - cur;
-            if (t + 1 < tiles) bring(t + 1, nxt);
+        // multiplies a step's fragments, set H, reads the next one's from `from` into the other set, and with LOAD issues the loads of step t
+        const auto step = [&](auto h, auto load, unsigned from, int t, unsigned to) {
+            constexpr int H = decltype(h)::value, READS = MI + MJ, AT_A_TIME = (READS * 4 + 3 * MI - 1) / (3 * MI);
+            const typename DP::Reads rp(lds + from, wi);
+            const typename DQ::Reads rq(lds + from + DP::BYTES, wj);
+            const typename DP::Loads lp(p, at(t), base + to, wave);
+            const typename DQ::Loads lq(q, at(t), base + to + DP::BYTES, wave);
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                v4u fp[MI], fq[MJ];
+            for (int a = 0; a < MI; ++a) {
 #pragma unroll
-                for (int a = 0; a < MI; ++a) fp[a] = DP::fragment(lds + cur, wi + a * 16, s);
-#pragma unroll
-                for (int b = 0; b < MJ; ++b) fq[b] = DQ::fragment(lds + cur + BI * 128, wj + b * 16, s);
-                part<0, SUMS>(fp, fq, unit);
-                if constexpr (Mfma<T>::PARTS > 1) part<1, SUMS>(fp, fq, unit);
-                if constexpr (Mfma<T>::PARTS > 2) {
-                    part<2, SUMS>(fp, fq, unit);
-                    part<3, SUMS>(fp, fq, unit);
+                for (int r = a * AT_A_TIME; r < (a + 1) * AT_A_TIME && r < READS; ++r) {
+                    if (r < MJ) fq[1 - H][r] = rq.block(r);
+                    else fp[1 - H][r - MJ] = rp.block(r - MJ);
                 }
+                if constexpr (decltype(load)::value) {
+#pragma unroll
+                    for (int k = a * LOADS / MI; k < (a + 1) * LOADS / MI; ++k) {
+                        if (k < DP::PER) lp.issue(k);
+                        else lq.issue(k - DP::PER);
+                    }
+                }
+#pragma unroll
+                for (int b = 0; b < MJ; ++b) Mfma<T>::template step<0>(fp[H][a], fq[H][b], acc[a][b]);
+                __builtin_amdgcn_sched_barrier(0);
             }
-            asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+            if constexpr (SUMS) sums<0>(fp[H], unit);
+        };
+        constexpr std::integral_constant<int, 0> even{};
+        constexpr std::integral_constant<int, 1> odd{};
+        // all loads have landed but those of the `later` newest steps
+        const auto wait = [&](auto later) {
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"(LOADS * decltype(later)::value) : "memory");
             __syncthreads();
+        };
+        bring(0, 0);
+        bring(1, BUF);
+        bring(2, 2 * BUF);
+        if (2 < whole) wait(std::integral_constant<int, 2>());
+        else wait(std::integral_constant<int, 0>());
+        {
+            const typename DP::Reads rp(lds, wi);
+            const typename DQ::Reads rq(lds + DP::BYTES, wj);
+#pragma unroll
+            for (int b = 0; b < MJ; ++b) fq[0][b] = rq.block(b);
+#pragma unroll
+            for (int a = 0; a < MI; ++a) fp[0][a] = rp.block(a);
+        }
+        unsigned cur = 0, nxt = BUF;   // buffers of steps t and t + 1
+        const auto on = [&]() {
+            cur = nxt;
+            nxt = nxt == 2 * BUF ? 0 : nxt + BUF;
+        };
+        int t = 0;
+        for (; t + 4 < whole; t += 2) {
+            wait(odd);
+            step(even, std::true_type(), nxt, t + 3, cur);
+            on();
+            wait(odd);
+            step(odd, std::true_type(), nxt, t + 4, cur);
+            on();
+        }
+        for (; t < tiles; t += 2) {
+            if (t + 2 < whole) wait(odd);
+            else wait(even);
+            bring(t + 3, cur);
+            step(even, std::false_type(), nxt, 0, 0);   // (behind the last step it reads what nobody uses)
+            on();
+            if (t + 1 < tiles) {
+                if (t + 3 < whole) wait(odd);
+                else wait(even);
+                bring(t + 4, cur);
+                step(odd, std::false_type(), nxt, 0, 0);
+                on();
+            }
         }
     }
 
@@ -361,6 +470,8 @@ template <class T, int BI, int BJ, int WI, int WJ> struct Tile {
     }
 };
 
+constexpr int lds_bytes(int bi, int bj, bool direct) { return (bi + bj) * (direct ? 3 * 64 : 2 * 128); }
+
 // consecutive tiles on one XCD: workgroups go to the 8 XCDs in turn, each of which has an L2 of its own
 PSH_OP long xcd_order(long b, long total) {
     const long per = (total + 7) / 8;
@@ -373,6 +484,7 @@ template <class T> struct RowsArgs {   // forward and dx
     const T* weight; long ld_w, stride_w;
     const T* bias; long stride_b;
     T* out;                            // [rows, n_out] contiguous
+    float* wide;                       // the same before its rounding, or NULL (bf16 only)
     int n_in, n_out, nonlin;
     long slots, tiles_i;
 };
@@ -403,16 +515,22 @@ template <class T, int COLS, class S> PSH_OP void store_tile(unsigned char* lds,
 }
 
 template <class T, int BI, int BJ, int WI, int WJ, bool TW, bool DIRECT>
-__global__ __launch_bounds__(64 * WI * WJ, BI * BJ > 4096 ? 2 : sizeof(T) == 2 && TW ? 3 : 4) void k_rows(const RowsArgs<T> a) {
+__global__ __launch_bounds__(64 * WI * WJ, BI * BJ > 4096 || (sizeof(T) == 2 && TW) ? 2 : TW ? 3 : 4) void k_rows(const RowsArgs<T> a) {
     extern __shared__ __align__(16) unsigned char lds[];
     const long id = xcd_order(blockIdx.x, a.slots * a.tiles_i);
     if (id >= a.slots * a.tiles_i) return;
-    const Piece q = find_piece(a.parts, (int)(id / a.tiles_i));
-    const int i0 = (int)(id % a.tiles_i) * BI;
+    // blocks of 8 tiles of units for all rows, one after the other: what the workgroups of an XCD read at a time stays in its L2
+    const long block = id / (a.slots * 8), in_block = id - block * a.slots * 8, wide = a.tiles_i - block * 8 < 8 ? a.tiles_i - block * 8 : 8;
+    const Piece q = find_piece(a.parts, (int)(in_block / wide));
+    const int i0 = (int)(block * 8 + in_block % wide) * BI;
     const int nj = q.end - q.begin, ni = min(BI, a.n_out - i0);
     if (nj <= 0) return;
     if (q.part >= a.parts.n) {   // rows behind the last group
-        for (int k = threadIdx.x; k < nj * ni; k += blockDim.x) a.out[(long)(q.begin + k / ni) * a.n_out + i0 + k % ni] = T(0);
+        for (int k = threadIdx.x; k < nj * ni; k += blockDim.x) {
+            const long at = (long)(q.begin + k / ni) * a.n_out + i0 + k % ni;
+            a.out[at] = T(0);
+            if (a.wide) a.wide[at] = 0;
+        }
         return;
     }
     const T* const w = a.weight + (long)q.part * a.stride_w;
@@ -435,8 +553,24 @@ __global__ __launch_bounds__(64 * WI * WJ, BI * BJ > 4096 ? 2 : sizeof(T) == 2 &
                 bias_of = i;
             }
             T e[4];
+            W y[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) e[r] = to_elem<T>(f((W)(v[r] + bias[r])));
+            for (int r = 0; r < 4; ++r) {
+                y[r] = f((W)(v[r] + bias[r]));
+                e[r] = to_elem<T>(y[r]);
+            }
+            if constexpr (sizeof(T) == 2) {
+                if (a.wide && j < nj) {
+                    float* const o = a.wide + (long)(q.begin + j) * a.n_out + i0 + i;
+                    if (i + 4 <= ni) {
+                        __builtin_memcpy(o, y, 16);
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (i + r < ni) o[r] = y[r];
+                    }
+                }
+            }
             if constexpr (sizeof(T) == 8) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) *tile_at<T, BI>(lds, j, i + 4 * r, swz(j)) = e[r];
@@ -455,11 +589,46 @@ __global__ __launch_bounds__(64 * WI * WJ, BI * BJ > 4096 ? 2 : sizeof(T) == 2 &
 
 // dp = dy f'(y), rounded to the element type as the gradient that reaches a layer's product in any composition of
 // layers is.  Rows behind the last group have no part in any sum.
-template <class T> __global__ __launch_bounds__(256) void k_preact(long n, int cols, const T* dy, long ld, const T* y, int nonlin, T* dp) {
-    for (long k = (long)blockIdx.x * 256 + threadIdx.x; k < n; k += (long)gridDim.x * 256) {
-        const long r = k / cols;
-        dp[k] = to_elem<T>(to_wide(dy[r * ld + (k - r * cols)]) * nonlin_slope_w(nonlin, to_wide(y[k])));
+// A thread takes V neighbouring elements, which lie in one row (V divides its length, or the rows follow one another).
+template <class T, class Y, int V> __global__ __launch_bounds__(256) void k_preact(long n, int cols, const T* dy, long ld, const Y* y, int nonlin, T* dp) {
+    for (long k = ((long)blockIdx.x * 256 + threadIdx.x) * V; k < n; k += (long)gridDim.x * 256 * V) {
+        long at = k;
+        if (ld != cols) {
+            const long r = k / cols;
+            at = r * ld + (k - r * cols);
+        }
+        const int live = (int)min((long)V, n - k);
+        T up[V], e[V];
+        Y value[V];
+        if (live == V) {
+            __builtin_memcpy(up, dy + at, sizeof(up));
+            __builtin_memcpy(value, y + k, sizeof(value));
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                up[i] = i < live ? dy[at + i] : T(0);
+                value[i] = i < live ? y[k + i] : Y(0);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) e[i] = to_elem<T>(to_wide(up[i]) * nonlin_slope_w(nonlin, to_wide(value[i])));
+        if (live == V) {
+            __builtin_memcpy(dp + k, e, sizeof(e));
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (i < live) dp[k + i] = e[i];
+        }
     }
+}
+template <class T, class Y> void launch_preact(const psh_linear_desc* d, const Y* y, T* dp, hipStream_t st) {
+    const long n = (long)d->rows * d->out_dim;
+    constexpr int V = 16 / (int)sizeof(T);
+    const bool wide = d->ld_dy == d->out_dim || d->out_dim % V == 0;
+    const long blocks = (n + 1023) / 1024;
+    const dim3 grid((unsigned)(blocks < 4096 ? blocks : 4096));
+    if (wide) hipLaunchKernelGGL((k_preact<T, Y, V>), grid, dim3(256), 0, st, n, (int)d->out_dim, (const T*)d->dy, (long)d->ld_dy, y, (int)d->nonlin, dp);
+    else hipLaunchKernelGGL((k_preact<T, Y, 1>), grid, dim3(256), 0, st, n, (int)d->out_dim, (const T*)d->dy, (long)d->ld_dy, y, (int)d->nonlin, dp);
 }
 
 template <class T> struct GradArgs {   // dW, db
@@ -474,7 +643,7 @@ template <class T> struct GradArgs {   // dW, db
 };
 
 template <class T, int BI, int BJ, int WI, int WJ, bool DIRECT>
-__global__ __launch_bounds__(64 * WI * WJ, BI * BJ > 4096 || sizeof(T) == 2 ? 2 : sizeof(T) == 4 ? 3 : 4) void k_weights(const GradArgs<T> a) {
+__global__ __launch_bounds__(64 * WI * WJ, BI * BJ > 4096 || sizeof(T) == 2 ? 2 : 3) void k_weights(const GradArgs<T> a) {
     extern __shared__ __align__(16) unsigned char lds[];
     const long tiles = a.tiles_i * a.tiles_j, total = a.slots * tiles;
     const long id = xcd_order(blockIdx.x, total);
@@ -503,9 +672,9 @@ __global__ __launch_bounds__(64 * WI * WJ, BI * BJ > 4096 || sizeof(T) == 2 ? 2 
         const auto put = [&](auto* out) {
             typedef typename std::remove_pointer<decltype(out)>::type O;
             const auto swz = [](int i) { return ((i >> 2) & 3) * (int)sizeof(O); };
-            // as many rows at a time as the two buffers of operands hold
-            constexpr int ROOM = 2 * (BI + BJ) * 128 / (BJ * (int)sizeof(O)), ROWS = ROOM < BI ? ROOM : BI;
-            static_assert(BI % ROWS == 0 && ROWS % 16 == 0, "whole blocks of a matrix instruction's rows");
+            // as many rows at a time as the operands' buffers hold
+            constexpr int ROOM = lds_bytes(BI, BJ, DIRECT) / (BJ * (int)sizeof(O)), ROWS = ROOM >= BI ? BI : ROOM >= BI / 2 ? BI / 2 : BI / 4;
+            static_assert(ROWS <= ROOM && ROWS % 16 == 0, "whole blocks of a matrix instruction's rows");
             for (int first = 0; first < BI; first += ROWS) {
                 if (first > 0) __syncthreads();
                 tile.each([&](int i, int j, auto v) {
@@ -522,10 +691,10 @@ __global__ __launch_bounds__(64 * WI * WJ, BI * BJ > 4096 || sizeof(T) == 2 ? 2 
         if (whole) put(a.dw);
         else put(a.part_w);
     }
-    if (sums && (threadIdx.x & 15) == 0 && (threadIdx.x >> 6) / WI == 0) {
-        const int wi = ((threadIdx.x >> 6) % WI) * (BI / WI);
+    if (sums && (threadIdx.x & 15) == 0) {
+        const int wave = threadIdx.x >> 6, wi = (wave % WI) * (BI / WI) + wave / WI * tile.OWN * 16;
 #pragma unroll
-        for (int m = 0; m < BI / WI / 16; ++m)
+        for (int m = 0; m < tile.OWN; ++m)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int i = wi + m * 16 + Mfma<T>::row((threadIdx.x & 63) >> 4, r);
@@ -570,7 +739,8 @@ template <class T, int BI, int BJ, int WI, int WJ, bool TW, bool DIRECT> int lau
     a.tiles_i = (a.n_out + BI - 1) / BI;
     const long total = (a.slots * a.tiles_i + 7) / 8 * 8;
     if (total > 0x7fffffffL) { set_err(c, "grouped_linear: too many tiles for one launch"); return PSH_ERR_UNSUPPORTED; }
-    constexpr int lds = 2 * (BI + BJ) * 128;
+    constexpr int lds = lds_bytes(BI, BJ, DIRECT);
+    static_assert(lds >= BI * BJ * (int)sizeof(T), "a result tile goes through it");
     const auto kernel = k_rows<T, BI, BJ, WI, WJ, TW, DIRECT>;
     const int rc = allow_lds(c, kernel, lds);
     if (rc != PSH_OK) return rc;
@@ -580,17 +750,21 @@ template <class T, int BI, int BJ, int WI, int WJ, bool TW, bool DIRECT> int lau
 }
 
 // Tiles [units][rows].  Large ones re-read the operands less often, small ones waste less where a group has few rows or a layer few
-// units, and there are more of them to fill the CUs.
+// units, and there are more of them to fill the CUs: the larger ones are for layers that have one and a half of them for every CU.
+// bf16, 8 groups of about 4096 rows, 1024 -> 2048: 180 us (760 TFLOP/s) in 256 x 128 with two workgroups on a CU, of which one stores its tile
+// while the other multiplies; 197 us in 256 x 256 with one on a CU; 228 us in 128 x 128.  Without its loads from memory the first takes
+// 143 us, without those from LDS too 105 us.  12 groups of 2500 rows, 513 -> 257, fp32, 64 x 64: 122 us (65 TFLOP/s, the matrix pipes busy for
+// 65 % of the time, a fifth of it with columns behind the 257th).
 template <class T, bool TW> int run_rows(psh_ctx* c, RowsArgs<T>& a, int rows, hipStream_t st) {
     const long mean = rows / a.parts.n;
     if (mean <= 24) return launch_rows<T, 64, 16, 4, 1, TW, false>(c, a, rows, st);
     if constexpr (sizeof(T) == 2) {
-        const long large = ((long)rows / 128 + a.parts.n / 2) * ((a.n_out + 127) / 128), huge = ((long)rows / 256 + a.parts.n / 2) * ((a.n_out + 255) / 256);
+        const long large = ((long)rows / 128 + a.parts.n / 2) * ((a.n_out + 127) / 128), huge = ((long)rows / 128 + a.parts.n / 2) * ((a.n_out + 255) / 256);
         if (mean >= 96 && a.n_out > 64 && large >= 192) {
             const bool direct = aligned16(a.rows_in, 2, a.ld_in) && aligned16(a.weight, 2, a.ld_w, a.stride_w) && (!TW || a.n_out % 8 == 0);
-            if (direct && mean >= 512 && a.n_out > 128 && huge >= 384) return launch_rows<T, 256, 256, 2, 4, TW, true>(c, a, rows, st);
+            if (direct && mean >= 512 && a.n_out > 128 && huge >= 768) return launch_rows<T, 256, 128, 2, 2, TW, true>(c, a, rows, st);
             if (direct) return launch_rows<T, 128, 128, 2, 2, TW, true>(c, a, rows, st);
-            return launch_rows<T, 128, 128, 2, 2, TW, false>(c, a, rows, st);
+            return launch_rows<T, 128, 128, 2, 4, TW, false>(c, a, rows, st);
         }
     }
     return launch_rows<T, 64, 64, 2, 2, TW, false>(c, a, rows, st);
@@ -640,6 +814,7 @@ int check(psh_ctx* c, const psh_linear_desc* d, bool grad) {
     }
     if (d->n_groups < 1 || d->rows < 0 || d->in_dim < 1 || d->out_dim < 1) { set_err(c, "grouped_linear: invalid sizes"); return PSH_ERR_ARG; }
     if (d->n_groups > (1 << 30) || d->rows > (1 << 30)) { set_err(c, "grouped_linear: at most 2^30 rows and groups"); return PSH_ERR_UNSUPPORTED; }
+    if (d->y_wide && d->dtype != PSH_BF16) { set_err(c, "grouped_linear: y_wide is for PSH_BF16"); return PSH_ERR_ARG; }
     if (!d->offsets || (d->rows > 0 && !d->x) || !d->weight || d->ld_x < d->in_dim || d->ld_w < d->in_dim || d->stride_w < 0 || d->stride_b < 0) {
         set_err(c, "grouped_linear: NULL array or a row stride below the row's length");
         return PSH_ERR_ARG;
@@ -648,7 +823,7 @@ int check(psh_ctx* c, const psh_linear_desc* d, bool grad) {
         if (d->rows > 0 && !d->y) { set_err(c, "grouped_linear: y is NULL"); return PSH_ERR_ARG; }
         return PSH_OK;
     }
-    if (d->rows > 0 && (!d->dy || d->ld_dy < d->out_dim || (d->nonlin != PSH_NL_NONE && !d->y))) {
+    if (d->rows > 0 && (!d->dy || d->ld_dy < d->out_dim || (d->nonlin != PSH_NL_NONE && !d->y && !d->y_wide))) {
         set_err(c, "grouped_linear_grad: dy (and y, with a nonlinearity) must be given");
         return PSH_ERR_ARG;
     }
@@ -660,14 +835,14 @@ int check(psh_ctx* c, const psh_linear_desc* d, bool grad) {
     return PSH_OK;
 }
 
-template <class T, int B, int WI, int WJ, bool DIRECT> int launch_weights(psh_ctx* c, GradArgs<T>& a, int rows, hipStream_t st) {
+template <class T, int BI, int BJ, int WI, int WJ, bool DIRECT> int launch_weights(psh_ctx* c, GradArgs<T>& a, int rows, hipStream_t st) {
     a.slots = parts_slots(rows, a.parts.n, a.parts.L);
-    a.tiles_i = (a.n + B - 1) / B;
-    a.tiles_j = a.dw ? (a.k + B - 1) / B : 1;
+    a.tiles_i = (a.n + BI - 1) / BI;
+    a.tiles_j = a.dw ? (a.k + BJ - 1) / BJ : 1;
     const long total = (a.slots * a.tiles_i * a.tiles_j + 7) / 8 * 8;
     if (total > 0x7fffffffL) { set_err(c, "grouped_linear_grad: too many tiles for one launch"); return PSH_ERR_UNSUPPORTED; }
-    constexpr int lds = 4 * B * 128;
-    const auto kernel = k_weights<T, B, B, WI, WJ, DIRECT>;
+    constexpr int lds = lds_bytes(BI, BJ, DIRECT);
+    const auto kernel = k_weights<T, BI, BJ, WI, WJ, DIRECT>;
     const int rc = allow_lds(c, kernel, lds);
     if (rc != PSH_OK) return rc;
     hipLaunchKernelGGL(kernel, dim3((unsigned)total), dim3(64 * WI * WJ), lds, st, a);
@@ -682,6 +857,7 @@ template <class T> int forward(psh_ctx* c, const psh_linear_desc* d) {
     a.weight = (const T*)d->weight; a.ld_w = d->ld_w; a.stride_w = d->stride_w;
     a.bias = (const T*)d->bias; a.stride_b = d->stride_b;
     a.out = (T*)d->y;
+    a.wide = d->y_wide;
     a.n_in = d->in_dim; a.n_out = d->out_dim; a.nonlin = d->nonlin;
     return run_rows<T, false>(c, a, d->rows, (hipStream_t)d->stream);
 }
@@ -694,10 +870,8 @@ template <class T> int backward(psh_ctx* c, const psh_linear_desc* d) {
     const T* dp = (const T*)d->dy;
     long ld_dp = d->ld_dy;
     if (d->nonlin != PSH_NL_NONE && d->rows > 0) {
-        const long n = (long)d->rows * d->out_dim;
-        const long blocks = (n + 1023) / 1024;
-        hipLaunchKernelGGL(k_preact<T>, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, n, (int)d->out_dim, dp, ld_dp,
-                           (const T*)d->y, (int)d->nonlin, (T*)space);
+        if (sizeof(T) == 2 && d->y_wide) launch_preact(d, (const float*)d->y_wide, (T*)space, st);
+        else launch_preact(d, (const T*)d->y, (T*)space, st);
         PSH_HIP(c, hipGetLastError());
         dp = (const T*)space;
         ld_dp = d->out_dim;
@@ -709,7 +883,7 @@ template <class T> int backward(psh_ctx* c, const psh_linear_desc* d) {
         a.weight = (const T*)d->weight; a.ld_w = d->ld_w; a.stride_w = d->stride_w;
         a.out = (T*)d->dx;
         a.n_in = d->out_dim; a.n_out = d->in_dim; a.nonlin = PSH_NL_NONE;
-            const int rc = run_rows<T, true>(c, a, d->rows, st);
+        const int rc = run_rows<T, true>(c, a, d->rows, st);
         if (rc != PSH_OK) return rc;
     }
     if (d->dweight || d->dbias) {
@@ -723,12 +897,12 @@ template <class T> int backward(psh_ctx* c, const psh_linear_desc* d) {
         int rc;
         if constexpr (sizeof(T) == 2) {
             const int t = grad_tile(d);
-            if (t == 64) rc = launch_weights<T, 64, 2, 2, false>(c, a, d->rows, st);
-            else if (!grad_direct(d)) rc = launch_weights<T, 128, 2, 2, false>(c, a, d->rows, st);
-            else if (t == 128) rc = launch_weights<T, 128, 2, 2, true>(c, a, d->rows, st);
-            else rc = launch_weights<T, 256, 2, 4, true>(c, a, d->rows, st);
+            if (t == 64) rc = launch_weights<T, 64, 64, 2, 2, false>(c, a, d->rows, st);
+            else if (!grad_direct(d)) rc = launch_weights<T, 128, 128, 2, 4, false>(c, a, d->rows, st);
+            else if (t == 128) rc = launch_weights<T, 128, 128, 2, 2, true>(c, a, d->rows, st);
+            else rc = launch_weights<T, 128, 256, 2, 2, true>(c, a, d->rows, st);
         } else {
-            rc = launch_weights<T, 64, 2, 2, false>(c, a, d->rows, st);
+            rc = launch_weights<T, 64, 64, 2, 2, false>(c, a, d->rows, st);
         }
         if (rc != PSH_OK) return rc;
         if (s.part_w + s.part_b > 0) {

@@ -1163,7 +1163,7 @@ ScanPlan scan_plan(const psh_scan_desc* d, bool grad) {
     const int widest = padded < 16 ? padded : 16;
     p.piece = whole;
     int lpc = least;
-    if (with(least) < 512) {
+    if (with(least) < 512 && d->n_seqs > 0) {
         if (d->rows > 192 * (int64_t)d->n_seqs) {
             p.piece = (int64_t)d->rows * p.blocks / 1024 / ts * ts;
             if (p.piece < 32) p.piece = 32;

@@ -172,30 +172,41 @@ def _linear_desc(x, weight, bias, offsets, nonlin):
             bias = bias.contiguous()
             stride_b = N
         b = bias.data_ptr()
-    d = abi.PshLinearDesc(_DTYPES[dt], _NONLINS[nonlin], G, R, K, N, offsets.data_ptr(), x.data_ptr(), weight.data_ptr(), b, None, ld_x,
+    d = abi.PshLinearDesc(_DTYPES[dt], _NONLINS[nonlin], G, R, K, N, offsets.data_ptr(), x.data_ptr(), weight.data_ptr(), b, None, None, ld_x,
                           ld_w if N > 1 else K, stride_w if G > 1 else 0, stride_b if G > 1 else 0)
     d.stream = eng._stream()
     return eng, d, (x, weight, bias, offsets), R, K, G, N, dt, dev    # the tensors have to outlive the call
 
 
-def _linear_forward(x, weight, bias, offsets, nonlin):
+def _linear_forward(x, weight, bias, offsets, nonlin, wide=False):
+    """ The layer's results, and with `wide` also what the gradient takes the nonlinearity's slope from: the results
+    before their rounding where that makes a difference. """
     eng, d, keep, R, K, G, N, dt, dev = _linear_desc(x, weight, bias, offsets, nonlin)
     y = torch.empty((R, N), dtype=dt, device=dev)
     d.y = y.data_ptr()
+    value = y
+    if wide and dt == torch.bfloat16 and nonlin in ('tanh', 'sigmoid'):
+        value = torch.empty((R, N), dtype=torch.float32, device=dev)
+        d.y_wide = value.data_ptr()
     eng._call('psh_grouped_linear', C.byref(d))
     del keep
-    return y
+    return (y, value) if wide else y
 
 
 def grouped_linear_grad(dy, y, x, weight, offsets, nonlin=None, want=(True, True, True)):
     """ The gradients (dx, dweight, dbias) of grouped_linear for the gradient dy of its result y; None where `want` is false.
-    y is only read with a nonlinearity (its slope is taken from the value, in y's type). """
+    y is only read with a nonlinearity, whose slope is taken from the value: of bfloat16 results, whose rounding is felt where a
+    nonlinearity is flat, the values may be given in float32. """
     eng, d, keep, R, K, G, N, dt, dev = _linear_desc(x, weight, None, offsets, nonlin)
     dy, d.ld_dy = _rows_arg('dy', dy, dt, dev, R, N)
     d.dy = dy.data_ptr()
     if nonlin is not None:
-        y = _param('y', y, dt, dev, (R, N))
-        d.y = y.data_ptr()
+        wide = dt == torch.bfloat16 and isinstance(y, _Tensor) and y.dtype == torch.float32
+        y = _param('y', y, torch.float32 if wide else dt, dev, (R, N))
+        if wide:
+            d.y_wide = y.data_ptr()
+        else:
+            d.y = y.data_ptr()
     dx = dw = db = None
     if want[0]:
         dx = torch.empty((R, K), dtype=dt, device=dev)
@@ -215,8 +226,8 @@ def grouped_linear_grad(dy, y, x, weight, offsets, nonlin=None, want=(True, True
 class _GroupedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, offsets, nonlin):
-        y = _linear_forward(x, weight, bias, offsets, nonlin)
-        ctx.save_for_backward(x, weight, offsets, y if nonlin is not None else None)
+        y, value = _linear_forward(x, weight, bias, offsets, nonlin, wide=True)
+        ctx.save_for_backward(x, weight, offsets, value if nonlin is not None else None)
         ctx.nonlin = nonlin
         return y
 

@@ -275,3 +275,41 @@ def test_refusals(ops):
     for bad in (None, check[:-8], check.float()):
         with pytest.raises(ValueErr):
             ops.selective_scan_grad(y, None, bad, *args)
+
+
+@pytest.mark.parametrize('nonlin', ['tanh', 'sigmoid'])
+def test_slopes_of_bfloat16_layers_where_they_are_flat(ops, nonlin):
+    """ A layer's own bfloat16 result is too coarse for its slope (tanh at 3: a result of 1 - 2^-8 and a slope of 2^-7 in steps of half its
+    size), so the gradient goes by the value before its rounding. """
+    gen = torch.Generator().manual_seed(5)
+    R, T = 4000, torch.bfloat16
+    x = (torch.rand(R, 1, generator=gen)*6 - 3).to(T).cuda().requires_grad_()
+    w, b, off = torch.ones(1, 1, 1, dtype=T, device='cuda'), torch.zeros(1, 1, dtype=T, device='cuda'), offs([R - 1])
+    dy = rnd(gen, R, 1, T=T)
+    y = ops.grouped_linear(x, w, b, off, nonlin)
+    got, = torch.autograd.grad(y, x, dy)
+    f = torch.tanh if nonlin == 'tanh' else torch.sigmoid
+    v = f(x.detach().double())
+    want = dy.double()*(1 - v*v if nonlin == 'tanh' else v*(1 - v))
+    want[-1] = 0
+    # the gradient before the layer and the result are rounded, 2^-8 each; the slope is at least 1/103 (tanh) or 1/23, and the
+    # value's error, a few times 2^-24, twice that in the slope: less than 2^-13 of it
+    assert ((got.double() - want).abs() <= (2*2**-8 + 2**-13)*want.abs()).all()
+    wide = torch.zeros(R, 1, dtype=torch.float32, device='cuda')
+    wide[:] = f(x.detach().float())
+    same = ops.grouped_linear_grad(dy, wide, x.detach(), w, off, nonlin)[0]
+    assert ((same.double() - want).abs() <= (2*2**-8 + 2**-13)*want.abs()).all()
+    with pytest.raises(TypeErr):
+        ops.grouped_linear_grad(dy, wide.double(), x.detach(), w, off, nonlin)
+
+
+@pytest.mark.parametrize('K, N', [(8, 40), (64, 100), (256, 264), (40, 520)])
+def test_values_before_their_rounding(ops, K, N):
+    """ Every tile shape writes them, rounded they are the results, and rows behind the last group are zero in both. """
+    gen = torch.Generator().manual_seed(6)
+    for lengths in ([3, 0, 9], [300, 1, 1000], [5000, 4000]):
+        R = sum(lengths) + 5
+        x, w, b = rnd(gen, R, K, T=torch.bfloat16), rnd(gen, len(lengths), N, K, T=torch.bfloat16, scale=K**-.5), rnd(gen, len(lengths), N, T=torch.bfloat16)
+        y, wide = ops._linear_forward(x, w, b, offs(lengths), 'sigmoid', wide=True)
+        assert wide.dtype == torch.float32 and torch.equal(wide.to(torch.bfloat16), y) and not wide[-5:].any()
+        assert torch.equal(y, ops.grouped_linear(x, w, b, offs(lengths), 'sigmoid'))
