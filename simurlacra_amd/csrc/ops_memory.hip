@@ -415,6 +415,7 @@ template <class W, int NP, int LPC> struct Shape {
     static constexpr int NL = NP * LPC;                  // states, padded
     static constexpr int E = TS * CB >= THREADS ? TS * CB / THREADS : 1;
     static constexpr int LOADERS = TS * CB / E;          // threads that load (all but for the widest fp64 shape)
+    static constexpr int CP = CB + 64 / LPC;             // stride of rows that the lanes of a channel write one each of: other banks for each
 };
 
 template <class T> struct ScanArgs {
@@ -487,6 +488,10 @@ PSH_OP double halves16(double a, double b) {
     const auto h = __builtin_amdgcn_permlane16_swap((unsigned)__double2hiint(a), (unsigned)__double2hiint(b), false, false);
     return __hiloint2double((int)h[0], (int)l[0]) + __hiloint2double((int)h[1], (int)l[1]);
 }
+
+// The compiler takes x to be computed here.
+PSH_OP void fixed(float& x) { asm volatile("" : "+v"(x)); }
+PSH_OP void fixed(double& x) { asm volatile("" : "+v"(x)); }
 
 // Keeps the scheduler from running several steps' exponentials side by side: in fp64 one step has enough of them to fill the
 // pipe, and more do not fit into the registers.
@@ -621,11 +626,11 @@ template <class T> PSH_OP void work_of(const ScanArgs<T>& a, int& slot, int& blo
 template <class T, int NP, int LPC, bool CARRY> __global__ __launch_bounds__(THREADS) void k_scan(const ScanArgs<T> a) {
     typedef typename Wide<T>::type W;
     typedef Shape<W, NP, LPC> SH;
-    constexpr int TS = SH::TS, CB = SH::CB, E = SH::E, NL = SH::NL;
+    constexpr int TS = SH::TS, CB = SH::CB, CP = SH::CP, E = SH::E, NL = SH::NL;
     __shared__ Pair<W> s_dt[TS][CB];
     __shared__ __align__(16) W s_b[TS * NL];
     __shared__ __align__(16) W s_c[CARRY ? 1 : TS * NL];
-    __shared__ __align__(16) W s_y[CARRY ? 1 : TS][CB];
+    __shared__ __align__(16) W s_y[CARRY ? 1 : TS][CP];
     int slot, block;
     work_of(a, slot, block);
     const int c0 = block * CB;
@@ -684,7 +689,9 @@ template <class T, int NP, int LPC, bool CARRY> __global__ __launch_bounds__(THR
         if constexpr (!CARRY) {
             if (a.check && d < a.D) store_line<NP>(a.check + ((check0 + tile) * a.D + d) * a.N, h, n0, a.N, a.vec_n);
         }
-#pragma unroll 1
+        // (four states a lane keep a wave busy for long enough by four steps; fewer do not: 73 us rolled, 69 us unrolled for 32 policies' 256
+        // rollouts of 65437 steps, 96 channels, 8 states, fp32)
+#pragma unroll NP >= 4 ? 1 : TS
         for (int t1 = 0; t1 < TS; t1 += LPC < TS ? LPC : TS) {
             W keep = 0;
 #pragma unroll
@@ -802,14 +809,14 @@ template <class T, bool BACK> __global__ __launch_bounds__(256) void k_scan_join
 template <class T, int NP, int LPC, bool CARRY> __global__ __launch_bounds__(THREADS, 2) void k_scan_grad(const ScanArgs<T> a) {
     typedef typename Wide<T>::type W;
     typedef Shape<W, NP, LPC> SH;
-    constexpr int TS = SH::TS, CB = SH::CB, E = SH::E, NL = SH::NL;
+    constexpr int TS = SH::TS, CB = SH::CB, CP = SH::CP, E = SH::E, NL = SH::NL;
     constexpr int NV = 2 * NP < 4 ? 4 : 2 * NP;     // gradients of B and C of a step and lane, padded
     constexpr int GS = LPC < TS ? LPC : TS;         // steps whose sums the lanes of a channel collect, one each
     __shared__ Pair<W> s_dt[TS][CB];
     __shared__ __align__(16) W s_dy[TS][CB];
     __shared__ __align__(16) W s_sz[CARRY ? 1 : TS][CB], s_sd[CARRY ? 1 : TS][CB];   // sigmoids of z and of delta + bias
     __shared__ __align__(16) W s_b[TS * NL], s_c[TS * NL];
-    __shared__ __align__(16) W s_1[CARRY ? 1 : TS][CB], s_2[CARRY ? 1 : TS][CB], s_y[CARRY ? 1 : TS][CB];
+    __shared__ __align__(16) W s_1[CARRY ? 1 : TS][CP], s_2[CARRY ? 1 : TS][CP], s_y[CARRY ? 1 : TS][CP];
     __shared__ __align__(16) W s_bc[CARRY ? 1 : 4 * TS * 2 * NL];
     int slot, block;
     work_of(a, slot, block);
@@ -924,14 +931,13 @@ template <class T, int NP, int LPC, bool CARRY> __global__ __launch_bounds__(THR
                         h[i] = av[t][i] * h[i] + x.dtu * s_b[t * NL + n0 + i];
                         y += s_c[t * NL + n0 + i] * h[i];
                     }
-                    if (a.z) {
-                        y = sum_states<LPC>(y);
-                        keep = ql == t2 ? y : keep;
-                    }
+                    // (only needed with z, but a branch in every step costs more than the sum: nothing would be scheduled across it)
+                    y = sum_states<LPC>(y);
+                    keep = ql == t2 ? y : keep;
                     step_fence<W, NP>();
                     if (t2 % 4 == 3) __builtin_amdgcn_sched_barrier(0);   // (else every LDS read of the tile is hoisted to its top, into registers that it has not got)
                 }
-                if (a.z && ql < GS) s_y[t1 + ql][cl] = keep;
+                if (ql < GS) s_y[t1 + ql][cl] = keep;
             }
 #pragma unroll
             for (int t1 = TS - GS; t1 >= 0; t1 -= GS) {
@@ -970,6 +976,7 @@ template <class T, int NP, int LPC, bool CARRY> __global__ __launch_bounds__(THR
                         W s = halves16(v[2 * i], v[2 * i + 1]);
                         if constexpr (LPC < 16) s += dpp_move<0x128>(s);   // row_ror:8
                         if constexpr (LPC < 8) s += dpp_move<0x124>(s);    // row_ror:4
+                        fixed(s);   // (else the last sum goes into the branch, and its DPP move stays outside by itself)
                         const int row = lane >> 4, k = 2 * (2 * i + (row & 1)) + (row >> 1);
                         if ((lane & 15) < LPC && k < 2 * NP)
                             s_bc[((wave * TS + t) * 2 + k / NP) * NL + n0 + k % NP] = s;
@@ -1017,7 +1024,8 @@ template <class T, int NP, int LPC, bool CARRY> __global__ __launch_bounds__(THR
                 }
             }
         }
-        __syncthreads();
+        // (what follows here is written for the next tile by the thread that has just read it, or was last read in front of the barrier above)
+        if constexpr (CARRY) __syncthreads();
     }
     if constexpr (CARRY) {
         if (d >= a.D) return;
@@ -1171,6 +1179,8 @@ ScanPlan scan_plan(const psh_scan_desc* d, bool grad) {
         } else {
             while (lpc < widest && with(lpc) < 512) lpc *= 2;
         }
+    } else if (grad && with(least) < 1024 && lpc < widest) {
+        lpc *= 2;   // (a gradient step has twice the latency for the same bytes: 190 us on 4 lanes, 166 us on 8 for 256 rollouts of 65437 steps, 96 channels, 8 states, fp32)
     }
     with(lpc);
     return p;
