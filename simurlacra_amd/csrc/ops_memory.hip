@@ -445,9 +445,13 @@ template <class T> struct ScanArgs {
     W* part_bc;              // [channel blocks, rows, 2 N], NULL: one block, results go to dB and dC
 };
 
-// exp(dt A) from A prepared once per lane
-PSH_OP float decay_rate(float a) { return a * (float)PSH_LOG2E; }
-PSH_OP double decay_rate(double a) { return a; }
+// exp(dt A) from A prepared once per lane.  A of minus infinity (a state without memory) becomes the lowest finite number: the
+// steps behind a sequence's end in a tile are steps of size 0, which must leave a state as it is.
+PSH_OP float decay_rate(float a) {
+    const float r = a * (float)PSH_LOG2E;
+    return r < -3.4028234663852886e38f ? -3.4028234663852886e38f : r;
+}
+PSH_OP double decay_rate(double a) { return a < -1.7976931348623157e308 ? -1.7976931348623157e308 : a; }
 PSH_OP float decay(float dt, float rate) { return exp2_w(dt * rate); }
 PSH_OP double decay(double dt, double rate) { return exp_w(dt * rate); }
 // sum of g a h' A from a sum with prepared rates

@@ -313,3 +313,84 @@ def test_values_before_their_rounding(ops, K, N):
         y, wide = ops._linear_forward(x, w, b, offs(lengths), 'sigmoid', wide=True)
         assert wide.dtype == torch.float32 and torch.equal(wide.to(torch.bfloat16), y) and not wide[-5:].any()
         assert torch.equal(y, ops.grouped_linear(x, w, b, offs(lengths), 'sigmoid'))
+
+
+@pytest.mark.parametrize('T', TYPES, ids=IDS)
+def test_states_without_memory(ops, T):
+    """ A of minus infinity: exp(delta A) is 0, and neither the steps that fill up a tile nor the joining of pieces make a NaN of it. """
+    gen = torch.Generator().manual_seed(10)
+    lengths = [1, 33, 1900]
+    v, off, _ = scan_inputs(gen, ops, T, lengths, 20, 8, None, tail=0)
+    A = v['A'].clone()
+    A[:, :5], A[:, 7, 3] = -float('inf'), -float('inf')
+    args = (v['u'], v['delta'], A, v['B'], v['C'], None, None, None, off)
+    y, last, check = ops.selective_scan_check(*args, state=v['state'])
+    dt = torch.nn.functional.softplus(v['delta'].double())
+    want = dt*v['u'].double()*(v['B'].double()*v['C'].double()).sum(1, keepdim=True)
+    # a product of three and a sum of eight in T's wide type (20 roundings at the most, the step size's few among them), one rounding to T
+    e, w = torch.finfo(T).eps/2, torch.finfo(ops.wide_dtype(T)).eps/2
+    size = dt*v['u'].double().abs()*(v['B'].double()*v['C'].double()).abs().sum(1, keepdim=True)
+    assert ((y.double() - want)[:, :5].abs() <= e*want[:, :5].abs() + 20*w*size[:, :5]).all()
+    assert torch.isfinite(y).all() and torch.isfinite(last).all()
+    grads = ops.selective_scan_grad(y, last, check, *args, state=v['state'])
+    assert all(torch.isfinite(g).all() for g in grads if g is not None)
+    assert not grads[8][:, :5].any()
+
+
+@pytest.mark.parametrize('T', TYPES, ids=IDS)
+def test_numbers_that_are_none_stay_in_their_sequence(ops, T):
+    """ NaNs and infinities of one sequence and one group reach nothing of the others, and those behind the last row nothing at all. """
+    gen = torch.Generator().manual_seed(11)
+    W, D, N = ops.wide_dtype(T), 24, 16
+    lengths = [50, 37, 400, 21]
+    R = sum(lengths) + 4
+    bad, grp = slice(50, 87), offs([1, 1, 2])
+    v, off, _ = scan_inputs(gen, ops, T, lengths, D, N, [1, 1, 2], tail=4)
+    cw, cb, cs, dy = rnd(gen, 3, D, 4, T=W), rnd(gen, 3, D, T=W), rnd(gen, 4, D, 3, T=T), rnd(gen, R, D, T=T)
+    x, w, b, dyl = rnd(gen, R, 40, T=T), rnd(gen, 4, 72, 40, T=T, scale=.2), rnd(gen, 4, 72, T=T), rnd(gen, R, 72, T=T)
+    dlast = rnd(gen, 4, D, N, T=W)
+
+    def run():
+        args = (v['u'], v['delta'], v['A'], v['B'], v['C'], v['D'], v['z'], v['delta_bias'], off, grp, v['state'])
+        y, last, check = ops.selective_scan_check(*args)
+        g = ops.selective_scan_grad(dy, dlast, check, *args)
+        yc, lc = ops.causal_conv(v['u'], cw, cb, off, grp, cs, return_state=True)
+        gc = ops.causal_conv_grad(dy, None, v['u'], cw, cb, off, grp, cs)
+        yl = ops.grouped_linear(x, w, b, off, 'tanh')
+        gl = ops.grouped_linear_grad(dyl, yl, x, w, off, 'tanh')
+        rows = [y, g[0], g[1], g[3], g[4], yc, gc[0], yl, gl[0]]
+        seqs = [last, lc, gc[3], gl[1], gl[2]]
+        pols = [g[2], gc[1], gc[2]]
+        return ([torch.cat([t[:50], t[87:]]) for t in rows] + [torch.cat([t[:1], t[2:]]) for t in seqs] + [torch.cat([t[:1], t[2:]]) for t in pols])
+    want = [t.clone() for t in run()]
+    for t in (v['u'], v['delta'], v['B'], v['C'], v['z'], x, dy, dyl):
+        t[bad][::3] = float('nan')
+        t[bad][1::3] = float('inf')
+        t[-4:] = float('nan')
+    for got, ref in zip(run(), want):
+        assert torch.equal(got, ref)
+
+
+def test_the_largest_tiles_in_a_graph(ops):
+    """ Tiles that need more LDS than a kernel has without being asked: captured, replayed and against the eager call. """
+    gen = torch.Generator().manual_seed(12)
+    T, R, K, N = torch.bfloat16, 32768, 200, 768
+    off = offs([20000, 0, R - 20007])
+    x, w, dy = rnd(gen, R, K, T=T), rnd(gen, 3, N, K, T=T, scale=.1), rnd(gen, R, N, T=T)
+
+    def run():
+        return [ops.grouped_linear(x, w, None, off), *ops.grouped_linear_grad(dy, None, x, w, off)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = run()
+    for _ in range(3):
+        x.copy_(rnd(gen, R, K, T=T))
+        want = run()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
