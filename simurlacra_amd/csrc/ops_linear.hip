@@ -350,7 +350,7 @@ template <class T, int BI, int BJ, int WI, int WJ> struct Tile {
     // barrier says that they are in everyone's registers, so that their buffer can be filled again, and that the next step's tile is in LDS.
     // Reads of LDS and loads are issued between the matrix instructions, a few behind each block of rows: in one go they would hold the wave up
     // until the queues have taken them, with its matrix instructions behind them.
-    template <bool TP, bool TQ, bool SUMS> PSH_OP void multiply_direct(const Operand<bf16_t>& p, const Operand<bf16_t>& q, unsigned char* lds) {
+    template <bool TP, bool TQ, bool SUMS> PSH_OP void multiply_direct(const Operand<bf16_t>& p, const Operand<bf16_t>& q, unsigned char* lds, unsigned block_x) {
         typedef Direct<BI, THREADS, TP> DP;
         typedef Direct<BJ, THREADS, TQ> DQ;
         constexpr int KC = DP::KC, LOADS = DP::PER + DQ::PER;
@@ -365,7 +365,7 @@ template <class T, int BI, int BJ, int WI, int WJ> struct Tile {
         v4u fp[2][MI], fq[2][MJ];
         // Rows of c are often powers of two apart, and then one step's reads of all rows lie in one or two of the 16 channels of an L2, 256
         // bytes each.  So every workgroup of an XCD begins elsewhere, two steps from the one before it.
-        const int turn = whole > 0 ? (int)((blockIdx.x >> 3) * 2 % whole) : 0;
+        const int turn = whole > 0 ? (int)((block_x >> 3) * 2 % whole) : 0;
         const auto at = [&](int t) { return (t + turn < whole ? t + turn : t + turn - whole) * KC; };
         const auto bring = [&](int t, unsigned buf) {
             if (t < whole) {
@@ -514,10 +514,8 @@ template <class T, int COLS, class S> PSH_OP void store_tile(unsigned char* lds,
     }
 }
 
-template <class T, int BI, int BJ, int WI, int WJ, bool TW, bool DIRECT>
-__global__ __launch_bounds__(64 * WI * WJ, BI * BJ > 4096 || (sizeof(T) == 2 && TW) ? 2 : TW ? 3 : 4) void k_rows(const RowsArgs<T> a) {
-    extern __shared__ __align__(16) unsigned char lds[];
-    const long id = xcd_order(blockIdx.x, a.slots * a.tiles_i);
+template <class T, int BI, int BJ, int WI, int WJ, bool TW, bool DIRECT> PSH_OP void rows_tile(const RowsArgs<T>& a, unsigned block_x, unsigned char* lds) {
+    const long id = xcd_order(block_x, a.slots * a.tiles_i);
     if (id >= a.slots * a.tiles_i) return;
     // blocks of 8 tiles of units for all rows, one after the other: what the workgroups of an XCD read at a time stays in its L2
     const long block = id / (a.slots * 8), in_block = id - block * a.slots * 8, wide = a.tiles_i - block * 8 < 8 ? a.tiles_i - block * 8 : 8;
@@ -537,7 +535,7 @@ __global__ __launch_bounds__(64 * WI * WJ, BI * BJ > 4096 || (sizeof(T) == 2 && 
     const Operand<T> p{TW ? w + i0 : w + (long)i0 * a.ld_w, a.ld_w, ni, a.n_in};
     const Operand<T> x{a.rows_in + (long)q.begin * a.ld_in, a.ld_in, nj, a.n_in};
     Tile<T, BI, BJ, WI, WJ> tile;
-    if constexpr (DIRECT) tile.template multiply_direct<TW, false, false>(p, x, lds);
+    if constexpr (DIRECT) tile.template multiply_direct<TW, false, false>(p, x, lds, block_x);
     else tile.template multiply<TW, false, false>(p, x, lds);
     typedef typename Wide<T>::type W;
     const T* const b = a.bias ? a.bias + (long)q.part * a.stride_b + i0 : nullptr;
@@ -585,6 +583,11 @@ __global__ __launch_bounds__(64 * WI * WJ, BI * BJ > 4096 || (sizeof(T) == 2 && 
     else finish([](W x) { return x; });
     __syncthreads();
     store_tile<T, BI>(lds, a.out + (long)q.begin * a.n_out + i0, a.n_out, nj, ni, swz);
+}
+template <class T, int BI, int BJ, int WI, int WJ, bool TW, bool DIRECT>
+__global__ __launch_bounds__(64 * WI * WJ, BI * BJ > 4096 || (sizeof(T) == 2 && TW) ? 2 : TW ? 3 : 4) void k_rows(const RowsArgs<T> a) {
+    extern __shared__ __align__(16) unsigned char lds[];
+    rows_tile<T, BI, BJ, WI, WJ, TW, DIRECT>(a, blockIdx.x, lds);
 }
 
 // dp = dy f'(y), rounded to the element type as the gradient that reaches a layer's product in any composition of
@@ -642,11 +645,9 @@ template <class T> struct GradArgs {   // dW, db
     long slots, tiles_i, tiles_j;
 };
 
-template <class T, int BI, int BJ, int WI, int WJ, bool DIRECT>
-__global__ __launch_bounds__(64 * WI * WJ, BI * BJ > 4096 || sizeof(T) == 2 ? 2 : 3) void k_weights(const GradArgs<T> a) {
-    extern __shared__ __align__(16) unsigned char lds[];
+template <class T, int BI, int BJ, int WI, int WJ, bool DIRECT> PSH_OP void weights_tile(const GradArgs<T>& a, unsigned block_x, unsigned char* lds) {
     const long tiles = a.tiles_i * a.tiles_j, total = a.slots * tiles;
-    const long id = xcd_order(blockIdx.x, total);
+    const long id = xcd_order(block_x, total);
     if (id >= total) return;
     const int slot = (int)(id / tiles);
     const Piece q = find_piece(a.parts, slot);
@@ -659,8 +660,8 @@ __global__ __launch_bounds__(64 * WI * WJ, BI * BJ > 4096 || sizeof(T) == 2 ? 2 
     const bool whole = q.part_end - q.part_begin <= a.parts.L;   // no other piece: the result itself
     const bool sums = j0 == 0 && a.db;
     if constexpr (DIRECT) {
-        if (sums) tile.template multiply_direct<true, true, true>(p, x, lds);
-        else tile.template multiply_direct<true, true, false>(p, x, lds);
+        if (sums) tile.template multiply_direct<true, true, true>(p, x, lds, block_x);
+        else tile.template multiply_direct<true, true, false>(p, x, lds, block_x);
     } else {
         if (sums) tile.template multiply<true, true, true>(p, x, lds);
         else tile.template multiply<true, true, false>(p, x, lds);
@@ -705,6 +706,22 @@ __global__ __launch_bounds__(64 * WI * WJ, BI * BJ > 4096 || sizeof(T) == 2 ? 2 
     }
 }
 
+template <class T, int BI, int BJ, int WI, int WJ, bool DIRECT>
+__global__ __launch_bounds__(64 * WI * WJ, BI * BJ > 4096 || sizeof(T) == 2 ? 2 : 3) void k_weights(const GradArgs<T> a) {
+    extern __shared__ __align__(16) unsigned char lds[];
+    weights_tile<T, BI, BJ, WI, WJ, DIRECT>(a, blockIdx.x, lds);
+}
+
+// dW, db and dx in one launch, where both go by tiles of one kind: the first workgroups of dx begin while the last ones of dW run.
+// Together and one after the other: 64 groups of 1200 rows, 64 -> 64, fp64: 50 and 57 us; 12 of 2500, 513 -> 257, fp32: 299 and 317 us (53
+// TFLOP/s); 8 of 4096, 1024 -> 2048, bf16: 396 and 448 us (694 TFLOP/s).
+template <class T, int BIG, int SMALL, int WI, int WJ, bool DIRECT>
+__global__ __launch_bounds__(64 * WI * WJ, BIG * SMALL > 4096 || sizeof(T) == 2 ? 2 : 3) void k_both(const GradArgs<T> w, const RowsArgs<T> r, unsigned first) {
+    extern __shared__ __align__(16) unsigned char lds[];
+    if (blockIdx.x < first) weights_tile<T, SMALL, BIG, WI, WJ, DIRECT>(w, blockIdx.x, lds);
+    else rows_tile<T, BIG, SMALL, WI, WJ, true, DIRECT>(r, blockIdx.x - first, lds);
+}
+
 // sums of the pieces of the groups that have several, in the order of the rows
 template <class T> __global__ __launch_bounds__(256) void k_join(const GradArgs<T> a) {
     const long nw = a.dw ? (long)a.n * a.k : 0, nb = a.db ? a.n : 0;
@@ -733,12 +750,24 @@ template <class K> int allow_lds(psh_ctx* c, K kernel, int bytes) {
     return PSH_OK;
 }
 
-template <class T, int BI, int BJ, int WI, int WJ, bool TW, bool DIRECT> int launch_rows(psh_ctx* c, RowsArgs<T>& a, int rows, hipStream_t st) {
-    a.parts.L = BJ;
-    a.slots = parts_slots(rows, a.parts.n, BJ);
-    a.tiles_i = (a.n_out + BI - 1) / BI;
+constexpr int TOO_MANY = -1;   // (workgroups of a launch)
+
+// the grid of a call by such tiles, as a multiple of the 8 XCDs
+template <class T> long rows_grid(RowsArgs<T>& a, int rows, int bi, int bj) {
+    a.parts.L = bj;
+    a.slots = parts_slots(rows, a.parts.n, bj);
+    a.tiles_i = (a.n_out + bi - 1) / bi;
     const long total = (a.slots * a.tiles_i + 7) / 8 * 8;
-    if (total > 0x7fffffffL) { set_err(c, "grouped_linear: too many tiles for one launch"); return PSH_ERR_UNSUPPORTED; }
+    return total > 0x3fffffffL ? TOO_MANY : total;
+}
+int too_many_tiles(psh_ctx* c) {
+    set_err(c, "grouped_linear: too many tiles for one launch");
+    return PSH_ERR_UNSUPPORTED;
+}
+
+template <class T, int BI, int BJ, int WI, int WJ, bool TW, bool DIRECT> int launch_rows(psh_ctx* c, RowsArgs<T>& a, int rows, hipStream_t st) {
+    const long total = rows_grid(a, rows, BI, BJ);
+    if (total == TOO_MANY) return too_many_tiles(c);
     constexpr int lds = lds_bytes(BI, BJ, DIRECT);
     static_assert(lds >= BI * BJ * (int)sizeof(T), "a result tile goes through it");
     const auto kernel = k_rows<T, BI, BJ, WI, WJ, TW, DIRECT>;
@@ -749,23 +778,33 @@ template <class T, int BI, int BJ, int WI, int WJ, bool TW, bool DIRECT> int lau
     return PSH_OK;
 }
 
+enum TileKind { TILE_ROWS16, TILE_64, TILE_128, TILE_128_DIRECT, TILE_256_DIRECT };
+
 // Tiles [units][rows].  Large ones re-read the operands less often, small ones waste less where a group has few rows or a layer few
 // units, and there are more of them to fill the CUs: the larger ones are for layers that have one and a half of them for every CU.
 // bf16, 8 groups of about 4096 rows, 1024 -> 2048: 180 us (760 TFLOP/s) in 256 x 128 with two workgroups on a CU, of which one stores its tile
 // while the other multiplies; 197 us in 256 x 256 with one on a CU; 228 us in 128 x 128.  Without its loads from memory the first takes
 // 143 us, without those from LDS too 105 us.  12 groups of 2500 rows, 513 -> 257, fp32, 64 x 64: 122 us (65 TFLOP/s, the matrix pipes busy for
 // 65 % of the time, a fifth of it with columns behind the 257th).
-template <class T, bool TW> int run_rows(psh_ctx* c, RowsArgs<T>& a, int rows, hipStream_t st) {
+template <class T, bool TW> TileKind rows_kind(const RowsArgs<T>& a, int rows) {
     const long mean = rows / a.parts.n;
-    if (mean <= 24) return launch_rows<T, 64, 16, 4, 1, TW, false>(c, a, rows, st);
+    if (mean <= 24) return TILE_ROWS16;
     if constexpr (sizeof(T) == 2) {
         const long large = ((long)rows / 128 + a.parts.n / 2) * ((a.n_out + 127) / 128), huge = ((long)rows / 128 + a.parts.n / 2) * ((a.n_out + 255) / 256);
         if (mean >= 96 && a.n_out > 64 && large >= 192) {
             const bool direct = aligned16(a.rows_in, 2, a.ld_in) && aligned16(a.weight, 2, a.ld_w, a.stride_w) && (!TW || a.n_out % 8 == 0);
-            if (direct && mean >= 512 && a.n_out > 128 && huge >= 768) return launch_rows<T, 256, 128, 2, 2, TW, true>(c, a, rows, st);
-            if (direct) return launch_rows<T, 128, 128, 2, 2, TW, true>(c, a, rows, st);
-            return launch_rows<T, 128, 128, 2, 4, TW, false>(c, a, rows, st);
+            return !direct ? TILE_128 : mean >= 512 && a.n_out > 128 && huge >= 768 ? TILE_256_DIRECT : TILE_128_DIRECT;
         }
+    }
+    return TILE_64;
+}
+template <class T, bool TW> int run_rows(psh_ctx* c, RowsArgs<T>& a, int rows, hipStream_t st) {
+    const TileKind kind = rows_kind<T, TW>(a, rows);
+    if (kind == TILE_ROWS16) return launch_rows<T, 64, 16, 4, 1, TW, false>(c, a, rows, st);
+    if constexpr (sizeof(T) == 2) {
+        if (kind == TILE_128) return launch_rows<T, 128, 128, 2, 4, TW, false>(c, a, rows, st);
+        if (kind == TILE_128_DIRECT) return launch_rows<T, 128, 128, 2, 2, TW, true>(c, a, rows, st);
+        if (kind == TILE_256_DIRECT) return launch_rows<T, 256, 128, 2, 2, TW, true>(c, a, rows, st);
     }
     return launch_rows<T, 64, 64, 2, 2, TW, false>(c, a, rows, st);
 }
@@ -835,17 +874,25 @@ int check(psh_ctx* c, const psh_linear_desc* d, bool grad) {
     return PSH_OK;
 }
 
-template <class T, int BI, int BJ, int WI, int WJ, bool DIRECT> int launch_weights(psh_ctx* c, GradArgs<T>& a, int rows, hipStream_t st) {
+TileKind grad_kind(const psh_linear_desc* d) {
+    const int t = grad_tile(d);
+    return t == 64 ? TILE_64 : !grad_direct(d) ? TILE_128 : t == 128 ? TILE_128_DIRECT : TILE_256_DIRECT;
+}
+
+// the weight gradient, with the input gradient in the same launch if `r` is given
+template <class T, int BIG, int SMALL, int WI, int WJ, bool DIRECT> int launch_weights(psh_ctx* c, GradArgs<T>& a, RowsArgs<T>* r, int rows, hipStream_t st) {
     a.slots = parts_slots(rows, a.parts.n, a.parts.L);
-    a.tiles_i = (a.n + BI - 1) / BI;
-    a.tiles_j = a.dw ? (a.k + BJ - 1) / BJ : 1;
-    const long total = (a.slots * a.tiles_i * a.tiles_j + 7) / 8 * 8;
-    if (total > 0x7fffffffL) { set_err(c, "grouped_linear_grad: too many tiles for one launch"); return PSH_ERR_UNSUPPORTED; }
-    constexpr int lds = lds_bytes(BI, BJ, DIRECT);
-    const auto kernel = k_weights<T, BI, BJ, WI, WJ, DIRECT>;
-    const int rc = allow_lds(c, kernel, lds);
+    a.tiles_i = (a.n + SMALL - 1) / SMALL;
+    a.tiles_j = a.dw ? (a.k + BIG - 1) / BIG : 1;
+    const long total = (a.slots * a.tiles_i * a.tiles_j + 7) / 8 * 8, also = r ? rows_grid(*r, rows, BIG, SMALL) : 0;
+    if (total > 0x3fffffffL || also == TOO_MANY) return too_many_tiles(c);
+    constexpr int lds = lds_bytes(BIG, SMALL, DIRECT);
+    const auto alone = k_weights<T, SMALL, BIG, WI, WJ, DIRECT>;
+    const auto both = k_both<T, BIG, SMALL, WI, WJ, DIRECT>;
+    const int rc = r ? allow_lds(c, both, lds) : allow_lds(c, alone, lds);
     if (rc != PSH_OK) return rc;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)total), dim3(64 * WI * WJ), lds, st, a);
+    if (r) hipLaunchKernelGGL(both, dim3((unsigned)(total + also)), dim3(64 * WI * WJ), lds, st, a, *r, (unsigned)total);
+    else hipLaunchKernelGGL(alone, dim3((unsigned)total), dim3(64 * WI * WJ), lds, st, a);
     PSH_HIP(c, hipGetLastError());
     return PSH_OK;
 }
@@ -876,17 +923,22 @@ template <class T> int backward(psh_ctx* c, const psh_linear_desc* d) {
         dp = (const T*)space;
         ld_dp = d->out_dim;
     }
-    if (d->dx && d->rows > 0) {
-        RowsArgs<T> a{};
-        a.parts = Parts{d->offsets, d->n_groups, d->rows, 0};
-        a.rows_in = dp; a.ld_in = ld_dp;
-        a.weight = (const T*)d->weight; a.ld_w = d->ld_w; a.stride_w = d->stride_w;
-        a.out = (T*)d->dx;
-        a.n_in = d->out_dim; a.n_out = d->in_dim; a.nonlin = PSH_NL_NONE;
-        const int rc = run_rows<T, true>(c, a, d->rows, st);
-        if (rc != PSH_OK) return rc;
+    RowsArgs<T> r{};
+    const bool weights = d->dweight || d->dbias;
+    bool rows = d->dx && d->rows > 0;
+    if (rows) {
+        r.parts = Parts{d->offsets, d->n_groups, d->rows, 0};
+        r.rows_in = dp; r.ld_in = ld_dp;
+        r.weight = (const T*)d->weight; r.ld_w = d->ld_w; r.stride_w = d->stride_w;
+        r.out = (T*)d->dx;
+        r.n_in = d->out_dim; r.n_out = d->in_dim; r.nonlin = PSH_NL_NONE;
+        if (!weights || rows_kind<T, true>(r, d->rows) != grad_kind(d)) {
+            const int rc = run_rows<T, true>(c, r, d->rows, st);
+            if (rc != PSH_OK) return rc;
+            rows = false;
+        }
     }
-    if (d->dweight || d->dbias) {
+    if (weights) {
         GradArgs<T> a{};
         a.parts = Parts{d->offsets, d->n_groups, d->rows, (int)grad_piece(d)};
         a.dp = dp; a.ld_dp = ld_dp;
@@ -894,15 +946,16 @@ template <class T> int backward(psh_ctx* c, const psh_linear_desc* d) {
         a.dw = (T*)d->dweight; a.db = (T*)d->dbias;
         a.part_w = (W*)(space + s.dp); a.part_b = (W*)(space + s.dp + s.part_w);
         a.n = d->out_dim; a.k = d->in_dim;
+        RowsArgs<T>* const also = rows ? &r : nullptr;
+        const TileKind kind = grad_kind(d);
         int rc;
         if constexpr (sizeof(T) == 2) {
-            const int t = grad_tile(d);
-            if (t == 64) rc = launch_weights<T, 64, 64, 2, 2, false>(c, a, d->rows, st);
-            else if (!grad_direct(d)) rc = launch_weights<T, 128, 128, 2, 4, false>(c, a, d->rows, st);
-            else if (t == 128) rc = launch_weights<T, 128, 128, 2, 2, true>(c, a, d->rows, st);
-            else rc = launch_weights<T, 128, 256, 2, 2, true>(c, a, d->rows, st);
+            if (kind == TILE_64) rc = launch_weights<T, 64, 64, 2, 2, false>(c, a, also, d->rows, st);
+            else if (kind == TILE_128) rc = launch_weights<T, 128, 128, 2, 4, false>(c, a, also, d->rows, st);
+            else if (kind == TILE_128_DIRECT) rc = launch_weights<T, 128, 128, 2, 2, true>(c, a, also, d->rows, st);
+            else rc = launch_weights<T, 256, 128, 2, 2, true>(c, a, also, d->rows, st);
         } else {
-            rc = launch_weights<T, 64, 64, 2, 2, false>(c, a, d->rows, st);
+            rc = launch_weights<T, 64, 64, 2, 2, false>(c, a, also, d->rows, st);
         }
         if (rc != PSH_OK) return rc;
         if (s.part_w + s.part_b > 0) {
