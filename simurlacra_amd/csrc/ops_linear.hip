@@ -722,21 +722,36 @@ __global__ __launch_bounds__(64 * WI * WJ, BIG * SMALL > 4096 || sizeof(T) == 2 
     else rows_tile<T, BIG, SMALL, WI, WJ, true, DIRECT>(r, blockIdx.x - first, lds);
 }
 
-// sums of the pieces of the groups that have several, in the order of the rows
-template <class T> __global__ __launch_bounds__(256) void k_join(const GradArgs<T> a) {
+// sums of the pieces of the groups that have several, in the order of the rows; V elements a thread (V divides n k), their loads of all
+// pieces in flight together
+template <class T, int V> __global__ __launch_bounds__(256) void k_join(const GradArgs<T> a) {
+    typedef typename Wide<T>::type W;
     const long nw = a.dw ? (long)a.n * a.k : 0, nb = a.db ? a.n : 0;
     for (int g = blockIdx.y; g < a.parts.n; g += gridDim.y) {
         const int begin = a.parts.at(g), end = a.parts.at(g + 1);
         if (end - begin <= a.parts.L) continue;
         const int pieces = (int)(((long)end - begin + a.parts.L - 1) / a.parts.L), first = a.parts.first_slot(g);
-        for (long e = (long)blockIdx.x * 256 + threadIdx.x; e < nw + nb; e += (long)gridDim.x * 256) {
-            const bool w = e < nw;
-            const typename Wide<T>::type* const src = w ? a.part_w + (long)first * nw + e : a.part_b + (long)first * nb + (e - nw);
-            const long stride = w ? nw : nb;
-            typename Wide<T>::type s = 0;
-            for (int j = 0; j < pieces; ++j) s += src[j * stride];
-            if (w) a.dw[(long)g * nw + e] = to_elem<T>(s);
-            else a.db[(long)g * nb + e - nw] = to_elem<T>(s);
+        const long threads = (long)gridDim.x * 256, me = (long)blockIdx.x * 256 + threadIdx.x;
+        for (long e = me * V; e < nw; e += threads * V) {
+            const W* const src = a.part_w + (long)first * nw + e;
+            W s[V] = {};
+            T out[V];
+#pragma unroll 4
+            for (int j = 0; j < pieces; ++j) {
+                W v[V];
+                __builtin_memcpy(v, src + j * nw, sizeof(v));
+#pragma unroll
+                for (int i = 0; i < V; ++i) s[i] += v[i];
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) out[i] = to_elem<T>(s[i]);
+            __builtin_memcpy(a.dw + (long)g * nw + e, out, sizeof(out));
+        }
+        for (long e = me; e < nb; e += threads) {
+            const W* const src = a.part_b + (long)first * nb + e;
+            W s = 0;
+            for (int j = 0; j < pieces; ++j) s += src[j * nb];
+            a.db[(long)g * nb + e] = to_elem<T>(s);
         }
     }
 }
@@ -960,9 +975,14 @@ template <class T> int backward(psh_ctx* c, const psh_linear_desc* d) {
         if (rc != PSH_OK) return rc;
         if (s.part_w + s.part_b > 0) {
             const long n = (long)a.n * (a.k + 1);
-            const unsigned bx = (unsigned)((n + 255) / 256 < 1024 ? (n + 255) / 256 : 1024);
+            // 16 bytes a thread once there are threads enough for four workgroups a CU: 37 us for 56 us where 24 pieces of 2048 x 1024 are summed, 10 us
+            // for 7.6 us with 64 groups of 64 x 64
+            const bool wide = (long)a.n * a.k % 4 == 0 && (int64_t)d->n_groups * n >= (1 << 20);
+            const long blocks = (n + (wide ? 1023 : 255)) / (wide ? 1024 : 256);
+            const unsigned bx = (unsigned)(blocks < 1024 ? blocks : 1024);
             const unsigned gy = (unsigned)(d->n_groups < 65535 ? d->n_groups : 65535);
-            hipLaunchKernelGGL(k_join<T>, dim3(bx, gy), dim3(256), 0, st, a);
+            if (wide) hipLaunchKernelGGL((k_join<T, 4>), dim3(bx, gy), dim3(256), 0, st, a);
+            else hipLaunchKernelGGL((k_join<T, 1>), dim3(bx, gy), dim3(256), 0, st, a);
             PSH_HIP(c, hipGetLastError());
         }
     }
