@@ -591,7 +591,7 @@ __global__ __launch_bounds__(64 * WI * WJ, BI * BJ > 4096 || (sizeof(T) == 2 && 
 }
 
 // dp = dy f'(y), rounded to the element type as the gradient that reaches a layer's product in any composition of
-// layers is.  Rows behind the last group have no part in any sum.
+// layers is.  Rows behind the last group have no part in any sum.  Bound by bytes: 76800 x 64 fp64 in 19 us (6.2 TB/s, two reads and a write).
 // A thread takes V neighbouring elements, which lie in one row (V divides its length, or the rows follow one another).
 template <class T, class Y, int V> __global__ __launch_bounds__(256) void k_preact(long n, int cols, const T* dy, long ld, const Y* y, int nonlin, T* dp) {
     for (long k = ((long)blockIdx.x * 256 + threadIdx.x) * V; k < n; k += (long)gridDim.x * 256 * V) {
@@ -795,10 +795,12 @@ template <class T, int BI, int BJ, int WI, int WJ, bool TW, bool DIRECT> int lau
 
 enum TileKind { TILE_ROWS16, TILE_64, TILE_128, TILE_128_DIRECT, TILE_256_DIRECT };
 
+// Few rows a group (up to 24): 16 of them a tile.  64 groups of 10 rows, 1024 -> 1024, bf16: 23 to 25 us (5.4 TB/s of weights; 30 us in
+// 64 x 64); 256 groups of 8 rows, 6 -> 64, fp64: 5.9 us, a launch's latency (8.7 us).
 // Tiles [units][rows].  Large ones re-read the operands less often, small ones waste less where a group has few rows or a layer few
 // units, and there are more of them to fill the CUs: the larger ones are for layers that have one and a half of them for every CU.
 // bf16, 8 groups of about 4096 rows, 1024 -> 2048: 180 us (760 TFLOP/s) in 256 x 128 with two workgroups on a CU, of which one stores its tile
-// while the other multiplies; 197 us in 256 x 256 with one on a CU; 228 us in 128 x 128.  Without its loads from memory the first takes
+// while the other multiplies; 197 us in 256 x 256 with one on a CU; 228 us in 128 x 128; 318 us in 64 x 64 (dx 174 and 633 us).  Without its loads from memory the first takes
 // 143 us, without those from LDS too 105 us.  12 groups of 2500 rows, 513 -> 257, fp32, 64 x 64: 122 us (65 TFLOP/s, the matrix pipes busy for
 // 65 % of the time, a fifth of it with columns behind the 257th).
 template <class T, bool TW> TileKind rows_kind(const RowsArgs<T>& a, int rows) {

@@ -58,9 +58,11 @@ template <int E, class T> PSH_OP typename Vec<T, E>::type load_raw(const T* line
 }
 
 // ====================================================================================================== convolution
-// A lane holds V neighbouring channels and walks down TL rows with the last K inputs in registers, so every input is
-// read once (K - 1 rows in TL again at a run's start).  One wave: one piece of a sequence, its lanes split over the channels
-// first and over runs of TL rows with what is left of the 64.
+// y[t, d] = f(b[d] + sum_k w[d, k] x[t - (K - 1) + k, d]).  A lane holds V neighbouring channels (16 bytes) and walks down a run of rows with
+// the last K inputs in registers, so every input is read once (K - 1 rows of a run again at its start).  One wave: one piece
+// of a sequence, its lanes split over the channels first and over runs with what is left of the 64.
+// Bound by the bytes of x and y: 120000 x 128 fp32 in 32 us (3.9 TB/s; a copy reaches 4.7), 131072 x 256 bf16 in 42 us
+// (3.2 TB/s: of its 2-byte values twice as many have to go through an exponential and a reciprocal in the same time).
 template <class T> struct ConvArgs {
     Parts parts;
     Policies pol;
@@ -157,7 +159,8 @@ template <class T, int V, int K> __global__ __launch_bounds__(256) void k_conv(c
     }
 }
 
-// One row per sequence.  A wave takes step_seqs() neighbouring sequences and 64 channels: with one policy (ONE) their parameters are read
+// One row per sequence: 16384 sequences of 128 channels in fp32 take 11.4 us (5.9 TB/s, nothing but the carried inputs, x and y).
+// A wave takes step_seqs() neighbouring sequences and 64 channels: with one policy (ONE) their parameters are read
 // once.  A thread reads its carried inputs before it writes the new ones, which may be in the same place.
 template <class T> constexpr int step_seqs() { return sizeof(T) == 8 ? 2 : 4; }
 template <class T, int K, bool ONE> __global__ __launch_bounds__(256) void k_conv_step(const ConvArgs<T> a, int n_seqs, int per_row) {
@@ -196,6 +199,7 @@ template <class T, int K, bool ONE> __global__ __launch_bounds__(256) void k_con
 // dx[t] = sum_k w[k] dpre[t + K-1-k],  dw[k] = sum_t dpre[t] x[t - (K-1) + k],  db = sum_t dpre[t],  dpre = dy f'(pre).
 // A run of rows needs dpre of K - 1 rows behind it, which it computes itself from the inputs (again): nothing but x and dy is read.
 // Rows t < 0 of a sequence are its carried inputs: the first run of a sequence computes their gradients too.
+// 131072 x 256 bf16: 82 us (2.5 TB/s); the vector pipes are busy for 71 % of that, with 60 instructions an element.
 template <class T, int V, int K> __global__ __launch_bounds__(256) void k_conv_grad(const ConvArgs<T> a, long slots) {
     typedef typename Wide<T>::type W;
     const long slot = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -319,7 +323,7 @@ template <class T, int V, int K> __global__ __launch_bounds__(256) void k_conv_g
 
 // ============================================================================== sums over the pieces of a policy
 // out[p, m] = sum of part[slot, m] over the slots of policy p's sequences, in two passes of about the square root of their
-// number, in the order of the slots.  `slot_of(p)`: the first slot of policy p.
+// number, in the order of the slots: 4 to 9 us each, the time of a few dependent loads.  `slot_of(p)`: the first slot of policy p.
 template <class W> struct JoinArgs {
     Parts parts;
     Policies pol;
@@ -408,6 +412,8 @@ template <class W> int run_join(psh_ctx* c, JoinArgs<W>& a, long slots, hipStrea
 // channels that the gradients of B and C need starts in registers.  A workgroup of 4 waves runs 256 / LPC channels over one
 // piece of a sequence, TS steps at a time: it loads the TS x channels tiles of u, delta (and z, dy) together, one 8- or
 // 16-byte load per thread and array, computes the step sizes once per element, and leaves dt and dt u in LDS for the steps.
+// TS = 16 steps (8 in fp64) are also as far apart as the states that the forward pass stores for the gradient (`check`): 4 N / TS
+// bytes an element, where storing every state would be 16 times as many, and computing from the beginning again impossible.
 constexpr int THREADS = 256;
 template <class W, int NP, int LPC> struct Shape {
     static constexpr int TS = sizeof(W) == 8 ? 8 : 16;   // steps of a tile = distance of the stored states
@@ -571,7 +577,8 @@ template <class T, class SH> struct StepRows {
 };
 
 // Sequences from the longest to the shortest (to 1/256 of the longest), for launches of whole sequences: workgroups are
-// handed out in this order, so that those that run last, or that share a CU, are not by chance the long ones.
+// handed out in this order, so that those that run last, or that share a CU, are not by chance the long ones.  It takes 3 us; 500 sequences
+// of 120000 rows, 128 channels, then take 89 us for 132 us as they come, the gradient of 256 of 131072 rows, 256 channels, 600 us for 809 us.
 constexpr int ORDER_MOST = 16384;   // sequences; with more, chance evens the CUs out
 __global__ __launch_bounds__(1024) void k_order(const Parts p, int* order) {
     __shared__ int count[256], most;
@@ -625,7 +632,10 @@ template <class T> PSH_OP void work_of(const ScanArgs<T>& a, int& slot, int& blo
     block = (int)(i % blocks);
 }
 
-// h_t along a piece.  CARRY: only the state at the piece's end from zero and the sum of its step sizes, for the joining
+// h_t = exp(dt_t A) h_{t-1} + dt_t u_t B_t and y_t = (C_t . h_t + D u_t) silu(z_t) along a piece.
+// Bound by instruction issue: a state costs an exponential (16 cycles a wave) and four or five others (4 each) a step, 32 to 36 cycles; the vector
+// pipes are busy all the time.  131072 x 256 x 16 states, bf16, with `check`: 164 us (2.5 TB/s); 120000 x 128 x 16, fp32, without: 89 us.
+// CARRY: only the state at the piece's end from zero and the sum of its step sizes, for the joining
 // of pieces; otherwise y as well, from the state at the piece's beginning.
 template <class T, int NP, int LPC, bool CARRY> __global__ __launch_bounds__(THREADS) void k_scan(const ScanArgs<T> a) {
     typedef typename Wide<T>::type W;
@@ -750,6 +760,7 @@ template <class T, int NP, int LPC, bool CARRY> __global__ __launch_bounds__(THR
 // (BACK) from the adjoint state at every piece's beginning to that at its end, from the last piece on.
 // A piece maps its beginning h to P h + own with P = exp(A sum dt), and such maps compose: 8 threads take an eighth of the
 // pieces of a state each, compose them, find their beginnings from the eighths before, and walk through theirs again.
+// 9 us for 256 pieces of 4096 states; 52 us with one thread a state.
 constexpr int JOIN_GROUPS = 8, JOIN_COLS = 256 / JOIN_GROUPS;
 template <class T, bool BACK> __global__ __launch_bounds__(256) void k_scan_join(const ScanArgs<T> a) {
     typedef typename Wide<T>::type W;
@@ -809,7 +820,12 @@ template <class T, bool BACK> __global__ __launch_bounds__(256) void k_scan_join
 
 // The adjoint recurrence of a piece, tiles of TS steps from its end:  g_t = C_t dy0_t + G_{t+1},  G_t = a_t g_t,  where dy0 = dy silu(z).
 // Each tile first runs forward from its stored state and keeps a_t and h_{t-1} of its steps in registers (2 TS NP values
-// per lane), then backward.  CARRY: only G at the piece's beginning, from zero.
+// per lane), then backward:  dA += G h_{t-1} dt,  ddt = sum_n G h_{t-1} A + u sum_n g B,  du = dt sum_n g B + D dy0,  and, summed over
+// the channels, dB = g dt u and dC = dy0 h.  The sums over a wave's 16 channels swap halves and quarters of the wave, so that eight sums
+// take 16 instructions; those over the waves go through LDS, those over workgroups through memory (k_sum_bc), none by atomics.
+// Bound by instruction issue at two waves a SIMD: 100 instructions a step for four states of 16 channels, 64 of them for the states, 28 for the
+// sums.  131072 x 256 x 16 states, bf16: 600 us; 65437 x 96 x 8, fp32, 256 sequences: 142 us, the time of the longest of them.
+// CARRY: only G at the piece's beginning, from zero.
 template <class T, int NP, int LPC, bool CARRY> __global__ __launch_bounds__(THREADS, 2) void k_scan_grad(const ScanArgs<T> a) {
     typedef typename Wide<T>::type W;
     typedef Shape<W, NP, LPC> SH;
@@ -1066,7 +1082,7 @@ template <class T, int NP, int LPC, bool CARRY> __global__ __launch_bounds__(THR
     }
 }
 
-// dB and dC from the channel blocks' sums
+// dB and dC from the channel blocks' sums (131072 rows of 2 x 16 sums from four blocks: 23 us, 3.2 TB/s)
 template <class T> __global__ __launch_bounds__(256) void k_sum_bc(const typename Wide<T>::type* part, long rows, const int* off, int n_seqs, int blocks, int N, T* dB, T* dC) {
     const Parts p{off, n_seqs, (int)rows, 1};
     const long stop = p.at(n_seqs) * 2L * N;
@@ -1082,6 +1098,7 @@ template <class T> __global__ __launch_bounds__(256) void k_sum_bc(const typenam
 
 // One step of every sequence: states read and written once, 4 lanes per channel with 4 neighbouring states each, 16
 // states per turn of the loop, step_seqs() neighbouring sequences a wave, whose loads are in flight together.  `last` may be `state`.
+// Bound by the states' bytes: 16384 sequences of 128 x 16 fp32 states take 52 us (5.5 TB/s); one sequence in fp64 takes 4.4 us, a launch's latency.
 template <class T, bool ONE> __global__ __launch_bounds__(256) void k_scan_step(const ScanArgs<T> a, int n_seqs, int per_row) {
     typedef typename Wide<T>::type W;
     constexpr int STEP_SEQS = step_seqs<T>();
@@ -1153,7 +1170,9 @@ int64_t tile_steps(int dtype) { return dtype == PSH_F64 ? 8 : 16; }
 // How a call's channels and rows are cut.  A step takes a wave 150 to 400 cycles however few waves there are, and a SIMD needs
 // two of them to be busy.  Long sequences that are too few for that are cut into pieces, at the price of a second pass over
 // the decays and of two more launches; short ones have their states spread over more lanes instead (more waves with a
-// shorter step each, at the price of its fixed work).
+// shorter step each, at the price of its fixed work).  Where sequences have more than 192 rows on average the pieces win: one
+// of 16384 rows, 256 channels, 16 states, bf16, takes 1536 us spread and 55 us in 256 pieces; 64 of 300 rows, 64 x 16, fp64, 147 and 87 us
+// (gradient 265 and 133 us).
 struct ScanPlan {
     int np, lpc, blocks;   // states a lane, lanes a channel, channel blocks
     int64_t piece;         // rows
@@ -1419,7 +1438,7 @@ int conv_vec(const psh_conv_desc* d, bool grad) {
     return ok ? V : 1;
 }
 // Rows of a run: a run reads K - 1 rows (the gradient computes as many) that the next one reads again, so they are as long as leaves
-// two waves a SIMD.  One episode of 16384 steps, 256 channels, bf16: 14 us in runs of 16, FIGURE_C in runs of 4.
+// two waves a SIMD.  One episode of 16384 steps, 256 channels, bf16: 14 us in runs of 16, 11 us in runs of 4.
 int conv_run(const psh_conv_desc* d, int V, bool grad) {
     const int lanes = lanes_for(d->channels, V);
     const int64_t across = (d->channels + lanes * V - 1) / (lanes * V);
