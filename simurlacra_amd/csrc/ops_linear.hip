@@ -244,6 +244,7 @@ template <class T, int BI, int BJ, int WI, int WJ> struct Tile {
     // sums of P over c, in every column (the bias gradient), if asked for: a block of 16 indices i is summed by one of the WJ waves that have it
     static constexpr int OWN = MI / WJ > 0 ? MI / WJ : 1;
     acc_t ones[OWN];
+    acc_t block[sizeof(T) == 4 ? OWN : 1];   // those of the last few steps, see fold()
     int wave_j;
 
     template <int K, bool SUMS> PSH_OP void part(const v4u (&fp)[MI], const v4u (&fq)[MJ], const v4u& unit) {
@@ -259,7 +260,7 @@ template <class T, int BI, int BJ, int WI, int WJ> struct Tile {
         for (int w = 0; w < WJ; ++w)
             if (w == wave_j)
 #pragma unroll
-                for (int k = 0; k < OWN; ++k) Mfma<T>::template step<K>(fp[w * OWN + k], unit, ones[k]);
+                for (int k = 0; k < OWN; ++k) Mfma<T>::template step<K>(fp[w * OWN + k], unit, sizeof(T) == 4 ? block[sizeof(T) == 4 ? k : 0] : ones[k]);
     }
 
     template <bool SUMS> PSH_OP void clear(v4u& unit) {
@@ -272,10 +273,23 @@ template <class T, int BI, int BJ, int WI, int WJ> struct Tile {
             wave_j = wave_id() / WI;
 #pragma unroll
             for (int k = 0; k < OWN; ++k) ones[k] = acc_t{0, 0, 0, 0};
+            if constexpr (sizeof(T) == 4)
+#pragma unroll
+                for (int k = 0; k < OWN; ++k) block[k] = acc_t{0, 0, 0, 0};
             T e[16 / sizeof(T)];
 #pragma unroll
             for (int k = 0; k < (int)(16 / sizeof(T)); ++k) e[k] = to_elem<T>(1);
             unit = __builtin_bit_cast(v4u, e);
+        }
+    }
+    // A sum of n numbers one after the other in fp32 is off by about sqrt(n / 2) roundings of itself, one of blocks' sums by that of a block.  The sums of
+    // products have library products of the same kind beside them; those of the rows themselves, which are usually summed in a tree,
+    // are kept in blocks of 128 rows (2500 rows: 4.8e-7 in one go, 2.7e-7 in blocks).
+    PSH_OP void fold() {
+#pragma unroll
+        for (int k = 0; k < OWN; ++k) {
+            ones[k] += block[k];
+            block[k] = acc_t{0, 0, 0, 0};
         }
     }
     template <bool SUMS> PSH_OP void parts(const v4u (&fp)[MI], const v4u (&fq)[MJ], const v4u& unit) {
@@ -342,6 +356,8 @@ template <class T, int BI, int BJ, int WI, int WJ> struct Tile {
             if (t + 1 < tiles) read(0, nxt);
             __builtin_amdgcn_sched_barrier(0);
             if (second) parts<SUMS>(fp[1], fq[1], unit);
+            if constexpr (SUMS && sizeof(T) == 4)
+                if ((t & 3) == 3 || t + 1 == tiles) fold();
         }
     }
 
@@ -736,12 +752,17 @@ template <class T, int V> __global__ __launch_bounds__(256) void k_join(const Gr
             const W* const src = a.part_w + (long)first * nw + e;
             W s[V] = {};
             T out[V];
+            for (int j0 = 0; j0 < pieces; j0 += 32) {   // (in blocks, for the same reason as in fold())
+                W p[V] = {};
 #pragma unroll 4
-            for (int j = 0; j < pieces; ++j) {
-                W v[V];
-                __builtin_memcpy(v, src + j * nw, sizeof(v));
+                for (int j = j0; j < min(pieces, j0 + 32); ++j) {
+                    W v[V];
+                    __builtin_memcpy(v, src + j * nw, sizeof(v));
 #pragma unroll
-                for (int i = 0; i < V; ++i) s[i] += v[i];
+                    for (int i = 0; i < V; ++i) p[i] += v[i];
+                }
+#pragma unroll
+                for (int i = 0; i < V; ++i) s[i] += p[i];
             }
 #pragma unroll
             for (int i = 0; i < V; ++i) out[i] = to_elem<T>(s[i]);
@@ -750,7 +771,11 @@ template <class T, int V> __global__ __launch_bounds__(256) void k_join(const Gr
         for (long e = me; e < nb; e += threads) {
             const W* const src = a.part_b + (long)first * nb + e;
             W s = 0;
-            for (int j = 0; j < pieces; ++j) s += src[j * nb];
+            for (int j0 = 0; j0 < pieces; j0 += 32) {
+                W p = 0;
+                for (int j = j0; j < min(pieces, j0 + 32); ++j) p += src[j * nb];
+                s += p;
+            }
             a.db[(long)g * nb + e] = to_elem<T>(s);
         }
     }
