@@ -199,7 +199,7 @@ template <class T, int K, bool ONE> __global__ __launch_bounds__(256) void k_con
 // dx[t] = sum_k w[k] dpre[t + K-1-k],  dw[k] = sum_t dpre[t] x[t - (K-1) + k],  db = sum_t dpre[t],  dpre = dy f'(pre).
 // A run of rows needs dpre of K - 1 rows behind it, which it computes itself from the inputs (again): nothing but x and dy is read.
 // Rows t < 0 of a sequence are its carried inputs: the first run of a sequence computes their gradients too.
-// 131072 x 256 bf16: 82 us (2.5 TB/s); the vector pipes are busy for 71 % of that, with 60 instructions an element.
+// 131072 x 256 bf16: 82 us (2.5 TB/s); the vector pipes are busy for 71 % of that, with 47 instructions an element.
 template <class T, int V, int K> __global__ __launch_bounds__(256) void k_conv_grad(const ConvArgs<T> a, long slots) {
     typedef typename Wide<T>::type W;
     const long slot = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -823,8 +823,8 @@ template <class T, bool BACK> __global__ __launch_bounds__(256) void k_scan_join
 // per lane), then backward:  dA += G h_{t-1} dt,  ddt = sum_n G h_{t-1} A + u sum_n g B,  du = dt sum_n g B + D dy0,  and, summed over
 // the channels, dB = g dt u and dC = dy0 h.  The sums over a wave's 16 channels swap halves and quarters of the wave, so that eight sums
 // take 16 instructions; those over the waves go through LDS, those over workgroups through memory (k_sum_bc), none by atomics.
-// Bound by instruction issue at two waves a SIMD: 100 instructions a step for four states of 16 channels, 64 of them for the states, 28 for the
-// sums.  131072 x 256 x 16 states, bf16: 600 us; 65437 x 96 x 8, fp32, 256 sequences: 142 us, the time of the longest of them.
+// Bound by instruction issue at two waves a SIMD: 100 instructions a step for four states of 16 channels, 52 of them the formulas, 33 the
+// sums, the rest reads of LDS and waits.  131072 x 256 x 16 states, bf16: 600 us; 65437 x 96 x 8, fp32, 256 sequences: 142 us, the time of the longest of them.
 // CARRY: only G at the piece's beginning, from zero.
 template <class T, int NP, int LPC, bool CARRY> __global__ __launch_bounds__(THREADS, 2) void k_scan_grad(const ScanArgs<T> a) {
     typedef typename Wide<T>::type W;
