@@ -342,9 +342,12 @@ template <class T, int BI, int BJ, int WI, int WJ> struct Tile {
         if (tiles > 1) fetch(1);
         __syncthreads();
         read(0, lds);
-        for (int t = 0; t < tiles; ++t) {
-            unsigned char* const cur = lds + (t & 1) * (BI + BJ) * 128;
-            unsigned char* const nxt = lds + (~t & 1) * (BI + BJ) * 128;
+        // (two steps a turn, in which the buffer is a constant of the code and goes into the offsets of the LDS instructions: 115 us for 122 us in 12
+        // groups of 2500 rows, 513 -> 257, fp32; not where both operands are transposed, V lines a thread: their registers do not suffice, 350 us for 298 us)
+        constexpr bool TWO = sizeof(T) == 8 || !TQ;
+        const auto step = [&](auto buffer, int t) {
+            unsigned char* const cur = lds + (int)buffer * (BI + BJ) * 128;
+            unsigned char* const nxt = lds + (1 - (int)buffer) * (BI + BJ) * 128;
             const bool second = nc - t * KC > KC / 2;   // (else nothing but zeros there)
             if (second) read(1, cur);
             __builtin_amdgcn_sched_barrier(0);
@@ -358,6 +361,14 @@ template <class T, int BI, int BJ, int WI, int WJ> struct Tile {
             if (second) parts<SUMS>(fp[1], fq[1], unit);
             if constexpr (SUMS && sizeof(T) == 4)
                 if ((t & 3) == 3 || t + 1 == tiles) fold();
+        };
+        if constexpr (TWO) {
+            for (int t = 0; t < tiles; t += 2) {
+                step(std::integral_constant<int, 0>(), t);
+                if (t + 1 < tiles) step(std::integral_constant<int, 1>(), t + 1);
+            }
+        } else {
+            for (int t = 0; t < tiles; ++t) step(t & 1, t);
         }
     }
 
@@ -826,8 +837,8 @@ enum TileKind { TILE_ROWS16, TILE_64, TILE_128, TILE_128_DIRECT, TILE_256_DIRECT
 // units, and there are more of them to fill the CUs: the larger ones are for layers that have one and a half of them for every CU.
 // bf16, 8 groups of about 4096 rows, 1024 -> 2048: 180 us (760 TFLOP/s) in 256 x 128 with two workgroups on a CU, of which one stores its tile
 // while the other multiplies; 197 us in 256 x 256 with one on a CU; 228 us in 128 x 128; 318 us in 64 x 64 (dx 174 and 633 us).  Without its loads from memory the first takes
-// 143 us, without those from LDS too 105 us.  12 groups of 2500 rows, 513 -> 257, fp32, 64 x 64: 122 us (65 TFLOP/s, the matrix pipes busy for
-// 65 % of the time, a fifth of it with columns behind the 257th).
+// 143 us, without those from LDS too 105 us.  12 groups of 2500 rows, 513 -> 257, fp32, 64 x 64: 115 us (69 TFLOP/s, the matrix pipes busy for
+// two thirds of the time, a fifth of it with columns behind the 257th).
 template <class T, bool TW> TileKind rows_kind(const RowsArgs<T>& a, int rows) {
     const long mean = rows / a.parts.n;
     if (mean <= 24) return TILE_ROWS16;
