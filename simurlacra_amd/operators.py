@@ -127,12 +127,12 @@ def _workspace(n, device):
     return torch.empty(n, dtype=torch.uint8, device=device) if n > 0 else None
 
 
-def _give_workspace(eng, desc, name, device):
-    """ The scratch memory of a call, written into its descriptor; it has to outlive the call. """
+def _give_workspace(eng, desc, name, like):
+    """ The scratch memory of a call, on the GPU of `like`, written into its descriptor; it has to outlive the call. """
     n = _size(eng, name, desc)
     if n == 0:
         return None
-    space = torch.empty(n, dtype=torch.uint8, device=device)
+    space = like.new_empty(-(-n//like.element_size()))   # (new_empty of plain sizes takes half the time of torch.empty with type and device)
     desc.workspace, desc.workspace_bytes = space.data_ptr(), n
     return space
 
@@ -182,7 +182,7 @@ def _linear_forward(x, weight, bias, offsets, nonlin, wide=False):
     """ The layer's results, and with `wide` also what the gradient takes the nonlinearity's slope from: the results
     before their rounding where that makes a difference. """
     eng, d, keep, R, K, G, N, dt, dev = _linear_desc(x, weight, bias, offsets, nonlin)
-    y = torch.empty((R, N), dtype=dt, device=dev)
+    y = x.new_empty(R, N)
     d.y = y.data_ptr()
     value = y
     if wide and dt == torch.bfloat16 and nonlin in ('tanh', 'sigmoid'):
@@ -209,15 +209,15 @@ def grouped_linear_grad(dy, y, x, weight, offsets, nonlin=None, want=(True, True
             d.y = y.data_ptr()
     dx = dw = db = None
     if want[0]:
-        dx = torch.empty((R, K), dtype=dt, device=dev)
+        dx = x.new_empty(R, K)
         d.dx = dx.data_ptr()
     if want[1]:
-        dw = torch.empty((G, N, K), dtype=dt, device=dev)
+        dw = x.new_empty(G, N, K)
         d.dweight = dw.data_ptr()
     if want[2]:
-        db = torch.empty((G, N), dtype=dt, device=dev)
+        db = x.new_empty(G, N)
         d.dbias = db.data_ptr()
-    space = _give_workspace(eng, d, 'psh_grouped_linear_grad_workspace', dev)
+    space = _give_workspace(eng, d, 'psh_grouped_linear_grad_workspace', x)
     eng._call('psh_grouped_linear_grad', C.byref(d))
     del keep, space
     return dx, dw, db
@@ -302,8 +302,8 @@ def _conv_desc(x, weight, bias, offsets, groups, state, silu, step):
 
 def _conv_forward(x, weight, bias, offsets, groups, state, silu):
     eng, d, keep, S, R, D, P, K, dt, dev = _conv_desc(x, weight, bias, offsets, groups, state, silu, False)
-    y = torch.empty((R, D), dtype=dt, device=dev)
-    last = torch.empty((S, D, K - 1), dtype=dt, device=dev)
+    y = x.new_empty(R, D)
+    last = x.new_empty(S, D, K - 1)
     d.y, d.last, d.stride_last = y.data_ptr(), last.data_ptr(), D*(K - 1)
     eng._call('psh_causal_conv', C.byref(d))
     del keep
@@ -319,13 +319,12 @@ def causal_conv_grad(dy, dlast, x, weight, bias, offsets, groups=None, state=Non
     if dlast is not None:
         dlast = _param('dlast', dlast, dt, dev, (S, D, K - 1))
         d.dlast = dlast.data_ptr()
-    W = wide_dtype(dt)
-    dx = torch.empty((R, D), dtype=dt, device=dev) if want[0] else None
-    dw = torch.empty((P, D, K), dtype=W, device=dev) if want[1] else None
-    db = torch.empty((P, D), dtype=W, device=dev) if want[2] else None
-    ds = torch.empty((S, D, K - 1), dtype=dt, device=dev) if want[3] else None
+    dx = x.new_empty(R, D) if want[0] else None
+    dw = weight.new_empty(P, D, K) if want[1] else None
+    db = weight.new_empty(P, D) if want[2] else None
+    ds = x.new_empty(S, D, K - 1) if want[3] else None
     d.dx, d.dweight, d.dbias, d.dstate = _ptr(dx), _ptr(dw), _ptr(db), _ptr(ds)
-    space = _give_workspace(eng, d, 'psh_causal_conv_grad_workspace', dev)
+    space = _give_workspace(eng, d, 'psh_causal_conv_grad_workspace', x)
     eng._call('psh_causal_conv_grad', C.byref(d))
     del keep, space
     return dx, dw, db, ds
@@ -372,7 +371,7 @@ def causal_conv_step(x, state, weight, bias, groups=None, silu: bool = True):
     eng, d, keep, S, R, D, P, K, dt, dev = _conv_desc(x, weight, bias, None, groups, state, silu, True)
     if S and K > 1 and keep[5] is not state:
         raise ValueErr(msg='state is updated in place: the values of each sequence have to be contiguous!')
-    y = torch.empty((R, D), dtype=dt, device=dev)
+    y = x.new_empty(R, D)
     d.y, d.last, d.stride_last = y.data_ptr(), state.data_ptr(), d.stride_state
     eng._call('psh_causal_conv', C.byref(d))
     del keep
@@ -411,14 +410,14 @@ def _scan_desc(u, delta, A, B, Cm, D, z, delta_bias, offsets, groups, state, ste
 
 def _scan_forward(u, delta, A, B, Cm, D, z, delta_bias, offsets, groups, state, keep_check):
     eng, d, keep, S, R, ch, P, N, dt, W, dev = _scan_desc(u, delta, A, B, Cm, D, z, delta_bias, offsets, groups, state, False)
-    y = torch.empty((R, ch), dtype=dt, device=dev)
-    last = torch.empty((S, ch, N), dtype=W, device=dev)
+    y = u.new_empty(R, ch)
+    last = A.new_empty(S, ch, N)
     d.y, d.last, d.stride_last = y.data_ptr(), last.data_ptr(), ch*N
     check = None
     if keep_check:
         check = _workspace(_size(eng, 'psh_selective_scan_check', d), dev)
         d.check = check.data_ptr()
-    space = _give_workspace(eng, d, 'psh_selective_scan_workspace', dev)
+    space = _give_workspace(eng, d, 'psh_selective_scan_workspace', u)
     eng._call('psh_selective_scan', C.byref(d))
     del keep, space
     return y, last, check
@@ -448,14 +447,18 @@ def _scan_grad(dy, dlast, check, u, delta, A, B, Cm, D, z, delta_bias, offsets, 
         raise ValueErr(msg='check must be the stored states that selective_scan_check returned for the same inputs!')
     d.check = check.data_ptr()
 
-    def out(k, there, shape, dtype):
-        return torch.empty(shape, dtype=dtype, device=dev) if want[k] and there else None
-    du, ddelta = out(0, True, (R, ch), dt), out(1, True, (R, ch), dt)
-    dA, dB, dC = out(2, True, (P, ch, N), W), out(3, True, (R, N), dt), out(4, True, (R, N), dt)
-    dD, dz = out(5, D is not None, (P, ch), W), out(6, z is not None, (R, ch), dt)
-    dbias, dstate = out(7, delta_bias is not None, (P, ch), W), out(8, state is not None, (S, ch, N), W)
+    rows, wide = u.new_empty, A.new_empty
+    du = rows(R, ch) if want[0] else None
+    ddelta = rows(R, ch) if want[1] else None
+    dA = wide(P, ch, N) if want[2] else None
+    dB = rows(R, N) if want[3] else None
+    dC = rows(R, N) if want[4] else None
+    dD = wide(P, ch) if want[5] and D is not None else None
+    dz = rows(R, ch) if want[6] and z is not None else None
+    dbias = wide(P, ch) if want[7] and delta_bias is not None else None
+    dstate = wide(S, ch, N) if want[8] and state is not None else None
     d.du, d.ddelta, d.dA, d.dB, d.dC, d.dD, d.dz, d.ddelta_bias, d.dstate = (_ptr(t) for t in (du, ddelta, dA, dB, dC, dD, dz, dbias, dstate))
-    space = _give_workspace(eng, d, 'psh_selective_scan_grad_workspace', dev)
+    space = _give_workspace(eng, d, 'psh_selective_scan_grad_workspace', u)
     eng._call('psh_selective_scan_grad', C.byref(d))
     del keep, space
     return du, ddelta, dA, dB, dC, dD, dz, dbias, dstate
@@ -510,7 +513,7 @@ def _scan_step(u, delta, state, A, B, Cm, D, z, delta_bias, groups):
     eng, d, keep, S, R, ch, P, N, dt, W, dev = _scan_desc(u, delta, A, B, Cm, D, z, delta_bias, None, groups, state, True)
     if S and keep[10] is not state:
         raise ValueErr(msg='state is updated in place: the values of each sequence have to be contiguous!')
-    y = torch.empty((R, ch), dtype=dt, device=dev)
+    y = u.new_empty(R, ch)
     d.y, d.last, d.stride_last = y.data_ptr(), state.data_ptr(), d.stride_state
     eng._call('psh_selective_scan', C.byref(d))
     del keep
