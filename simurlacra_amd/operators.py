@@ -17,8 +17,8 @@ sums run in fp32, and each result is rounded once.  Parameters and states of the
 float64 rows and float32 for the others.
 
 All calls run on the current stream of the tensors' GPU and are ordered like any other work on it.  They can be captured
-into graphs; for gradients inside a capture use the *_grad functions, which autograd's bookkeeping has no part in.  Without
-a GPU every call raises: there is no CPU fallback.
+into graphs; for gradients inside a capture use the *_grad functions, which autograd's bookkeeping has no part in (a call that autograd
+would differentiate is refused there).  Without a GPU every call raises: there is no CPU fallback.
 """
 import ctypes as C
 
@@ -142,6 +142,17 @@ def _first_derivative_only():
         raise ValueErr(msg='the policy operators have no second derivatives!')
 
 
+def _autograd(*tensors):
+    """ Whether a call of these tensors is to be differentiated.  A backward pass in a capture waits for the streams of every autograd graph
+    that its leaves are in, and where one of them lives outside the capture the process ends; so such a call is refused here. """
+    if not (torch.is_grad_enabled() and _any_requires_grad(*tensors)):
+        return False
+    if torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
+        raise ValueErr(msg='an operator cannot be differentiated by autograd while it is captured into a graph: call it under '
+                           'torch.no_grad(), and its *_grad function for the gradients!')
+    return True
+
+
 def _grad_tensor(t, like_dtype):
     """ An incoming gradient as the kernels take it. """
     return None if t is None else t.to(like_dtype).contiguous()
@@ -243,7 +254,7 @@ def grouped_linear(x, weight, bias, offsets, nonlin: str = None):
 
     x [R, K]; weight [G, N, K] and bias [G, N] (or None) of x's type, views into a matrix of whole parameter vectors
     included; nonlin None, 'tanh', 'relu' or 'sigmoid'.  Returns y [R, N]. """
-    if torch.is_grad_enabled() and _any_requires_grad(x, weight, bias):
+    if _autograd(x, weight, bias):
         return _GroupedLinear.apply(x, weight, bias, offsets, nonlin)
     return _linear_forward(x, weight, bias, offsets, nonlin)
 
@@ -356,7 +367,7 @@ def causal_conv(x, weight, bias, offsets, groups=None, state=None, silu: bool = 
     x [R, D]; weight [P, D, K] and bias [P, D] (or None) of policy p, whose sequences `groups` name; state [S, D, K - 1] the inputs
     before each sequence's first step, oldest first (None: zeros).  Returns y [R, D], with return_state also the state
     after each sequence's last step. """
-    if torch.is_grad_enabled() and _any_requires_grad(x, weight, bias, state):
+    if _autograd(x, weight, bias, state):
         y, last = _CausalConv.apply(x, weight, bias, state, offsets, groups, silu)
     else:
         y, last = _conv_forward(x, weight, bias, offsets, groups, state, silu)
@@ -493,7 +504,7 @@ def selective_scan(u, delta, A, B, C, D, z, delta_bias, offsets, groups=None, st
     before each sequence's first step (None: zeros).  D, z and delta_bias may be None.  Returns y [R, D], with return_state
     also the state after each sequence's last step. """
     args = (u, delta, A, B, C, D, z, delta_bias, state)
-    if torch.is_grad_enabled() and _any_requires_grad(*args):
+    if _autograd(*args):
         y, last = _SelectiveScan.apply(*args, offsets, groups)
     else:
         y, last, _ = _scan_forward(u, delta, A, B, C, D, z, delta_bias, offsets, groups, state, False)

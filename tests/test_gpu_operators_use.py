@@ -410,3 +410,24 @@ def test_gradients_against_differences(ops):
     names = ('u', 'delta', 'A', 'B', 'C', 'D', 'z', 'delta_bias', 'state')
     args = [v[n].detach().clone().requires_grad_() for n in names]
     assert torch.autograd.gradcheck(lambda *t: ops.selective_scan(*t[:8], off, grp, t[8], return_state=True), args, eps=1e-6, atol=1e-6, rtol=1e-6)
+
+
+def test_autograd_in_a_capture_is_refused(ops):
+    gen = torch.Generator().manual_seed(14)
+    x, w, off = rnd(gen, 50, 8), rnd(gen, 2, 6, 8).requires_grad_(), offs([20, 30])
+    cw = rnd(gen, 1, 8, 4).requires_grad_()
+    v, soff, _ = scan_inputs(gen, ops, torch.float64, [40, 10], 8, 4, None, tail=0)
+    A = v['A'].clone().requires_grad_()
+    with torch.no_grad():
+        want = ops.grouped_linear(x, w, None, off)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        for call in (lambda: ops.grouped_linear(x, w, None, off), lambda: ops.causal_conv(x, cw, None, off),
+                     lambda: ops.selective_scan(v['u'], v['delta'], A, v['B'], v['C'], None, None, None, soff)):
+            with pytest.raises(ValueErr, match='captured'):
+                call()
+        with torch.no_grad():
+            y = ops.grouped_linear(x, w, None, off)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, want)
