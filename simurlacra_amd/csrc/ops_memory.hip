@@ -499,7 +499,7 @@ PSH_OP double halves16(double a, double b) {
     return __hiloint2double((int)h[0], (int)l[0]) + __hiloint2double((int)h[1], (int)l[1]);
 }
 
-// The compiler takes x to be computed here.
+// The compiler takes x to be computed here.  (Not for what a DPP instruction reads next: the wait states it needs are not counted across this.)
 PSH_OP void fixed(float& x) { asm volatile("" : "+v"(x)); }
 PSH_OP void fixed(double& x) { asm volatile("" : "+v"(x)); }
 
