@@ -137,6 +137,11 @@ def _give_workspace(eng, desc, name, like):
     return space
 
 
+def _advanced(state):
+    """ The kernel has written the state past torch, whose count of its changes tells a backward pass that saved it. """
+    torch.autograd.graph.increment_version(state)
+
+
 def _first_derivative_only():
     if torch.is_grad_enabled():   # as it is in a backward pass with create_graph=True
         raise ValueErr(msg='the policy operators have no second derivatives!')
@@ -385,6 +390,7 @@ def causal_conv_step(x, state, weight, bias, groups=None, silu: bool = True):
     y = x.new_empty(R, D)
     d.y, d.last, d.stride_last = y.data_ptr(), state.data_ptr(), d.stride_state
     eng._call('psh_causal_conv', C.byref(d))
+    _advanced(state)
     del keep
     return y
 
@@ -527,5 +533,6 @@ def _scan_step(u, delta, state, A, B, Cm, D, z, delta_bias, groups):
     y = u.new_empty(R, ch)
     d.y, d.last, d.stride_last = y.data_ptr(), state.data_ptr(), d.stride_state
     eng._call('psh_selective_scan', C.byref(d))
+    _advanced(state)
     del keep
     return y
