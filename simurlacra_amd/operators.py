@@ -23,6 +23,7 @@ would differentiate is refused there).  Without a GPU every call raises: there i
 import ctypes as C
 
 import torch
+import torch.autograd.forward_ad as _forward
 
 from . import _abi as abi
 from .engine import get_engine
@@ -104,6 +105,15 @@ def _any_requires_grad(*tensors):
         if isinstance(t, _Tensor) and t.requires_grad:
             return True
     return False
+
+
+def _seen_by_torch(*tensors):
+    """ The kernels run past torch, which sees the tensors that come out and nothing of how they came about.  What it can only do with
+    operations that it sees is refused: a tangent of forward differentiation would be dropped, and the derivative read as zero. """
+    if _forward._current_level >= 0:
+        for t in tensors:
+            if isinstance(t, _Tensor) and _forward.unpack_dual(t).tangent is not None:
+                raise ValueErr(msg='the policy operators have no forward derivatives!')
 
 
 def _no_grad_args(what, *tensors):
@@ -213,6 +223,7 @@ def grouped_linear_grad(dy, y, x, weight, offsets, nonlin=None, want=(True, True
     """ The gradients (dx, dweight, dbias) of grouped_linear for the gradient dy of its result y; None where `want` is false.
     y is only read with a nonlinearity, whose slope is taken from the value: of bfloat16 results, whose rounding is felt where a
     nonlinearity is flat, the values may be given in float32. """
+    _seen_by_torch(dy, y, x, weight)
     eng, d, keep, R, K, G, N, dt, dev = _linear_desc(x, weight, None, offsets, nonlin)
     dy, d.ld_dy = _rows_arg('dy', dy, dt, dev, R, N)
     d.dy = dy.data_ptr()
@@ -259,6 +270,7 @@ def grouped_linear(x, weight, bias, offsets, nonlin: str = None):
 
     x [R, K]; weight [G, N, K] and bias [G, N] (or None) of x's type, views into a matrix of whole parameter vectors
     included; nonlin None, 'tanh', 'relu' or 'sigmoid'.  Returns y [R, N]. """
+    _seen_by_torch(x, weight, bias)
     if _autograd(x, weight, bias):
         return _GroupedLinear.apply(x, weight, bias, offsets, nonlin)
     return _linear_forward(x, weight, bias, offsets, nonlin)
@@ -329,6 +341,7 @@ def _conv_forward(x, weight, bias, offsets, groups, state, silu):
 def causal_conv_grad(dy, dlast, x, weight, bias, offsets, groups=None, state=None, silu: bool = True, want=(True,)*4):
     """ The gradients (dx, dweight, dbias, dstate) of causal_conv for those of its results (dlast may be None); None
     where `want` is false. """
+    _seen_by_torch(dy, dlast, x, weight, bias, state)
     eng, d, keep, S, R, D, P, K, dt, dev = _conv_desc(x, weight, bias, offsets, groups, state, silu, False)
     dy, d.ld_dy = _rows_arg('dy', dy, dt, dev, R, D)
     d.dy = dy.data_ptr()
@@ -372,6 +385,7 @@ def causal_conv(x, weight, bias, offsets, groups=None, state=None, silu: bool = 
     x [R, D]; weight [P, D, K] and bias [P, D] (or None) of policy p, whose sequences `groups` name; state [S, D, K - 1] the inputs
     before each sequence's first step, oldest first (None: zeros).  Returns y [R, D], with return_state also the state
     after each sequence's last step. """
+    _seen_by_torch(x, weight, bias, state)
     if _autograd(x, weight, bias, state):
         y, last = _CausalConv.apply(x, weight, bias, state, offsets, groups, silu)
     else:
@@ -381,6 +395,7 @@ def causal_conv(x, weight, bias, offsets, groups=None, state=None, silu: bool = 
 
 def causal_conv_step(x, state, weight, bias, groups=None, silu: bool = True):
     """ causal_conv for one step of every sequence: x [S, D]; state [S, D, K - 1] is updated in place.  Returns y [S, D]. """
+    _seen_by_torch(x, state, weight, bias)
     _no_grad_args('causal_conv_step', x, state, weight, bias)
     if state is None:
         raise TypeErr(given=state, given_name='state', expected_type=_Tensor)
@@ -442,6 +457,7 @@ def _scan_forward(u, delta, A, B, Cm, D, z, delta_bias, offsets, groups, state, 
 
 def selective_scan_check(u, delta, A, B, C, D, z, delta_bias, offsets, groups=None, state=None):
     """ selective_scan for a gradient taken with selective_scan_grad: (y, last state, stored states). """
+    _seen_by_torch(u, delta, A, B, C, D, z, delta_bias, state)
     return _scan_forward(u, delta, A, B, C, D, z, delta_bias, offsets, groups, state, True)
 
 
@@ -453,6 +469,7 @@ def selective_scan_grad(dy, dlast, check, u, delta, A, B, C, D, z, delta_bias, o
 
 
 def _scan_grad(dy, dlast, check, u, delta, A, B, Cm, D, z, delta_bias, offsets, groups, state, want):
+    _seen_by_torch(dy, dlast, u, delta, A, B, Cm, D, z, delta_bias, state)
     eng, d, keep, S, R, ch, P, N, dt, W, dev = _scan_desc(u, delta, A, B, Cm, D, z, delta_bias, offsets, groups, state, False)
     dy, d.ld_dy = _rows_arg('dy', dy, dt, dev, R, ch)
     d.dy = dy.data_ptr()
@@ -510,6 +527,7 @@ def selective_scan(u, delta, A, B, C, D, z, delta_bias, offsets, groups=None, st
     before each sequence's first step (None: zeros).  D, z and delta_bias may be None.  Returns y [R, D], with return_state
     also the state after each sequence's last step. """
     args = (u, delta, A, B, C, D, z, delta_bias, state)
+    _seen_by_torch(*args)
     if _autograd(*args):
         y, last = _SelectiveScan.apply(*args, offsets, groups)
     else:
@@ -524,6 +542,7 @@ def selective_scan_step(u, delta, state, A, B, C, D, z, delta_bias, groups=None)
 
 
 def _scan_step(u, delta, state, A, B, Cm, D, z, delta_bias, groups):
+    _seen_by_torch(u, delta, state, A, B, Cm, D, z, delta_bias)
     _no_grad_args('selective_scan_step', u, delta, state, A, B, Cm, D, z, delta_bias)
     if state is None:
         raise TypeErr(given=state, given_name='state', expected_type=_Tensor)

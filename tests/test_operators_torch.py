@@ -4,9 +4,11 @@ nothing: whatever a call returns is empty memory, and the tests are about what i
 """
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
 from simurlacra_amd import operators as ops
 from simurlacra_amd.engine import load_library
+from simurlacra_amd.utils.exceptions import ValueErr
 
 
 class _NoEngine:
@@ -80,3 +82,76 @@ def test_a_refused_step_changes_nothing(engine):
     with pytest.raises(ValueError):
         ops.causal_conv_step(x, state, torch.randn(1, 4, 9), b)
     assert state._version == before and not engine.calls
+
+
+# -------------------------------------------------------------------------------------------------- forward derivatives
+def entry_points():
+    """ Every call of the module with its tensors by name: [(name, function of the tensors, tensors)] """
+    off = torch.arange(4, dtype=torch.int32)
+    x, state, w, b = conv_args()
+    v, h = scan_args(), torch.randn(3, 4, 2)
+    dy, dlast = torch.randn(3, 4), torch.randn(3, 4, 2)
+    lin = dict(x=torch.randn(3, 5), weight=torch.randn(3, 4, 5), bias=torch.randn(3, 4))
+    check = torch.zeros(load_library().psh_selective_scan_check(ops.C.byref(
+        ops.abi.PshScanDesc(ops.abi.DTYPE_F32, 0, 1, 3, 3, 4, 2))), dtype=torch.uint8)
+    return [
+        ('grouped_linear', lambda **t: ops.grouped_linear(**t, offsets=off, nonlin='tanh'), lin),
+        ('grouped_linear_grad', lambda **t: ops.grouped_linear_grad(**t, offsets=off, nonlin='tanh'),
+         dict(dy=dy, y=torch.randn(3, 4), x=lin['x'], weight=lin['weight'])),
+        ('causal_conv', lambda **t: ops.causal_conv(**t, offsets=off), dict(x=x, weight=w, bias=b, state=state)),
+        ('causal_conv_grad', lambda **t: ops.causal_conv_grad(**t, offsets=off),
+         dict(dy=dy, dlast=state.clone(), x=x, weight=w, bias=b, state=state)),
+        ('causal_conv_step', ops.causal_conv_step, dict(x=x, state=state, weight=w, bias=b)),
+        ('selective_scan', lambda **t: ops.selective_scan(**t, offsets=off), dict(v, state=h)),
+        ('selective_scan_check', lambda **t: ops.selective_scan_check(**t, offsets=off), dict(v, state=h)),
+        ('selective_scan_grad', lambda **t: ops.selective_scan_grad(check=check, offsets=off, **t), dict(v, state=h, dy=dy, dlast=dlast)),
+        ('selective_scan_step', ops.selective_scan_step, dict(v, state=h)),
+    ]
+
+
+NAMES = ['grouped_linear', 'grouped_linear_grad', 'causal_conv', 'causal_conv_grad', 'causal_conv_step', 'selective_scan',
+         'selective_scan_check', 'selective_scan_grad', 'selective_scan_step']
+
+
+def test_the_entry_points_run_here(engine):
+    for name, f, tensors in entry_points():
+        f(**tensors)
+    assert [n for n, _, _ in entry_points()] == NAMES and len(engine.calls) == len(NAMES)
+
+
+@pytest.mark.parametrize('k', range(len(NAMES)), ids=NAMES)
+def test_forward_derivatives_are_refused_and_not_zero(engine, k):
+    """ A tangent on any of the tensors; without one, calls inside a dual level are calls as usual. """
+    name, f, tensors = entry_points()[k]
+    for which in tensors:
+        with fwd.dual_level():
+            dual = fwd.make_dual(tensors[which], torch.ones_like(tensors[which]))
+            for mode in (torch.no_grad, torch.enable_grad):
+                with mode(), pytest.raises(ValueErr, match='forward'):
+                    f(**dict(tensors, **{which: dual}))
+    assert not engine.calls
+    with fwd.dual_level():
+        f(**tensors)
+    assert len(engine.calls) == 1
+
+
+def test_forward_derivatives_beside_those_that_are_differentiated_are_refused(engine):
+    """ also where another tensor asks for a gradient, so that the call is autograd's """
+    name, f, tensors = entry_points()[0]
+    with fwd.dual_level():
+        dual = fwd.make_dual(tensors['x'], torch.ones_like(tensors['x']))
+        with pytest.raises(ValueErr, match='forward'):
+            f(x=dual, weight=tensors['weight'].clone().requires_grad_(), bias=tensors['bias'])
+    with pytest.raises(Exception):
+        torch.func.jvp(lambda x: f(**dict(tensors, x=x)), (tensors['x'],), (torch.ones_like(tensors['x']),))
+    assert not engine.calls
+
+
+@pytest.mark.parametrize('k', [0, 2, 5], ids=[NAMES[k] for k in (0, 2, 5)])
+def test_forward_derivatives_of_backward_passes_are_refused(engine, k):
+    name, f, tensors = entry_points()[k]
+    first = next(iter(tensors))
+    y = f(**dict(tensors, **{first: tensors[first].requires_grad_()}))
+    with fwd.dual_level(), pytest.raises(ValueErr, match='forward'):
+        torch.autograd.grad(y, tensors[first], fwd.make_dual(torch.ones_like(y), torch.ones_like(y)))
+    assert len(engine.calls) == 1
