@@ -107,9 +107,16 @@ def _any_requires_grad(*tensors):
     return False
 
 
+_is_tracing, _modes, _dispatched_with = torch._C._is_tracing, torch._C._len_torch_dispatch_stack, torch._C._dispatch_tls_is_dispatch_key_included
+_PRE_DISPATCH, _PROXY = torch._C.DispatchKey.PreDispatch, torch._C._TorchDispatchModeKey.PROXY
+
+
 def _seen_by_torch(*tensors):
     """ The kernels run past torch, which sees the tensors that come out and nothing of how they came about.  What it can only do with
-    operations that it sees is refused: a tangent of forward differentiation would be dropped, and the derivative read as zero. """
+    operations that it sees is refused: a recorded call would be empty memory whenever it is played back, and a tangent of forward
+    differentiation would be dropped and the derivative read as zero. """
+    if _is_tracing() or _dispatched_with(_PRE_DISPATCH) or (_modes() and torch._C._get_dispatch_mode(_PROXY) is not None):
+        raise ValueErr(msg='the policy operators cannot be recorded (torch.jit.trace, make_fx): torch does not see what they do!')
     if _forward._current_level >= 0:
         for t in tensors:
             if isinstance(t, _Tensor) and _forward.unpack_dual(t).tangent is not None:

@@ -5,6 +5,9 @@ nothing: whatever a call returns is empty memory, and the tests are about what i
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
+from torch.fx.experimental.proxy_tensor import make_fx
+from torch.utils._python_dispatch import TorchDispatchMode
+from torch.utils.flop_counter import FlopCounterMode
 
 from simurlacra_amd import operators as ops
 from simurlacra_amd.engine import load_library
@@ -155,3 +158,39 @@ def test_forward_derivatives_of_backward_passes_are_refused(engine, k):
     with fwd.dual_level(), pytest.raises(ValueErr, match='forward'):
         torch.autograd.grad(y, tensors[first], fwd.make_dual(torch.ones_like(y), torch.ones_like(y)))
     assert len(engine.calls) == 1
+
+
+# -------------------------------------------------------------------------------------------------------------- traces
+TRACERS = {'jit.trace': lambda f, t: torch.jit.trace(f, t, check_trace=False),
+           'make_fx': lambda f, t: make_fx(f)(*t),
+           'make_fx before the dispatcher': lambda f, t: make_fx(f, pre_dispatch=True)(*t)}
+
+
+@pytest.mark.parametrize('tracer', TRACERS)
+@pytest.mark.parametrize('k', range(len(NAMES)), ids=NAMES)
+def test_traces_are_refused(engine, k, tracer):
+    """ A recorded call would be the allocation of its results and nothing else. """
+    name, f, tensors = entry_points()[k]
+    with pytest.raises(ValueErr, match='recorded'):
+        TRACERS[tracer](lambda *t: f(**dict(zip(tensors, t))), tuple(tensors.values()))
+    assert not engine.calls
+    f(**tensors)
+    assert len(engine.calls) == 1
+
+
+def test_traces_of_differentiated_calls_are_refused(engine):
+    name, f, tensors = entry_points()[0]
+    with pytest.raises(ValueErr, match='recorded'):
+        torch.jit.trace(lambda x: f(**dict(tensors, x=x)), tensors['x'].clone().requires_grad_(), check_trace=False)
+    assert not engine.calls
+
+
+def test_modes_that_only_watch_are_no_traces(engine):
+    class Watch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+    for mode in (Watch(), FlopCounterMode(display=False)):
+        for name, f, tensors in entry_points():
+            with mode:
+                f(**tensors)
+    assert len(engine.calls) == 2*len(NAMES)
