@@ -130,7 +130,13 @@ def _no_grad_args(what, *tensors):
 
 
 def _ptr(t):
-    return None if t is None else t.data_ptr()
+    """ The address of a tensor that need not be there, of which a null pointer tells the library (an empty tensor has none either). """
+    if t is None:
+        return None
+    at = t.data_ptr()
+    if at == 0 and t.numel():   # it stands for a tensor in a program that is being transformed
+        raise ValueErr(msg=f'the policy operators need tensors that lie in memory, but {type(t).__name__} of shape {list(t.shape)} has no memory!')
+    return at
 
 
 def _size(eng, name, desc):
@@ -204,7 +210,7 @@ def _linear_desc(x, weight, bias, offsets, nonlin):
         if step != 1 and N > 1:
             bias = bias.contiguous()
             stride_b = N
-        b = bias.data_ptr()
+        b = _ptr(bias)
     d = abi.PshLinearDesc(_DTYPES[dt], _NONLINS[nonlin], G, R, K, N, offsets.data_ptr(), x.data_ptr(), weight.data_ptr(), b, None, None, ld_x,
                           ld_w if N > 1 else K, stride_w if G > 1 else 0, stride_b if G > 1 else 0)
     d.stream = eng._stream()
@@ -220,7 +226,7 @@ def _linear_forward(x, weight, bias, offsets, nonlin, wide=False):
     value = y
     if wide and dt == torch.bfloat16 and nonlin in ('tanh', 'sigmoid'):
         value = torch.empty((R, N), dtype=torch.float32, device=dev)
-        d.y_wide = value.data_ptr()
+        d.y_wide = _ptr(value)
     eng._call('psh_grouped_linear', C.byref(d))
     del keep
     return (y, value) if wide else y
@@ -238,19 +244,19 @@ def grouped_linear_grad(dy, y, x, weight, offsets, nonlin=None, want=(True, True
         wide = dt == torch.bfloat16 and isinstance(y, _Tensor) and y.dtype == torch.float32
         y = _param('y', y, torch.float32 if wide else dt, dev, (R, N))
         if wide:
-            d.y_wide = y.data_ptr()
+            d.y_wide = _ptr(y)
         else:
-            d.y = y.data_ptr()
+            d.y = _ptr(y)
     dx = dw = db = None
     if want[0]:
         dx = x.new_empty(R, K)
-        d.dx = dx.data_ptr()
+        d.dx = _ptr(dx)
     if want[1]:
         dw = x.new_empty(G, N, K)
-        d.dweight = dw.data_ptr()
+        d.dweight = _ptr(dw)
     if want[2]:
         db = x.new_empty(G, N)
-        d.dbias = db.data_ptr()
+        d.dbias = _ptr(db)
     space = _give_workspace(eng, d, 'psh_grouped_linear_grad_workspace', x)
     eng._call('psh_grouped_linear_grad', C.byref(d))
     del keep, space
@@ -330,7 +336,7 @@ def _conv_desc(x, weight, bias, offsets, groups, state, silu, step):
     d.ld_x = ld_x
     if state is not None:
         state, d.stride_state = _state_arg('state', state, dt, dev, (S, D, K - 1))
-        d.state = state.data_ptr()
+        d.state = _ptr(state)
     d.stream = eng._stream()
     return eng, d, (x, weight, bias, offsets, groups, state), S, R, D, P, K, dt, dev
 
@@ -339,7 +345,7 @@ def _conv_forward(x, weight, bias, offsets, groups, state, silu):
     eng, d, keep, S, R, D, P, K, dt, dev = _conv_desc(x, weight, bias, offsets, groups, state, silu, False)
     y = x.new_empty(R, D)
     last = x.new_empty(S, D, K - 1)
-    d.y, d.last, d.stride_last = y.data_ptr(), last.data_ptr(), D*(K - 1)
+    d.y, d.last, d.stride_last = y.data_ptr(), _ptr(last), D*(K - 1)
     eng._call('psh_causal_conv', C.byref(d))
     del keep
     return y, last
@@ -354,7 +360,7 @@ def causal_conv_grad(dy, dlast, x, weight, bias, offsets, groups=None, state=Non
     d.dy = dy.data_ptr()
     if dlast is not None:
         dlast = _param('dlast', dlast, dt, dev, (S, D, K - 1))
-        d.dlast = dlast.data_ptr()
+        d.dlast = _ptr(dlast)
     dx = x.new_empty(R, D) if want[0] else None
     dw = weight.new_empty(P, D, K) if want[1] else None
     db = weight.new_empty(P, D) if want[2] else None
@@ -451,11 +457,11 @@ def _scan_forward(u, delta, A, B, Cm, D, z, delta_bias, offsets, groups, state, 
     eng, d, keep, S, R, ch, P, N, dt, W, dev = _scan_desc(u, delta, A, B, Cm, D, z, delta_bias, offsets, groups, state, False)
     y = u.new_empty(R, ch)
     last = A.new_empty(S, ch, N)
-    d.y, d.last, d.stride_last = y.data_ptr(), last.data_ptr(), ch*N
+    d.y, d.last, d.stride_last = y.data_ptr(), _ptr(last), ch*N
     check = None
     if keep_check:
         check = _workspace(_size(eng, 'psh_selective_scan_check', d), dev)
-        d.check = check.data_ptr()
+        d.check = _ptr(check)
     space = _give_workspace(eng, d, 'psh_selective_scan_workspace', u)
     eng._call('psh_selective_scan', C.byref(d))
     del keep, space
@@ -482,7 +488,7 @@ def _scan_grad(dy, dlast, check, u, delta, A, B, Cm, D, z, delta_bias, offsets, 
     d.dy = dy.data_ptr()
     if dlast is not None:
         dlast = _param('dlast', dlast, W, dev, (S, ch, N))
-        d.dlast = dlast.data_ptr()
+        d.dlast = _ptr(dlast)
     need = _size(eng, 'psh_selective_scan_check', d)
     if check is None or check.dtype != torch.uint8 or check.device != dev or not check.is_contiguous() or check.numel() != need:
         raise ValueErr(msg='check must be the stored states that selective_scan_check returned for the same inputs!')

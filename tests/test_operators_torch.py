@@ -5,6 +5,7 @@ nothing: whatever a call returns is empty memory, and the tests are about what i
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
+from torch._subclasses.fake_tensor import FakeTensorMode
 from torch.fx.experimental.proxy_tensor import make_fx
 from torch.utils._python_dispatch import TorchDispatchMode
 from torch.utils.flop_counter import FlopCounterMode
@@ -194,3 +195,18 @@ def test_modes_that_only_watch_are_no_traces(engine):
             with mode:
                 f(**tensors)
     assert len(engine.calls) == 2*len(NAMES)
+
+
+@pytest.mark.parametrize('name,which', [('grouped_linear', 'bias'), ('causal_conv', 'bias'), ('causal_conv', 'state'), ('causal_conv_grad', 'dlast'),
+                                        ('selective_scan', 'D'), ('selective_scan', 'z'), ('selective_scan', 'delta_bias'), ('selective_scan', 'state'),
+                                        ('selective_scan_grad', 'dlast')])
+def test_a_tensor_without_memory_is_not_an_absent_one(engine, name, which):
+    """ What stands for a tensor while a program is being transformed has no address, which the kernels would take for 'not given'. """
+    f, tensors = next((f, t) for n, f, t in entry_points() if n == name)
+    mode = FakeTensorMode()
+    fake = mode.from_tensor(tensors[which])
+    with pytest.raises(ValueErr, match='no memory'):
+        f(**dict(tensors, **{which: fake}))
+    with pytest.raises(ValueErr, match='no memory'):
+        torch.func.functionalize(lambda t: f(**dict(tensors, **{which: t})))(tensors[which])
+    assert not engine.calls
