@@ -42,6 +42,7 @@ def wide_dtype(dtype: torch.dtype) -> torch.dtype:
 # (These run before every call, and a small call takes a few microseconds on the GPU: each check is one expression on the
 # common path, and what is wrong is only worked out once something is.)
 _Tensor = torch.Tensor
+_MOST = 2**31 - 1    # what the descriptors' sizes hold (ctypes would keep the low bits of more)
 
 
 def _refuse(name, t, dtype, device, shape):
@@ -55,6 +56,10 @@ def _refuse(name, t, dtype, device, shape):
     if device is not None and t.device != device:
         raise ValueErr(msg=f'{name} must be on {device}, but is on {t.device}!')
     raise ShapeErr(msg=f'{name} must have the shape [{", ".join("any" if n is None else str(n) for n in shape)}], but has {list(t.shape)}!')
+
+
+def _too_large(name, n):
+    raise ValueErr(msg=f'{name} has a size of {n}, more than the 2^31 - 1 that the operators can count!')
 
 
 def _rows_arg(name, t, dtype, device, rows, cols):
@@ -73,6 +78,8 @@ def _first_rows_arg(name, t):
     if not isinstance(t, _Tensor) or t.dtype not in _DTYPES or not t.is_cuda or t.dim() != 2:
         _refuse(name, t, None, None, (None, None))
     rows, cols = t.shape
+    if rows > _MOST or cols > _MOST:
+        _too_large(name, max(rows, cols))
     ld, step = t.stride()
     if (step != 1 and cols > 1) or (ld < cols and rows > 1):
         t = t.contiguous()
@@ -97,6 +104,8 @@ def _offsets(name, t, device):
         raise ValueErr(msg=f'{name} must be on {device}, but is on {t.device}!')
     if t.dim() != 1 or t.shape[0] < 2:
         raise ShapeErr(msg=f'{name} must have one entry more than there are parts (at least two), but has the shape {list(t.shape)}!')
+    if t.shape[0] > _MOST:
+        _too_large(name, t.shape[0])
     return t.contiguous()
 
 
@@ -198,6 +207,8 @@ def _linear_desc(x, weight, bias, offsets, nonlin):
     groups, N, cols = weight.shape
     if groups != G or cols != K or N < 1 or K < 1:
         raise ShapeErr(msg=f'weight must have the shape [{G}, outputs, {K}] with at least one input and output, but has {list(weight.shape)}!')
+    if N > _MOST:
+        _too_large('weight', N)
     stride_w, ld_w, step = weight.stride()
     if (step != 1 and K > 1) or (ld_w < K and N > 1):
         weight = weight.contiguous()
@@ -326,6 +337,8 @@ def _conv_desc(x, weight, bias, offsets, groups, state, silu, step):
     P, K = weight.shape[0], weight.shape[2]
     if not 1 <= K <= abi.PSH_MAX_TAPS or P < 1 or D < 1:
         raise ValueErr(msg=f'causal_conv takes 1 to {abi.PSH_MAX_TAPS} taps and at least one policy and channel, but weight is {list(weight.shape)}!')
+    if P > _MOST:
+        _too_large('weight', P)
     weight = _param('weight', weight, W, dev, (P, D, K))
     bias = None if bias is None else _param('bias', bias, W, dev, (P, D))
     groups = _policies(groups, dev, P)
@@ -432,6 +445,8 @@ def _scan_desc(u, delta, A, B, Cm, D, z, delta_bias, offsets, groups, state, ste
     P, _, N = A.shape
     if not 1 <= N <= abi.PSH_MAX_MEM_STATES or P < 1 or ch < 1:
         raise ValueErr(msg=f'selective_scan takes 1 to {abi.PSH_MAX_MEM_STATES} states and at least one policy and channel, but A is {list(A.shape)}!')
+    if P > _MOST:
+        _too_large('A', P)
     delta, ld_delta = _rows_arg('delta', delta, dt, dev, R, ch)
     B, ld_B = _rows_arg('B', B, dt, dev, R, N)
     Cm, ld_C = _rows_arg('C', Cm, dt, dev, R, N)

@@ -210,3 +210,40 @@ def test_a_tensor_without_memory_is_not_an_absent_one(engine, name, which):
     with pytest.raises(ValueErr, match='no memory'):
         torch.func.functionalize(lambda t: f(**dict(tensors, **{which: t})))(tensors[which])
     assert not engine.calls
+
+
+# --------------------------------------------------------------------------------------------------------------- sizes
+BIG = 2**32 + 5      # of which 32 bits keep 5
+
+
+def test_sizes_that_32_bits_do_not_hold_are_refused(engine):
+    """ The descriptors hold sizes in 32 bits.  (Nothing here is ever written, so the memory is never there.) """
+    off = torch.arange(2, dtype=torch.int32)
+    bf, f = torch.bfloat16, torch.float32
+    long, short = torch.empty(BIG, 1, dtype=bf), torch.empty(3, 1, dtype=bf)
+    many = torch.zeros(1, dtype=torch.int32).expand(BIG + 1)
+    one = torch.zeros(1, 1, 1)
+    rows = dict(delta=long, B=long, C=long, D=None, z=None, delta_bias=None)
+    calls = {
+        'rows': lambda: ops.grouped_linear(long, one.to(bf), None, off),
+        'inputs': lambda: ops.grouped_linear(long.view(1, BIG), long.view(1, 1, BIG), None, off),
+        'outputs': lambda: ops.grouped_linear(short, long.view(1, BIG, 1), None, off),
+        'groups': lambda: ops.grouped_linear(short, one.to(bf).expand(BIG, 1, 1), None, many),
+        'rows of a gradient': lambda: ops.grouped_linear_grad(long, None, long, one.to(bf), off),
+        'rows of a convolution': lambda: ops.causal_conv(long, one, None, off),
+        'channels': lambda: ops.causal_conv(long.view(1, BIG), torch.empty(1, 1, 1).expand(1, BIG, 1), None, off),
+        'sequences': lambda: ops.causal_conv(short, one, None, many),
+        'policies': lambda: ops.causal_conv(short, one.expand(BIG, 1, 1), None, off, groups=many),
+        'taps': lambda: ops.causal_conv(short, one.expand(1, 1, BIG), None, off),
+        'sequences of a step': lambda: ops.causal_conv_step(long, torch.empty(BIG, 1, 0, dtype=bf), one, None),
+        'rows of a recurrence': lambda: ops.selective_scan(long, A=one, offsets=off, **rows),
+        'sequences of a recurrence': lambda: ops.selective_scan(short, A=one, offsets=many, **dict(rows, delta=short, B=short, C=short)),
+        'policies of a recurrence': lambda: ops.selective_scan(short, A=one.expand(BIG, 1, 1), offsets=off, groups=many,
+                                                               **dict(rows, delta=short, B=short, C=short)),
+        'sequences of its step': lambda: ops.selective_scan_step(long, state=torch.empty(1, 1, 1).expand(BIG, 1, 1), A=one, **rows),
+    }
+    for what, call in calls.items():
+        with pytest.raises(ValueErr):
+            call()
+            pytest.fail(what)
+        assert not engine.calls, what
