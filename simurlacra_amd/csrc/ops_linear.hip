@@ -198,8 +198,8 @@ template <int N, int THREADS, bool TR> struct Direct {
             }
             // (by hand, because the compiler would wait for a builtin's load before the next read of any part of LDS; the
             // waits are in front of the barriers)
-            // One wait state has to lie between a write of m0 and a load to LDS.  The compiler keeps nothing in m0, it writes it where it reads it.
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds + k * WAVES * 1024), "v"(g) : "memory");
+            // One wait state has to lie between a write of m0 and a load to LDS.
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds + k * WAVES * 1024), "v"(g) : "memory", "m0");
         }
     };
     // the last, partial tile of c through registers, zero where there is none
