@@ -199,7 +199,12 @@ template <int N, int THREADS, bool TR> struct Direct {
             // (by hand, because the compiler would wait for a builtin's load before the next read of any part of LDS; the
             // waits are in front of the barriers)
             // One wait state has to lie between a write of m0 and a load to LDS.
+            // (m0 is a reserved register, which the compiler warns of on a clobber list; it keeps nothing there across the statement, but it is
+            // told of the write, so that it does not take a value of its own in front of the statement for the one behind it)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
             asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds + k * WAVES * 1024), "v"(g) : "memory", "m0");
+#pragma clang diagnostic pop
         }
     };
     // the last, partial tile of c through registers, zero where there is none
