@@ -763,7 +763,7 @@ template <class T, int V> __global__ __launch_bounds__(256) void k_join(const Gr
     for (int g = blockIdx.y; g < a.parts.n; g += gridDim.y) {
         const int begin = a.parts.at(g), end = a.parts.at(g + 1);
         if (end - begin <= a.parts.L) continue;
-        const int pieces = (int)(((long)end - begin + a.parts.L - 1) / a.parts.L), first = a.parts.first_slot(g);
+        const int pieces = piece_count(begin, end, a.parts.L), first = a.parts.first_slot(g);
         const long threads = (long)gridDim.x * 256, me = (long)blockIdx.x * 256 + threadIdx.x;
         for (long e = me * V; e < nw; e += threads * V) {
             const W* const src = a.part_w + (long)first * nw + e;

@@ -8,17 +8,7 @@
 
 namespace {
 
-// which policy's parameters a sequence uses: the part of the sequences it lies in (the last part ends with the last
-// sequence, whatever groups[P] says)
-struct Policies {
-    const int* groups;
-    int n, n_seqs;
-    PSH_OP int at(int p) const {
-        if (p <= 0) return 0;
-        if (p >= n) return n_seqs;
-        const int o = groups[p];
-        return o < 0 ? 0 : (o > n_seqs ? n_seqs : o);
-    }
+struct Policies : Shares {
     PSH_OP int of(int seq) const { return n == 1 || !groups ? 0 : wave_search(n - 1, seq, [&](int p) { return at(p); }); }
 };
 
@@ -324,25 +314,18 @@ template <class T, int V, int K> __global__ __launch_bounds__(256) void k_conv_g
 // ============================================================================== sums over the pieces of a policy
 // out[p, m] = sum of part[slot, m] over the slots of policy p's sequences, in two passes of about the square root of their
 // number, in the order of the slots: 4 to 9 us each, the time of a few dependent loads.  `slot_of(p)`: the first slot of policy p.
-template <class W> struct JoinArgs {
-    Parts parts;
-    Policies pol;
+template <class W> struct JoinArgs : PolicySlots {   // (seg = 0: few enough slots for one pass over `part`)
     const W* part; W* mid;
     W *out0, *out1, *out2;    // columns [0, n0) -> out0, then n1 -> out1, then n2 -> out2 (NULL: not wanted)
     long n0, n1, n2, split;   // split: column layout [.., split + 1] with the last of each row going to out1 (0: plain)
-    int seg;                  // 0: few enough slots for one pass over `part`
-    PSH_OP int slot_of(int p) const { return p >= pol.n ? parts.first_slot(parts.n) : parts.first_slot(pol.at(p)); }
-    PSH_OP int seg_of(int p) const { return slot_of(p) / seg + p; }
 };
 template <class W> __global__ __launch_bounds__(256) void k_join_mid(const JoinArgs<W> a) {
     const int seg = blockIdx.x;
     const int p = a.pol.n == 1 ? 0 : wave_search(a.pol.n - 1, seg, [&](int i) { return a.seg_of(i); });
     const long m = (long)blockIdx.y * 256 + threadIdx.x, cols = a.n0 + a.n1 + a.n2;
     if (m >= cols) return;
-    const int first = a.slot_of(p), end = a.slot_of(p + 1);
-    const long begin = (long)first + (long)(seg - a.seg_of(p)) * a.seg;
-    const long stop = begin + a.seg < end ? begin + a.seg : end;
-    if (begin >= end && seg != a.seg_of(p)) return;
+    int64_t begin, stop;
+    if (!a.segment(seg, p, begin, stop)) return;
     W s = 0;
     long k = begin;
     for (; k + 8 <= stop; k += 8) {
@@ -359,8 +342,8 @@ template <class W> __global__ __launch_bounds__(256) void k_join_out(const JoinA
     const int p = blockIdx.x;
     const long m = (long)blockIdx.y * 256 + threadIdx.x, cols = a.n0 + a.n1 + a.n2;
     if (m >= cols) return;
-    const int slots = max(0, a.slot_of(p + 1) - a.slot_of(p)), first = a.seg ? a.seg_of(p) : a.slot_of(p);
-    const int n = a.seg ? (slots + a.seg - 1) / a.seg : slots;
+    int first, n;
+    a.of_policy(p, first, n);
     const W* const mid = a.seg ? a.mid : a.part;
     W s = 0;
     int k0 = 0;
@@ -389,7 +372,7 @@ int join_seg(long slots) {
     while ((long)seg * seg < slots) seg *= 2;
     return seg;
 }
-long join_segs(long slots, int policies) { return slots / join_seg(slots) + policies + 1; }
+long join_segs(long slots, int policies) { return policy_segments(slots, policies, join_seg(slots)); }
 template <class W> int run_join(psh_ctx* c, JoinArgs<W>& a, long slots, hipStream_t st) {
     const unsigned by = (unsigned)((a.n0 + a.n1 + a.n2 + 255) / 256);
     a.seg = 0;
@@ -683,7 +666,7 @@ template <class T, int NP, int LPC, bool CARRY> __global__ __launch_bounds__(THR
     StepRows<T, SH> bc;
     ld.template fetch<false>(next, a, q.begin, q.end);
     bc.template fetch<!CARRY>(a, q.begin, q.end);
-    const long check0 = (long)q.part_begin / TS + q.part + (q.begin - q.part_begin) / TS;
+    const long check0 = check_slot(q, TS);
     for (int r0 = q.begin, tile = 0; r0 < q.end; r0 += TS, ++tile) {
         now = next;
         if (ld.on) {
@@ -769,7 +752,7 @@ template <class T, bool BACK> __global__ __launch_bounds__(256) void k_scan_join
     const long cols = (long)a.D * a.N;
     const int begin = a.parts.at(s), end = a.parts.at(s + 1);
     if (end - begin <= a.parts.L) return;
-    const int n = (int)(((long)end - begin + a.parts.L - 1) / a.parts.L), first = a.parts.first_slot(s);
+    const int n = piece_count(begin, end, a.parts.L), first = a.parts.first_slot(s);
     const int p = a.pol.of(s);
     const long m = min((long)blockIdx.y * JOIN_COLS + col, cols - 1);   // (threads behind the last state repeat it, and do not store)
     const bool mine = (long)blockIdx.y * JOIN_COLS + col < cols;
@@ -887,7 +870,7 @@ template <class T, int NP, int LPC, bool CARRY> __global__ __launch_bounds__(THR
     Rows<T, E> now, next;
     StepRows<T, SH> bc;
     const int tiles = q.begin < q.end ? (q.end - q.begin + TS - 1) / TS : 0;
-    const long check0 = (long)q.part_begin / TS + q.part + (q.begin - q.part_begin) / TS;
+    const long check0 = check_slot(q, TS);
     if (tiles > 0) {
         ld.template fetch<true>(next, a, q.begin + (tiles - 1) * TS, q.end);
         bc.template fetch<true>(a, q.begin + (tiles - 1) * TS, q.end);
@@ -1252,7 +1235,7 @@ template <class T> ScanArgs<T> scan_args(const psh_scan_desc* d, bool grad) {
     typedef typename Wide<T>::type W;
     ScanArgs<T> a{};
     a.parts = Parts{d->offsets, d->n_seqs, d->rows, (int)scan_piece(d, grad)};
-    a.pol = Policies{d->groups, d->groups ? d->n_policies : 1, d->n_seqs};
+    a.pol = Policies{{d->groups, d->groups ? d->n_policies : 1, d->n_seqs}};
     a.D = d->channels; a.N = d->states;
     a.u = (const T*)d->u; a.delta = (const T*)d->delta; a.z = (const T*)d->z; a.B = (const T*)d->B; a.C = (const T*)d->C;
     a.ld_u = d->ld_u; a.ld_delta = d->ld_delta; a.ld_z = d->ld_z; a.ld_B = d->ld_B; a.ld_C = d->ld_C;
@@ -1471,7 +1454,7 @@ template <class T, int K> int run_conv(psh_ctx* c, const psh_conv_desc* d, bool 
     constexpr int VW = conv_wide(sizeof(T), false), VG = conv_wide(sizeof(T), true);
     hipStream_t st = (hipStream_t)d->stream;
     ConvArgs<T> a{};
-    a.pol = Policies{d->groups, d->groups ? d->n_policies : 1, d->n_seqs};
+    a.pol = Policies{{d->groups, d->groups ? d->n_policies : 1, d->n_seqs}};
     a.x = (const T*)d->x; a.ld_x = d->ld_x;
     a.w = (const W*)d->weight; a.b = (const W*)d->bias;
     a.state = K > 1 ? (const T*)d->state : nullptr; a.stride_state = d->stride_state;

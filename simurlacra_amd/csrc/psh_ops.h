@@ -1,5 +1,5 @@
 // What the translation units of the policy operators (ops_linear.hip, ops_memory.hip) share: element types, the search
-// for the part of the rows that a workgroup works on, and the fp32 / fp64 elementary functions.
+// for the part of the rows that a workgroup works on (its arithmetic: psh_parts.h), and the fp32 / fp64 elementary functions.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -8,6 +8,7 @@
 
 #include "psh_ctx.h"
 #include "psh_math.h"
+#include "psh_parts.h"
 
 #define PSH_OP __device__ __forceinline__
 
@@ -92,56 +93,19 @@ template <class W> PSH_OP W nonlin_slope_w(int kind, W y) {
 }
 
 // ------------------------------------------------------------------------------------------ parts of the rows
-// Rows are cut into n parts by offsets (device memory, so the host cannot count tiles) and a launch works in pieces of L
-// rows.  Piece j of part i gets the slot  floor(off[i] / L) + i + j.  Two parts never share a slot: with off[i] = a L + r
-// and off[i+1] = b L + r', part i has ceil((b - a) + (r' - r) / L) <= b - a + 1 pieces, exactly the distance of the two
-// parts' first slots.  So slots are found without a prefix sum or a second launch, there are at most rows / L + n + 1 of
-// them, and every part owns at least one, empty parts too.  Part n stands for the rows behind the last offset.
-struct Parts {
-    const int* off;
-    int n, rows, L;
-    PSH_OP int at(int i) const {
-        if (i <= 0) return 0;
-        if (i > n) return rows;
-        const int o = off[i];
-        return o < 0 ? 0 : (o > rows ? rows : o);
-    }
-    PSH_OP int first_slot(int i) const { return at(i) / L + i; }
-};
-static inline long parts_slots(long rows, long n, long L) { return rows / L + n + 1; }
-
-struct Piece {
-    int part, j;      // piece j of the part
-    int begin, end;   // its rows (begin >= end: none)
-    int part_begin, part_end;
-};
-
-// the largest i in [0, n] with key(i) <= slot, for ascending keys with key(0) <= slot: every lane of the wave probes one of 64
-// candidates at once, so 4096 parts take two rounds of loads where a binary search takes twelve
 template <class F> PSH_OP int wave_search(int n, int slot, F key) {
     const int lane = __lane_id();
-    int lo = 0, count = n + 1;
-    while (count > 1) {
-        const int step = (count + 63) / 64;
-        const int i = lo + lane * step;
-        const bool below = lane * step < count && key(i) <= slot;
-        const int next = lo + (63 - __clzll(__ballot(below) | 1)) * step;   // (lane 0 probes lo itself: key(lo) <= slot)
-        count = min(step, lo + count - next);
-        lo = next;
+    Search s{0, n + 1};
+    while (s.count > 1) {
+        const int i = s.candidate(lane);
+        s.narrow(__ballot(s.probes(lane) && key(i) <= slot));
     }
-    return __builtin_amdgcn_readfirstlane(lo);
+    return __builtin_amdgcn_readfirstlane(s.lo);
 }
 
 PSH_OP Piece find_piece(const Parts& p, int slot) {
-    Piece q;
-    q.part = wave_search(p.n, slot, [&](int i) { return p.first_slot(i); });
-    q.part_begin = __builtin_amdgcn_readfirstlane(p.at(q.part));
-    q.part_end = __builtin_amdgcn_readfirstlane(p.at(q.part + 1));
-    q.j = slot - (q.part_begin / p.L + q.part);
-    const long b = (long)q.part_begin + (long)q.j * p.L, e = b + p.L;
-    q.begin = (int)(b < p.rows ? b : p.rows);
-    q.end = (int)(e < q.part_end ? e : q.part_end);
-    return q;
+    const int part = wave_search(p.n, slot, [&](int i) { return p.first_slot(i); });
+    return piece_of(p, part, __builtin_amdgcn_readfirstlane(p.at(part)), __builtin_amdgcn_readfirstlane(p.at(part + 1)), slot);
 }
 
 // ------------------------------------------------------------------------------------------ host side
