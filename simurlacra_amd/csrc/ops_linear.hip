@@ -16,6 +16,7 @@
 
 #include <type_traits>
 
+#include "psh_linear_plan.h"
 #include "psh_ops.h"
 
 namespace {
@@ -798,10 +799,6 @@ template <class T, int V> __global__ __launch_bounds__(256) void k_join(const Gr
     }
 }
 
-inline bool aligned16(const void* p, int size, int64_t ld, int64_t stride = 0) {
-    return ((uintptr_t)p & 15) == 0 && (ld * size) % 16 == 0 && (stride * size) % 16 == 0;
-}
-
 template <class K> int allow_lds(psh_ctx* c, K kernel, int bytes) {
     if (bytes > 64 * 1024) PSH_HIP(c, hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
     return PSH_OK;
@@ -835,30 +832,7 @@ template <class T, int BI, int BJ, int WI, int WJ, bool TW, bool DIRECT> int lau
     return PSH_OK;
 }
 
-enum TileKind { TILE_ROWS16, TILE_64, TILE_128, TILE_128_DIRECT, TILE_256_DIRECT };
-
-// Few rows a group (up to 24): 16 of them a tile.  64 groups of 10 rows, 1024 -> 1024, bf16: 23 to 25 us (5.4 TB/s of weights; 30 us in
-// 64 x 64); 256 groups of 8 rows, 6 -> 64, fp64: 5.9 us, a launch's latency (8.7 us).
-// Tiles [units][rows].  Large ones re-read the operands less often, small ones waste less where a group has few rows or a layer few
-// units, and there are more of them to fill the CUs: the larger ones are for layers that have one and a half of them for every CU.
-// bf16, 8 groups of about 4096 rows, 1024 -> 2048: 180 us (760 TFLOP/s) in 256 x 128 with two workgroups on a CU, of which one stores its tile
-// while the other multiplies; 197 us in 256 x 256 with one on a CU; 228 us in 128 x 128; 318 us in 64 x 64 (dx 174 and 633 us).  Without its loads from memory the first takes
-// 143 us, without those from LDS too 105 us.  12 groups of 2500 rows, 513 -> 257, fp32, 64 x 64: 115 us (69 TFLOP/s, the matrix pipes busy for
-// two thirds of the time, a fifth of it with columns behind the 257th).
-template <class T, bool TW> TileKind rows_kind(const RowsArgs<T>& a, int rows) {
-    const long mean = rows / a.parts.n;
-    if (mean <= 24) return TILE_ROWS16;
-    if constexpr (sizeof(T) == 2) {
-        const long large = ((long)rows / 128 + a.parts.n / 2) * ((a.n_out + 127) / 128), huge = ((long)rows / 128 + a.parts.n / 2) * ((a.n_out + 255) / 256);
-        if (mean >= 96 && a.n_out > 64 && large >= 192) {
-            const bool direct = aligned16(a.rows_in, 2, a.ld_in) && aligned16(a.weight, 2, a.ld_w, a.stride_w) && (!TW || a.n_out % 8 == 0);
-            return !direct ? TILE_128 : mean >= 512 && a.n_out > 128 && huge >= 768 ? TILE_256_DIRECT : TILE_128_DIRECT;
-        }
-    }
-    return TILE_64;
-}
-template <class T, bool TW> int run_rows(psh_ctx* c, RowsArgs<T>& a, int rows, hipStream_t st) {
-    const TileKind kind = rows_kind<T, TW>(a, rows);
+template <class T, bool TW> int run_rows(psh_ctx* c, RowsArgs<T>& a, TileKind kind, int rows, hipStream_t st) {
     if (kind == TILE_ROWS16) return launch_rows<T, 64, 16, 4, 1, TW, false>(c, a, rows, st);
     if constexpr (sizeof(T) == 2) {
         if (kind == TILE_128) return launch_rows<T, 128, 128, 2, 4, TW, false>(c, a, rows, st);
@@ -866,42 +840,6 @@ template <class T, bool TW> int run_rows(psh_ctx* c, RowsArgs<T>& a, int rows, h
         if (kind == TILE_256_DIRECT) return launch_rows<T, 256, 128, 2, 2, TW, true>(c, a, rows, st);
     }
     return launch_rows<T, 64, 64, 2, 2, TW, false>(c, a, rows, st);
-}
-
-// whether the weight gradient's bf16 operands can come by direct loads (dp is the caller's dy, or contiguous in the workspace)
-bool grad_direct(const psh_linear_desc* d) {
-    return (d->nonlin != PSH_NL_NONE || aligned16(d->dy, 2, d->ld_dy)) && aligned16(d->x, 2, d->ld_x) && d->out_dim % 8 == 0 && d->in_dim % 8 == 0;
-}
-// the weight gradient's tile: [out units][in units]
-int grad_tile(const psh_linear_desc* d) {
-    if (d->dtype != PSH_BF16 || d->out_dim <= 64 || d->in_dim <= 64) return 64;
-    const int64_t tiles = (int64_t)((d->out_dim + 127) / 128) * ((d->in_dim + 127) / 128);
-    const int64_t huge = (int64_t)((d->out_dim + 255) / 256) * ((d->in_dim + 255) / 256);
-    if (grad_direct(d) && d->out_dim > 128 && d->in_dim > 128 && huge * (d->rows / 2048 + d->n_groups) >= 384) return 256;
-    return tiles * (d->rows / 2048 + d->n_groups) >= 192 ? 128 : 64;
-}
-// rows of one piece of the weight gradient's contraction: enough pieces for about four workgroups a CU
-int64_t grad_piece(const psh_linear_desc* d) {
-    const int t = grad_tile(d);
-    const int64_t tiles = (int64_t)((d->out_dim + t - 1) / t) * ((d->in_dim + t - 1) / t);
-    const int64_t whole = ((int64_t)d->rows + 64) / 64 * 64;
-    const int64_t wanted = t == 256 ? 512 : t == 128 ? 1024 : 2048;
-    if (tiles >= wanted / 2) return whole;
-    int64_t L = ((int64_t)d->rows * tiles / wanted + 63) / 64 * 64;
-    if (L < 128) L = 128;
-    return L < whole ? L : whole;
-}
-
-struct GradSpace { int64_t dp, part_w, part_b, total; };
-GradSpace grad_space(const psh_linear_desc* d) {
-    GradSpace s{};
-    const int64_t slots = parts_slots(d->rows, d->n_groups, grad_piece(d));
-    if (d->nonlin != PSH_NL_NONE) s.dp = align256((int64_t)d->rows * d->out_dim * elem_size(d->dtype));
-    if (d->dweight) s.part_w = align256(slots * d->out_dim * d->in_dim * wide_size(d->dtype));
-    if (d->dbias) s.part_b = align256(slots * d->out_dim * wide_size(d->dtype));
-    if (d->rows <= grad_piece(d)) s.part_w = s.part_b = 0;   // no group has a second piece
-    s.total = s.dp + s.part_w + s.part_b;
-    return s;
 }
 
 int check(psh_ctx* c, const psh_linear_desc* d, bool grad) {
@@ -933,11 +871,6 @@ int check(psh_ctx* c, const psh_linear_desc* d, bool grad) {
     return PSH_OK;
 }
 
-TileKind grad_kind(const psh_linear_desc* d) {
-    const int t = grad_tile(d);
-    return t == 64 ? TILE_64 : !grad_direct(d) ? TILE_128 : t == 128 ? TILE_128_DIRECT : TILE_256_DIRECT;
-}
-
 // the weight gradient, with the input gradient in the same launch if `r` is given
 template <class T, int BIG, int SMALL, int WI, int WJ, bool DIRECT> int launch_weights(psh_ctx* c, GradArgs<T>& a, RowsArgs<T>* r, int rows, hipStream_t st) {
     a.slots = parts_slots(rows, a.parts.n, a.parts.L);
@@ -965,7 +898,7 @@ template <class T> int forward(psh_ctx* c, const psh_linear_desc* d) {
     a.out = (T*)d->y;
     a.wide = d->y_wide;
     a.n_in = d->in_dim; a.n_out = d->out_dim; a.nonlin = d->nonlin;
-    return run_rows<T, false>(c, a, d->rows, (hipStream_t)d->stream);
+    return run_rows<T, false>(c, a, forward_kind(d), d->rows, (hipStream_t)d->stream);
 }
 
 template <class T> int backward(psh_ctx* c, const psh_linear_desc* d) {
@@ -983,21 +916,19 @@ template <class T> int backward(psh_ctx* c, const psh_linear_desc* d) {
         ld_dp = d->out_dim;
     }
     RowsArgs<T> r{};
-    const bool weights = d->dweight || d->dbias;
-    bool rows = d->dx && d->rows > 0;
-    if (rows) {
+    const GradPlan plan = grad_plan(d);
+    if (d->dx && d->rows > 0) {
         r.parts = Parts{d->offsets, d->n_groups, d->rows, 0};
         r.rows_in = dp; r.ld_in = ld_dp;
         r.weight = (const T*)d->weight; r.ld_w = d->ld_w; r.stride_w = d->stride_w;
         r.out = (T*)d->dx;
         r.n_in = d->out_dim; r.n_out = d->in_dim; r.nonlin = PSH_NL_NONE;
-        if (!weights || rows_kind<T, true>(r, d->rows) != grad_kind(d)) {
-            const int rc = run_rows<T, true>(c, r, d->rows, st);
+        if (!plan.joint) {
+            const int rc = run_rows<T, true>(c, r, plan.rows, d->rows, st);
             if (rc != PSH_OK) return rc;
-            rows = false;
         }
     }
-    if (weights) {
+    if (d->dweight || d->dbias) {
         GradArgs<T> a{};
         a.parts = Parts{d->offsets, d->n_groups, d->rows, (int)grad_piece(d)};
         a.dp = dp; a.ld_dp = ld_dp;
@@ -1005,8 +936,8 @@ template <class T> int backward(psh_ctx* c, const psh_linear_desc* d) {
         a.dw = (T*)d->dweight; a.db = (T*)d->dbias;
         a.part_w = (W*)(space + s.dp); a.part_b = (W*)(space + s.dp + s.part_w);
         a.n = d->out_dim; a.k = d->in_dim;
-        RowsArgs<T>* const also = rows ? &r : nullptr;
-        const TileKind kind = grad_kind(d);
+        RowsArgs<T>* const also = plan.joint ? &r : nullptr;
+        const TileKind kind = plan.weights;
         int rc;
         if constexpr (sizeof(T) == 2) {
             if (kind == TILE_64) rc = launch_weights<T, 64, 64, 2, 2, false>(c, a, also, d->rows, st);

@@ -127,6 +127,3 @@ struct DeviceScope {
         set_err(ctx, "cannot make the context's GPU current");                     \
         return PSH_ERR_HIP;                                                        \
     }
-static inline int64_t align256(int64_t n) { return (n + 255) & ~(int64_t)255; }
-static inline int elem_size(int dtype) { return dtype == PSH_F64 ? 8 : dtype == PSH_F32 ? 4 : 2; }
-static inline int wide_size(int dtype) { return dtype == PSH_F64 ? 8 : 4; }

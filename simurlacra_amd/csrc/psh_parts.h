@@ -5,6 +5,8 @@
 
 #include <cstdint>
 
+#include "../../include/pysimhip.h"
+
 #define PSH_BOTH __host__ __device__ __forceinline__
 
 // Rows are cut into n parts by offsets (device memory, so the host cannot count tiles) and a launch works in pieces of L
@@ -98,3 +100,7 @@ struct PolicySlots {
     }
 };
 PSH_BOTH int64_t policy_segments(int64_t slots, int policies, int seg) { return slots / seg + policies + 1; }
+
+static inline int64_t align256(int64_t n) { return (n + 255) & ~(int64_t)255; }
+static inline int elem_size(int dtype) { return dtype == PSH_F64 ? 8 : dtype == PSH_F32 ? 4 : 2; }
+static inline int wide_size(int dtype) { return dtype == PSH_F64 ? 8 : 4; }

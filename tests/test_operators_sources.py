@@ -1,10 +1,15 @@
 """
 CPU tests of the policy operators' kernel sources: what the compiler has to be told about assembly that is written by hand.
 """
+import ctypes
 import glob
 import os
 import re
 import subprocess
+
+from simurlacra_amd import _abi as abi
+from simurlacra_amd.engine import load_library
+from tests import layer_cases, linear_plan
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 SOURCES = sorted(glob.glob(os.path.join(ROOT, 'simurlacra_amd', 'csrc', 'ops_*.hip')) + [os.path.join(ROOT, 'simurlacra_amd', 'csrc', 'psh_ops.h')])
@@ -40,7 +45,37 @@ def test_fixed_registers_that_assembly_writes_are_named_to_the_compiler():
 def test_rows_slots_and_segments_for_offsets_of_any_kind(tmp_path):
     """ The arithmetic of csrc/psh_parts.h, which every kernel of the operators takes its rows from, compiled for the CPU (overflows trap). """
     exe = str(tmp_path/'parts_check')
-    subprocess.check_call(['g++', '-std=c++17', '-O1', '-ftrapv', '-D__host__=', '-D__device__=', '-D__forceinline__=inline', '-include', 'algorithm',
-                           '-I', os.path.join(ROOT, 'simurlacra_amd', 'csrc'), os.path.join(ROOT, 'tests', 'native', 'parts_check.cpp'), '-o', exe])
+    subprocess.check_call(['g++', '-std=c++17', '-O1', '-ftrapv', '-include', 'algorithm', *linear_plan.NATIVE, os.path.join(ROOT, 'tests', 'native', 'parts_check.cpp'), '-o', exe])
     run = subprocess.run([exe, '6000'], capture_output=True, text=True)
     assert run.returncode == 0 and run.stdout.strip() == 'ok', run.stdout + run.stderr
+
+
+def _descriptor(lengths, K, N, shift, nonlin):
+    """ of a call as tests/test_gpu_operators_tiles.py makes it """
+    d = abi.PshLinearDesc()
+    ld = (K + 7)//8*8 + 8
+    d.dtype, d.nonlin, d.n_groups, d.rows, d.in_dim, d.out_dim = abi.DTYPE_BF16, abi.NL_IDS[nonlin], len(lengths), sum(lengths) + 3, K, N
+    d.ld_x = d.ld_w = ld
+    d.stride_w, d.ld_dy = N*ld, (N + 7)//8*8
+    d.x = d.weight = 4096 + 2*shift
+    d.offsets = d.y = d.dy = d.dx = d.dweight = d.dbias = d.workspace = 4096
+    return d
+
+
+def test_the_layer_cases_reach_every_kind_of_tile():
+    reached = set()
+    for name, (lengths, K, N, shift, nonlin, forward, dx, dw, joint) in layer_cases.CASES.items():
+        p = linear_plan.plan(_descriptor(lengths, K, N, shift, nonlin))
+        assert (p.forward, p.dx, p.dw, p.joint) == (forward, dx, dw, joint), (name, [linear_plan.KINDS[k] for k in p[:3]], p.joint)
+        reached |= linear_plan.kernels(p)
+    kinds = range(len(linear_plan.KINDS))
+    every = {(k, t) for k in ('forward', 'dx') for t in kinds} | {(k, t) for k in ('dw', 'both') for t in kinds if t != linear_plan.ROWS16}
+    assert reached >= every, every - reached
+
+
+def test_the_rules_are_those_of_the_library():
+    """ (as far as the library tells: the size of the scratch memory, which follows from the tiles and pieces) """
+    lib = load_library()
+    for lengths, K, N, shift, nonlin, *_ in layer_cases.CASES.values():
+        d = _descriptor(lengths, K, N, shift, nonlin)
+        assert lib.psh_grouped_linear_grad_workspace(ctypes.byref(d)) == linear_plan.plan(d).space
