@@ -673,7 +673,8 @@ template <class T> struct GradArgs {   // dW, db
     const T* dp; long ld_dp;
     const T* x; long ld_x;
     T* dw; T* db;                      // [G, n, k], [G, n]
-    typename Wide<T>::type* part_w;    // [slots, n, k] and [slots, n]: sums of groups that are cut into several pieces
+    CutPlaces places;
+    typename Wide<T>::type* part_w;    // [places, n, k] and [places, n]: sums of groups that are cut into several pieces
     typename Wide<T>::type* part_b;
     int n, k;
     long slots, tiles_i, tiles_j;
@@ -701,7 +702,7 @@ template <class T, int BI, int BJ, int WI, int WJ, bool DIRECT> PSH_OP void weig
         else tile.template multiply<true, true, false>(p, x, lds);
     }
     constexpr int step = sizeof(T) == 8 ? 4 : 1;
-    const long at = (long)(whole ? q.part : slot) * a.n;
+    const long at = (whole ? q.part : a.places.first(a.parts, q.part, q.part_begin) + q.j) * a.n;
     if (a.dw) {
         // rows of the tile are output units here
         const auto put = [&](auto* out) {
@@ -764,10 +765,11 @@ template <class T, int V> __global__ __launch_bounds__(256) void k_join(const Gr
     for (int g = blockIdx.y; g < a.parts.n; g += gridDim.y) {
         const int begin = a.parts.at(g), end = a.parts.at(g + 1);
         if (end - begin <= a.parts.L) continue;
-        const int pieces = piece_count(begin, end, a.parts.L), first = a.parts.first_slot(g);
+        const int pieces = piece_count(begin, end, a.parts.L);
+        const long first = a.places.first(a.parts, g, begin);
         const long threads = (long)gridDim.x * 256, me = (long)blockIdx.x * 256 + threadIdx.x;
         for (long e = me * V; e < nw; e += threads * V) {
-            const W* const src = a.part_w + (long)first * nw + e;
+            const W* const src = a.part_w + first * nw + e;
             W s[V] = {};
             T out[V];
             for (int j0 = 0; j0 < pieces; j0 += 32) {   // (in blocks, for the same reason as in fold())
@@ -787,7 +789,7 @@ template <class T, int V> __global__ __launch_bounds__(256) void k_join(const Gr
             __builtin_memcpy(a.dw + (long)g * nw + e, out, sizeof(out));
         }
         for (long e = me; e < nb; e += threads) {
-            const W* const src = a.part_b + (long)first * nb + e;
+            const W* const src = a.part_b + first * nb + e;
             W s = 0;
             for (int j0 = 0; j0 < pieces; j0 += 32) {
                 W p = 0;
@@ -931,6 +933,7 @@ template <class T> int backward(psh_ctx* c, const psh_linear_desc* d) {
     if (d->dweight || d->dbias) {
         GradArgs<T> a{};
         a.parts = Parts{d->offsets, d->n_groups, d->rows, (int)grad_piece(d)};
+        a.places = cut_places(d->rows, d->n_groups, a.parts.L);
         a.dp = dp; a.ld_dp = ld_dp;
         a.x = (const T*)d->x; a.ld_x = d->ld_x;
         a.dw = (T*)d->dweight; a.db = (T*)d->dbias;

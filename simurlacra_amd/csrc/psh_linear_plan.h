@@ -63,10 +63,10 @@ inline int64_t grad_piece(const psh_linear_desc* d) {
 struct GradSpace { int64_t dp, part_w, part_b, total; };
 inline GradSpace grad_space(const psh_linear_desc* d) {
     GradSpace s{};
-    const int64_t slots = parts_slots(d->rows, d->n_groups, grad_piece(d));
+    const int64_t places = cut_places_count(d->rows, d->n_groups, grad_piece(d));
     if (d->nonlin != PSH_NL_NONE) s.dp = align256((int64_t)d->rows * d->out_dim * elem_size(d->dtype));
-    if (d->dweight) s.part_w = align256(slots * d->out_dim * d->in_dim * wide_size(d->dtype));
-    if (d->dbias) s.part_b = align256(slots * d->out_dim * wide_size(d->dtype));
+    if (d->dweight) s.part_w = align256(places * d->out_dim * d->in_dim * wide_size(d->dtype));
+    if (d->dbias) s.part_b = align256(places * d->out_dim * wide_size(d->dtype));
     if (d->rows <= grad_piece(d)) s.part_w = s.part_b = 0;   // no group has a second piece
     s.total = s.dp + s.part_w + s.part_b;
     return s;

@@ -45,6 +45,19 @@ PSH_BOTH Piece piece_of(const Parts& p, int part, int part_begin, int part_end, 
     q.end = (int)(e < part_end ? e : part_end);
     return q;
 }
+// Room for partial results of the parts of more than L rows, which are cut; the others have none.  Piece j of a part from row b has the
+// place floor(2 b / L) + j: a part of x L rows has ceil(x) pieces, no more than floor(2 x) for x > 1, and the next part's places begin
+// at least floor(2 x) further on.  These are at most 2 rows / L + 1 places however many parts there are; with few parts there are
+// fewer slots than that, and a piece's place is its slot.
+struct CutPlaces {
+    bool by_rows;
+    PSH_BOTH int64_t first(const Parts& p, int part, int part_begin) const { return by_rows ? 2 * (int64_t)part_begin / p.L : part_begin / p.L + part; }
+};
+PSH_BOTH int64_t places_by_rows(int64_t rows, int64_t L) { return 2 * rows / L + 1; }
+PSH_BOTH CutPlaces cut_places(int64_t rows, int64_t n, int64_t L) { return CutPlaces{places_by_rows(rows, L) < parts_slots(rows, n, L)}; }
+PSH_BOTH int64_t cut_places_count(int64_t rows, int64_t n, int64_t L) {
+    return cut_places(rows, n, L).by_rows ? places_by_rows(rows, L) : parts_slots(rows, n, L);
+}
 // where the states stored before every tile of TS steps of a piece begin (TS divides L)
 PSH_BOTH int64_t check_slot(const Piece& q, int TS) { return (int64_t)q.part_begin / TS + q.part + (q.begin - q.part_begin) / TS; }
 

@@ -88,6 +88,20 @@ int main(int argc, char** argv) {
                     seen[r] = 1;
                 }
         }
+        for (const CutPlaces by : {CutPlaces{true}, CutPlaces{false}, cut_places(rows, n, L)}) {   // places of the pieces of parts that are cut
+            const int64_t count = by.by_rows ? places_by_rows(rows, L) : slots;
+            NEED(count >= cut_places_count(rows, n, L));
+            std::vector<char> taken(count, 0);
+            for (int i = 0; i < n; ++i) {
+                const int b = parts.at(i), e = parts.at(i + 1);
+                if (e - b <= L) continue;
+                for (int j = 0; j < piece_count(b, e, L); ++j) {
+                    const int64_t at = by.first(parts, i, b) + j;
+                    NEED(at >= 0 && at < count && !(ascend && taken[at]));
+                    taken[at] = 1;
+                }
+            }
+        }
         for (int i = 0; i < n; ++i) {   // pieces that are joined
             const int b = parts.at(i), e = parts.at(i + 1);
             if (e - b > L) NEED(parts.first_slot(i) + (int64_t)piece_count(b, e, L) <= slots);

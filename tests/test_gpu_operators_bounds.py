@@ -8,7 +8,8 @@ import math
 import pytest
 import torch
 
-from tests.test_gpu_operators import IDS, TYPES, offs, rnd, scan_inputs
+from tests import operators_ref as ref
+from tests.test_gpu_operators import IDS, TYPES, close, offs, rnd, scan_inputs
 
 pytestmark = pytest.mark.gpu
 FENCE, MARK = 1 << 16, 0xA5
@@ -123,3 +124,20 @@ def test_the_fences_see_a_byte():
         with pytest.raises(AssertionError):
             fences.check()
         fences.given[0][0][at] = MARK
+
+
+@pytest.mark.parametrize('T', TYPES, ids=IDS)
+def test_few_large_groups_among_many_small_ones(ops, monkeypatch, T):
+    """ The sums of the large ones are cut into pieces, which alone have scratch memory: against the definition, and between fences. """
+    gen = torch.Generator().manual_seed(8)
+    lengths, K, N = [2]*150 + [1000] + [0, 3]*80 + [700, 129, 128], 40, 72
+    off, R, G = offs(lengths), sum(lengths) + 2, len(lengths)
+    x, w, dy = rnd(gen, R, K, T=T), rnd(gen, G, N, K, T=T, scale=K**-.5), rnd(gen, R, N, T=T)
+    want, M = (ref.linear(x, w, None, off, None, dy, mag=m) for m in (False, True))
+    fences = Fences()
+    with fences.around(monkeypatch):
+        got = ops.grouped_linear_grad(dy, None, x, w, off)
+    fences.check()
+    assert sum(n for _, n in fences.given) < 2*sum(t.numel()*t.element_size() for t in got)
+    for name, g, n in zip(('dx', 'dw', 'db'), got, (N + 8, max(lengths) + 8, max(lengths) + 8)):
+        close(name, g, want[name], M[name], n, T)

@@ -7,6 +7,8 @@ import os
 import re
 import subprocess
 
+import pytest
+
 from simurlacra_amd import _abi as abi
 from simurlacra_amd.engine import load_library
 from tests import layer_cases, linear_plan
@@ -79,3 +81,14 @@ def test_the_rules_are_those_of_the_library():
     for lengths, K, N, shift, nonlin, *_ in layer_cases.CASES.values():
         d = _descriptor(lengths, K, N, shift, nonlin)
         assert lib.psh_grouped_linear_grad_workspace(ctypes.byref(d)) == linear_plan.plan(d).space
+
+
+@pytest.mark.parametrize('groups,rows,K,N', [(64, 640, 1024, 1024), (256, 2560, 2048, 2048), (1000, 130, 40, 72), (5000, 20000, 256, 256)])
+def test_groups_that_are_not_cut_take_no_scratch_memory(groups, rows, K, N):
+    """ Only a group of more rows than a piece has partial sums, of its pieces: there are no more than twice as many of those as
+    pieces fit into the rows, and one, however many groups there are. """
+    for dtype, wide in ((abi.DTYPE_BF16, 4), (abi.DTYPE_F32, 4), (abi.DTYPE_F64, 8)):
+        d = _descriptor([rows//groups]*(groups - 1) + [rows - 3 - rows//groups*(groups - 1)], K, N, 0, None)
+        d.dtype = dtype
+        piece = linear_plan.plan(d).piece
+        assert load_library().psh_grouped_linear_grad_workspace(ctypes.byref(d)) <= (2*rows//piece + 1)*(N*K + N)*wide + 2*256
