@@ -171,7 +171,7 @@ class SSMPolicy(RecurrentPolicy):
         hidden = to.zeros(n, self.hidden_size, dtype=w.dtype, device=w.device) if hidden is None else hidden.to(w.device, w.dtype)
         if tuple(hidden.shape) != (n, self.hidden_size):
             raise ShapeErr(msg=f'hidden must have {self.hidden_size} entries for each of {n} environments, but has the shape {list(hidden.shape)}!')
-        return obs.to(w.device, w.dtype), hidden
+        return obs.to(w.device, w.dtype), hidden.contiguous()   # (whose memory is divided into the layers' states)
 
     def forward(self, obs: to.Tensor, hidden: to.Tensor = None):
         """ One step: obs [O] and hidden [H], or obs [B, O] and hidden [B, H] (None: the state before a first step). """
