@@ -145,4 +145,4 @@ class FNNPolicy(Policy):
 
     def population_evaluate(self, params: to.Tensor, obs: to.Tensor, offsets: to.Tensor, groups: to.Tensor) -> to.Tensor:
         """ The actions for whole episodes obs[offsets[s]:offsets[s + 1]], of which groups[p] .. groups[p + 1] - 1 are policy p's. """
-        return self.population_forward(params, obs, offsets[groups.long()])
+        return self.population_forward(params.to(obs.device, obs.dtype), obs, offsets[groups.long()])

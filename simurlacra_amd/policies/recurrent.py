@@ -210,4 +210,4 @@ class SSMPolicy(RecurrentPolicy):
     def population_evaluate(self, params: to.Tensor, obs: to.Tensor, offsets: to.Tensor, groups: to.Tensor) -> to.Tensor:
         """ The actions for whole episodes obs[offsets[s]:offsets[s + 1]], of which groups[p] .. groups[p + 1] - 1 are policy p's. """
         obs, hidden = self._inputs(obs, None, offsets.shape[0] - 1)
-        return self._run(self._named(params), obs, offsets[groups.long()], offsets, groups, hidden, False)[0]
+        return self._run(self._named(params.to(obs.device, obs.dtype)), obs, offsets[groups.long()], offsets, groups, hidden, False)[0]

@@ -17,6 +17,30 @@ def env():
     return ActNormWrapper(QQubeSim(dt=1/250., max_steps=30))
 
 
+@pytest.mark.parametrize('make', [lambda spec: SSMPolicy(spec, hidden_size=8, dtype=to.float32),
+                                  lambda spec: SSMPolicy(spec, hidden_size=8),
+                                  lambda spec: FNNPolicy(spec, hidden_sizes=[80], hidden_nonlin=to.tanh)], ids=['ssm f32', 'ssm f64', 'fnn'])
+@pytest.mark.parametrize('dtype', [to.float64, to.float32], ids=['f64 sets', 'f32 sets'])
+def test_parameter_sets_of_either_type_are_sampled_and_evaluated(make, dtype):
+    """ sample() takes them as any type, so the evaluation of what it recorded does; the gradient has theirs """
+    pyrado.set_seed(1)
+    e = env()
+    policy = make(e.spec)
+    sets = (policy.param_values.detach().cpu().double() + 0.2*to.randn(3, policy.num_param, dtype=to.float64)).to(dtype)
+    res = ParameterExplorationSampler(e, policy, num_rollouts_per_param=2, seed=3).sample(sets)
+    leaf = sets.clone().requires_grad_()
+    acts, off = evaluate_population(policy, leaf, res.batch)
+    own = next(policy.parameters()).dtype
+    assert acts.dtype == own and int(off[-1]) == acts.shape[0]
+    # the rollouts' own actions: sums of at most 80 terms of order 1 in a few layers, 30 steps, in another order
+    tol = 1e-9 if own == to.float64 else 30*80*8*2.**-24
+    for k in range(6):
+        want = to.as_tensor(res.batch[k].actions)
+        assert (acts[int(off[k]):int(off[k + 1])].cpu().double() - want).abs().max() <= tol
+    grad, = to.autograd.grad(acts.double().square().sum(), leaf)
+    assert grad.dtype == dtype and grad.shape == sets.shape and bool(grad.isfinite().all()) and bool((grad != 0).any())
+
+
 def test_hidden_states_of_any_layout():
     pyrado.set_seed(2)
     policy = SSMPolicy(env().spec, hidden_size=8, num_layers=2)
