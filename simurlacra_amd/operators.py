@@ -116,15 +116,20 @@ def _any_requires_grad(*tensors):
     return False
 
 
-_is_tracing, _modes, _dispatched_with = torch._C._is_tracing, torch._C._len_torch_dispatch_stack, torch._C._dispatch_tls_is_dispatch_key_included
-_PRE_DISPATCH, _PROXY = torch._C.DispatchKey.PreDispatch, torch._C._TorchDispatchModeKey.PROXY
+_is_tracing, _modes, _function_modes = torch._C._is_tracing, torch._C._len_torch_dispatch_stack, torch._C._len_torch_function_stack
+
+
+def _recorded():
+    """ Whether torch is recording: by jit.trace, or by make_fx in one of the two places where it listens. """
+    return (_is_tracing() or torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None
+            or torch._C._dispatch_tls_is_dispatch_key_included(torch._C.DispatchKey.PreDispatch))
 
 
 def _seen_by_torch(*tensors):
     """ The kernels run past torch, which sees the tensors that come out and nothing of how they came about.  What it can only do with
     operations that it sees is refused: a recorded call would be empty memory whenever it is played back, and a tangent of forward
     differentiation would be dropped and the derivative read as zero. """
-    if _is_tracing() or _dispatched_with(_PRE_DISPATCH) or (_modes() and torch._C._get_dispatch_mode(_PROXY) is not None):
+    if (_is_tracing() or _modes() or _function_modes()) and _recorded():
         raise ValueErr(msg='the policy operators cannot be recorded (torch.jit.trace, make_fx): torch does not see what they do!')
     if _forward._current_level >= 0:
         for t in tensors:
@@ -347,11 +352,12 @@ def _conv_desc(x, weight, bias, offsets, groups, state, silu, step):
     d = abi.PshConvDesc(_DTYPES[dt], 1 if silu else 0, 1 if step else 0, P, S, R, D, K, _ptr(offsets), _ptr(groups), x.data_ptr(), weight.data_ptr(),
                         _ptr(bias))
     d.ld_x = ld_x
+    stride = 0
     if state is not None:
-        state, d.stride_state = _state_arg('state', state, dt, dev, (S, D, K - 1))
-        d.state = _ptr(state)
+        state, stride = _state_arg('state', state, dt, dev, (S, D, K - 1))
+        d.state, d.stride_state = _ptr(state), stride
     d.stream = eng._stream()
-    return eng, d, (x, weight, bias, offsets, groups, state), S, R, D, P, K, dt, dev
+    return eng, d, (x, weight, bias, offsets, groups, state, stride), S, R, D, P, K, dt, dev
 
 
 def _conv_forward(x, weight, bias, offsets, groups, state, silu):
@@ -428,8 +434,8 @@ def causal_conv_step(x, state, weight, bias, groups=None, silu: bool = True):
     eng, d, keep, S, R, D, P, K, dt, dev = _conv_desc(x, weight, bias, None, groups, state, silu, True)
     if S and K > 1 and keep[5] is not state:
         raise ValueErr(msg='state is updated in place: the values of each sequence have to be contiguous!')
-    y = x.new_empty(R, D)
-    d.y, d.last, d.stride_last = y.data_ptr(), state.data_ptr(), d.stride_state
+    y, stride = x.new_empty(R, D), keep[6]
+    d.y, d.last, d.stride_last = y.data_ptr(), state.data_ptr(), stride
     eng._call('psh_causal_conv', C.byref(d))
     _advanced(state)
     del keep
@@ -465,7 +471,7 @@ def _scan_desc(u, delta, A, B, Cm, D, z, delta_bias, offsets, groups, state, ste
     d = abi.PshScanDesc(_DTYPES[dt], 1 if step else 0, P, S, R, ch, N, 0, _ptr(offsets), _ptr(groups), u.data_ptr(), delta.data_ptr(), _ptr(z), B.data_ptr(),
                         Cm.data_ptr(), A.data_ptr(), _ptr(D), _ptr(delta_bias), _ptr(state), None, None, ld_u, ld_delta, ld_z, ld_B, ld_C, stride)
     d.stream = eng._stream()
-    return eng, d, (u, delta, A, B, Cm, D, z, delta_bias, offsets, groups, state), S, R, ch, P, N, dt, W, dev
+    return eng, d, (u, delta, A, B, Cm, D, z, delta_bias, offsets, groups, state, stride), S, R, ch, P, N, dt, W, dev
 
 
 def _scan_forward(u, delta, A, B, Cm, D, z, delta_bias, offsets, groups, state, keep_check):
@@ -577,8 +583,8 @@ def _scan_step(u, delta, state, A, B, Cm, D, z, delta_bias, groups):
     eng, d, keep, S, R, ch, P, N, dt, W, dev = _scan_desc(u, delta, A, B, Cm, D, z, delta_bias, None, groups, state, True)
     if S and keep[10] is not state:
         raise ValueErr(msg='state is updated in place: the values of each sequence have to be contiguous!')
-    y = u.new_empty(R, ch)
-    d.y, d.last, d.stride_last = y.data_ptr(), state.data_ptr(), d.stride_state
+    y, stride = u.new_empty(R, ch), keep[11]
+    d.y, d.last, d.stride_last = y.data_ptr(), state.data_ptr(), stride
     eng._call('psh_selective_scan', C.byref(d))
     _advanced(state)
     del keep

@@ -59,3 +59,33 @@ def test_more_rows_than_can_be_counted_are_refused(ops):
         ops.grouped_linear(x, w, None, offs([5]))
     with pytest.raises(ValueErr, match='can count'):
         ops.causal_conv_step(x, x.view(-1, 1, 1)[:, :, :0], torch.ones(1, 1, 1, device='cuda'), None)
+
+
+@pytest.mark.parametrize('name', ['grouped_linear', 'causal_conv', 'selective_scan', 'causal_conv_step', 'selective_scan_step'])
+def test_compiled_functions_call_the_operators_between_their_graphs(ops, name):
+    """ torch.compile leaves the calls as they are, differentiated ones too, and sees what the steps change """
+    gen = torch.Generator().manual_seed(3)
+    S, D, N = 6, 8, 4
+    off = offs([1]*S)
+    x, w, st, cw = rnd(gen, S, D), rnd(gen, S, 5, D), rnd(gen, S, D, 3), rnd(gen, 1, D, 4)
+    v, _, _ = scan_inputs(gen, ops, torch.float64, [1]*S, D, N, None, tail=0)
+    h = v.pop('state')
+    rest = {k: t for k, t in v.items() if k != 'u'}
+    calls = {'grouped_linear': lambda x, s: ops.grouped_linear(2*x, w, None, off, 'tanh') + 1,
+             'causal_conv': lambda x, s: ops.causal_conv(2*x, cw, None, off, state=s) + 1,
+             'selective_scan': lambda x, s: ops.selective_scan(2*x, **rest, offsets=off, state=s) + 1,
+             'causal_conv_step': lambda x, s: ops.causal_conv_step(2*x, s, cw, None) + s.sum(),
+             'selective_scan_step': lambda x, s: ops.selective_scan_step(2*x, state=s, **rest) + s.sum()}
+    f, state = calls[name], h if 'scan' in name else st
+    torch._dynamo.reset()
+    for backend in ('eager', 'aot_eager'):
+        compiled = torch.compile(f, backend=backend)
+        for train in (False, True) if 'step' not in name else (False,):
+            for turn in range(3):
+                a, b = (x + turn).requires_grad_(train), (x + turn).requires_grad_(train)
+                s, t = state.clone(), state.clone()
+                want, got = f(a, s), compiled(b, t)
+                assert torch.equal(want, got) and torch.equal(s, t)
+                if train:
+                    assert torch.equal(*(torch.autograd.grad(y.sum(), q)[0] for y, q in ((want, a), (got, b))))
+    torch._dynamo.reset()
