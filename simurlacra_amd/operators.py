@@ -102,10 +102,11 @@ def _offsets(name, t, device):
         raise TypeErr(msg=f'{name} must be of type torch.int32, but is {t.dtype}!')
     if t.device != device:
         raise ValueErr(msg=f'{name} must be on {device}, but is on {t.device}!')
-    if t.dim() != 1 or t.shape[0] < 2:
-        raise ShapeErr(msg=f'{name} must have one entry more than there are parts (at least two), but has the shape {list(t.shape)}!')
-    if t.shape[0] > _MOST:
-        _too_large(name, t.shape[0])
+    shape = t.shape
+    if len(shape) != 1 or shape[0] < 2:
+        raise ShapeErr(msg=f'{name} must have one entry more than there are parts (at least two), but has the shape {list(shape)}!')
+    if shape[0] > _MOST:
+        _too_large(name, shape[0])
     return t.contiguous()
 
 
@@ -326,12 +327,14 @@ def _state_arg(name, t, dtype, dev, shape):
         raise TypeErr(given=t, given_name=name, expected_type=_Tensor)
     if t.dtype != dtype or t.device != dev:
         raise TypeErr(msg=f'{name} must be of type {dtype} on {dev}, but is {t.dtype} on {t.device}!')
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ShapeErr(msg=f'{name} must have the shape {list(shape)}, but has {list(t.shape)}!')
     size = shape[1]*shape[2]
-    if t.numel() and not (t[0].is_contiguous() and (shape[0] == 1 or t.stride(0) >= size)):
-        return t.contiguous(), size
-    return t, (t.stride(0) if shape[0] > 1 else size)
+    apart, line, step = t.stride()
+    if (step != 1 and shape[2] > 1) or (line != shape[2] and shape[1] > 1) or (apart < size and shape[0] > 1):
+        if size:
+            return t.contiguous(), size
+    return t, (apart if shape[0] > 1 else size)
 
 
 def _conv_desc(x, weight, bias, offsets, groups, state, silu, step):
