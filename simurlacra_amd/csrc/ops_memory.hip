@@ -51,8 +51,9 @@ template <int E, class T> PSH_OP typename Vec<T, E>::type load_raw(const T* line
 // y[t, d] = f(b[d] + sum_k w[d, k] x[t - (K - 1) + k, d]).  A lane holds V neighbouring channels (16 bytes) and walks down a run of rows with
 // the last K inputs in registers, so every input is read once (K - 1 rows of a run again at its start).  One wave: one piece
 // of a sequence, its lanes split over the channels first and over runs with what is left of the 64.
-// Bound by the bytes of x and y: 120000 x 128 fp32 in 32 us (3.9 TB/s; a copy reaches 4.7), 131072 x 256 bf16 in 42 us
-// (3.2 TB/s: of its 2-byte values twice as many have to go through an exponential and a reciprocal in the same time).
+// Bound by the bytes of x and y: 120000 x 128 fp32 in 32 us (3.9 TB/s; a copy reaches 4.7).  131072 x 256 bf16 in 42 us (3.2 TB/s) is bound by
+// neither: the vector pipes are busy for half of it (18 instructions an element, two of them an exponential and a reciprocal), and the
+// waves wait for the other half, with the loads of four rows each in flight.
 template <class T> struct ConvArgs {
     Parts parts;
     Policies pol;
@@ -806,8 +807,10 @@ template <class T, bool BACK> __global__ __launch_bounds__(256) void k_scan_join
 // per lane), then backward:  dA += G h_{t-1} dt,  ddt = sum_n G h_{t-1} A + u sum_n g B,  du = dt sum_n g B + D dy0,  and, summed over
 // the channels, dB = g dt u and dC = dy0 h.  The sums over a wave's 16 channels swap halves and quarters of the wave, so that eight sums
 // take 16 instructions; those over the waves go through LDS, those over workgroups through memory (k_sum_bc), none by atomics.
-// Bound by instruction issue at two waves a SIMD: 100 instructions a step for four states of 16 channels, 52 of them the formulas, 33 the
-// sums, the rest reads of LDS and waits.  131072 x 256 x 16 states, bf16: 600 us; 65437 x 96 x 8, fp32, 256 sequences: 142 us, the time of the longest of them.
+// Bound by instruction issue for three quarters of the time, by what two waves a SIMD leave uncovered of the steps' latency for the rest: 101 vector
+// instructions a step for four states of 16 channels, 52 of them the formulas, 33 the sums, besides 12 reads and writes of LDS.  131072 x 256 x 16
+// states, bf16: 590 us (690 cycles a step of a wave, of which the vector pipe is busy for 450); 65437 x 96 x 8, fp32, 256 sequences: 145 us,
+// the time of the longest of them (vector pipes busy for 60 %).
 // CARRY: only G at the piece's beginning, from zero.
 template <class T, int NP, int LPC, bool CARRY> __global__ __launch_bounds__(THREADS, 2) void k_scan_grad(const ScanArgs<T> a) {
     typedef typename Wide<T>::type W;
@@ -1156,6 +1159,13 @@ int64_t tile_steps(int dtype) { return dtype == PSH_F64 ? 8 : 16; }
 // shorter step each, at the price of its fixed work).  Where sequences have more than 192 rows on average the pieces win: one
 // of 16384 rows, 256 channels, 16 states, bf16, takes 1536 us spread and 55 us in 256 pieces; 64 of 300 rows, 64 x 16, fp64, 147 and 87 us
 // (gradient 265 and 133 us).
+// The limit of 512 workgroups, by sequences of 256 rows on average, forward (gradient) in us, in pieces and whole:
+//   fp32, 96 x 8, two workgroups a sequence:    64: 30, 60 (69, 130)    192: 64, 64 (155, 136)   255: 80, 65 (205, 139)   257: 78, 65 (202, 138)
+//   bf16, 256 x 16, four workgroups a sequence: 64: 67, 65 (134, 134)   100: 96, 65 (214, 141)   127: 113, 65 (251, 170)  129: 112, 65 (246, 163)
+//   fp64, 64 x 16, one workgroup (two) a sequence: 128: 118, 248 (201, 255)   256: 216, 250 (403, 279)   480: 396, 264 (735, 392)   513: 436, 267 (820, 440)
+// So pieces win to about 256 workgroups there, and between that and the limit calls are up to twice as long as they would be whole; with
+// longer sequences the pieces gain (one of 16384 rows, above).  Sequences of 100 rows, which are spread there, take 27 us for 30 (fp32) and 72 us
+// for 105 (fp64).
 struct ScanPlan {
     int np, lpc, blocks;   // states a lane, lanes a channel, channel blocks
     int64_t piece;         // rows
@@ -1185,8 +1195,11 @@ ScanPlan scan_plan(const psh_scan_desc* d, bool grad) {
         } else {
             while (lpc < widest && with(lpc) < 512) lpc *= 2;
         }
-    } else if (grad && with(least) < 1024 && lpc < widest) {
-        lpc *= 2;   // (a gradient step has twice the latency for the same bytes: 190 us on 4 lanes, 166 us on 8 for 256 rollouts of 65437 steps, 96 channels, 8 states, fp32)
+    } else if (grad && d->dtype != PSH_F64 && with(least) < 1024 && lpc < widest) {
+        // a gradient step has twice the latency for the same bytes: 256 to 511 sequences of 256 rows, 96 x 8, fp32, two workgroups each, take 161 to 272 us on
+        // 4 lanes and 138 to 241 us on 8 (512: 270 and 243; 640: 313 and 286); bf16, 256 x 16, four each, 128: 195 and 169, 255: 318 and 314.  Not fp64,
+        // which begins on 8 lanes: 64 x 16, two each, 256: 279 us on 8 and 348 on 16, 480: 392 and 599, of 100 rows 167 and 252
+        lpc *= 2;
     }
     with(lpc);
     return p;

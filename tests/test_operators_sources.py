@@ -92,3 +92,15 @@ def test_groups_that_are_not_cut_take_no_scratch_memory(groups, rows, K, N):
         d.dtype = dtype
         piece = linear_plan.plan(d).piece
         assert load_library().psh_grouped_linear_grad_workspace(ctypes.byref(d)) <= (2*rows//piece + 1)*(N*K + N)*wide + 2*256
+
+
+def test_float64_gradients_of_the_recurrence_stay_on_eight_lanes():
+    """ 16 lanes a channel make them slower (64 channels, 16 states, 480 sequences of 256 rows: 392 us on 8, 599 us on 16).  The lanes show
+    in the channel blocks, each of which has room for its own sums over its channels. """
+    lib = load_library()
+    for seqs in (256, 300, 511, 512, 600):
+        d = abi.PshScanDesc()
+        d.n_policies, d.n_seqs, d.rows, d.channels, d.states, d.dtype = 1, seqs, 256*seqs, 64, 16, abi.DTYPE_F64
+        sums = 2*d.rows*2*16*8          # two blocks of 32 channels
+        d.dB = d.dC = 4096
+        assert sums <= lib.psh_selective_scan_grad_workspace(ctypes.byref(d)) <= sums + 4*seqs + 512
