@@ -14,7 +14,8 @@ inline bool aligned16(const void* p, int size, int64_t ld, int64_t stride = 0) {
 enum TileKind { TILE_ROWS16, TILE_64, TILE_128, TILE_128_DIRECT, TILE_256_DIRECT };
 
 // Few rows a group (up to 24): 16 of them a tile.  64 groups of 10 rows, 1024 -> 1024, bf16: 23 to 25 us (5.4 TB/s of weights; 30 us in
-// 64 x 64); 256 groups of 8 rows, 6 -> 64, fp64: 5.9 us, a launch's latency (8.7 us).
+// 64 x 64); 256 groups of 8 rows, 6 -> 64, fp64: 5.7 us (8.7 us), three times the shortest launch here: the search for the group, loads of single
+// elements (6 inputs fill no 16-byte unit's line), one product and the store follow one another, and the waves wait for 70 % of that.
 // Tiles [units][rows].  Large ones re-read the operands less often, small ones waste less where a group has few rows or a layer few
 // units, and there are more of them to fill the CUs: the larger ones are for layers that have one and a half of them for every CU.
 // bf16, 8 groups of about 4096 rows, 1024 -> 2048: 180 us (760 TFLOP/s) in 256 x 128 with two workgroups on a CU, of which one stores its tile
@@ -40,7 +41,9 @@ inline TileKind forward_kind(const psh_linear_desc* d) { return rows_kind(d, fal
 inline bool grad_direct(const psh_linear_desc* d) {
     return (d->nonlin != PSH_NL_NONE || aligned16(d->dy, 2, d->ld_dy)) && aligned16(d->x, 2, d->ld_x) && d->out_dim % 8 == 0 && d->in_dim % 8 == 0;
 }
-// the weight gradient's tile: [out units][in units]
+// The weight gradient's tile: [out units][in units].  256 stands for 128 x 256, of which there are two to every 256 x 256 that is counted here and in
+// grad_piece: 8 groups of about 4096 rows, 1024 -> 2048, bf16, are cut into pieces of 2048 rows and joined by 37 us of k_join, where 512 workgroups
+// of whole groups would be two a CU (not measured).
 inline int grad_tile(const psh_linear_desc* d) {
     if (d->dtype != PSH_BF16 || d->out_dim <= 64 || d->in_dim <= 64) return 64;
     const int64_t tiles = (int64_t)((d->out_dim + 127) / 128) * ((d->in_dim + 127) / 128);
