@@ -13,12 +13,15 @@ for the GPU; values that do not ascend or that leave the range give meaningless 
 behind the last offset belong to nobody: they are zero in the results and have zero gradients.
 
 Element types are float64 (what the policies of this package use), float32 and bfloat16.  With bfloat16 rows the products and
-sums run in fp32, and each result is rounded once.  Parameters and states of the recurrence are float64 for
-float64 rows and float32 for the others.
+sums run in fp32, and each result is rounded once; with a nonlinearity, grouped_linear's gradient also rounds dy f'(y) to
+bfloat16 before the products that read it.  Parameters and states of the recurrence are float64 for float64 rows and float32 for the others.
 
 All calls run on the current stream of the tensors' GPU and are ordered like any other work on it.  They can be captured
 into graphs; for gradients inside a capture use the *_grad functions, which autograd's bookkeeping has no part in (a call that autograd
 would differentiate is refused there).  Without a GPU every call raises: there is no CPU fallback.
+
+Torch does not see into the calls.  The single steps tell it that they have changed their state, so that a backward pass that needs the state as it
+was raises; torch.compile leaves the calls as they are; recording them (torch.jit.trace, make_fx) and forward differentiation are refused.
 """
 import ctypes as C
 
