@@ -932,7 +932,7 @@ template <class T> int backward(psh_ctx* c, const psh_linear_desc* d) {
     }
     if (d->dweight || d->dbias) {
         GradArgs<T> a{};
-        a.parts = Parts{d->offsets, d->n_groups, d->rows, (int)grad_piece(d)};
+        a.parts = Parts{d->offsets, d->n_groups, d->rows, (int)grad_piece(d, grad_direct(d))};
         a.places = cut_places(d->rows, d->n_groups, a.parts.L);
         a.dp = dp; a.ld_dp = ld_dp;
         a.x = (const T*)d->x; a.ld_x = d->ld_x;
@@ -951,7 +951,7 @@ template <class T> int backward(psh_ctx* c, const psh_linear_desc* d) {
             rc = launch_weights<T, 64, 64, 2, 2, false>(c, a, also, d->rows, st);
         }
         if (rc != PSH_OK) return rc;
-        if (s.part_w + s.part_b > 0) {
+        if (d->rows > a.parts.L) {
             const long n = (long)a.n * (a.k + 1);
             // 16 bytes a thread once there are threads enough for four workgroups a CU: 37 us for 56 us where 24 pieces of 2048 x 1024 are summed, 10 us
             // for 7.6 us with 64 groups of 64 x 64

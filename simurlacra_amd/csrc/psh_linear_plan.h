@@ -44,16 +44,16 @@ inline bool grad_direct(const psh_linear_desc* d) {
 // The weight gradient's tile: [out units][in units].  256 stands for 128 x 256, of which there are two to every 256 x 256 that is counted here and in
 // grad_piece: 8 groups of about 4096 rows, 1024 -> 2048, bf16, are cut into pieces of 2048 rows and joined by 37 us of k_join, where 512 workgroups
 // of whole groups would be two a CU (not measured).
-inline int grad_tile(const psh_linear_desc* d) {
+inline int grad_tile(const psh_linear_desc* d, bool direct) {
     if (d->dtype != PSH_BF16 || d->out_dim <= 64 || d->in_dim <= 64) return 64;
     const int64_t tiles = (int64_t)((d->out_dim + 127) / 128) * ((d->in_dim + 127) / 128);
     const int64_t huge = (int64_t)((d->out_dim + 255) / 256) * ((d->in_dim + 255) / 256);
-    if (grad_direct(d) && d->out_dim > 128 && d->in_dim > 128 && huge * (d->rows / 2048 + d->n_groups) >= 384) return 256;
+    if (direct && d->out_dim > 128 && d->in_dim > 128 && huge * (d->rows / 2048 + d->n_groups) >= 384) return 256;
     return tiles * (d->rows / 2048 + d->n_groups) >= 192 ? 128 : 64;
 }
 // rows of one piece of the weight gradient's contraction: enough pieces for about four workgroups a CU
-inline int64_t grad_piece(const psh_linear_desc* d) {
-    const int t = grad_tile(d);
+inline int64_t grad_piece(const psh_linear_desc* d, bool direct) {
+    const int t = grad_tile(d, direct);
     const int64_t tiles = (int64_t)((d->out_dim + t - 1) / t) * ((d->in_dim + t - 1) / t);
     const int64_t whole = ((int64_t)d->rows + 64) / 64 * 64;
     const int64_t wanted = t == 256 ? 512 : t == 128 ? 1024 : 2048;
@@ -64,18 +64,22 @@ inline int64_t grad_piece(const psh_linear_desc* d) {
 }
 
 struct GradSpace { int64_t dp, part_w, part_b, total; };
+// (room for the pieces of either kind of tile, so that the size can be asked for before the arrays are there)
 inline GradSpace grad_space(const psh_linear_desc* d) {
     GradSpace s{};
-    const int64_t places = cut_places_count(d->rows, d->n_groups, grad_piece(d));
+    int64_t places = 0;
+    for (int direct = 0; direct < 2; ++direct) {
+        const int64_t L = grad_piece(d, direct), n = cut_places_count(d->rows, d->n_groups, L);
+        if (d->rows > L && n > places) places = n;   // (else no group has a second piece)
+    }
     if (d->nonlin != PSH_NL_NONE) s.dp = align256((int64_t)d->rows * d->out_dim * elem_size(d->dtype));
     if (d->dweight) s.part_w = align256(places * d->out_dim * d->in_dim * wide_size(d->dtype));
     if (d->dbias) s.part_b = align256(places * d->out_dim * wide_size(d->dtype));
-    if (d->rows <= grad_piece(d)) s.part_w = s.part_b = 0;   // no group has a second piece
     s.total = s.dp + s.part_w + s.part_b;
     return s;
 }
 inline TileKind grad_kind(const psh_linear_desc* d) {
-    const int t = grad_tile(d);
+    const int t = grad_tile(d, grad_direct(d));
     return t == 64 ? TILE_64 : !grad_direct(d) ? TILE_128 : t == 128 ? TILE_128_DIRECT : TILE_256_DIRECT;
 }
 

@@ -8,6 +8,6 @@ extern "C" void plan(const psh_linear_desc* d, int64_t* out) {
     out[1] = p.rows;
     out[2] = p.weights;
     out[3] = p.joint;
-    out[4] = grad_piece(d);
+    out[4] = grad_piece(d, grad_direct(d));
     out[5] = grad_space(d).total;
 }

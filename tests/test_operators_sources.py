@@ -104,3 +104,18 @@ def test_float64_gradients_of_the_recurrence_stay_on_eight_lanes():
         sums = 2*d.rows*2*16*8          # two blocks of 32 channels
         d.dB = d.dC = 4096
         assert sums <= lib.psh_selective_scan_grad_workspace(ctypes.byref(d)) <= sums + 4*seqs + 512
+
+
+@pytest.mark.parametrize('lengths,K,N', [(c[0], c[1], c[2]) for c in layer_cases.CASES.values()], ids=list(layer_cases.CASES))
+@pytest.mark.parametrize('nonlin', [None, 'tanh'])
+def test_the_size_of_the_scratch_memory_does_not_depend_on_addresses(lengths, K, N, nonlin):
+    """ A caller may ask for it before the arrays are there: pointers are only compared with NULL.  It is enough for a call with any of them. """
+    lib = load_library()
+    sizes, needed = set(), []
+    for shift in range(3):
+        for dy in (4096, 4098):
+            d = _descriptor(lengths, K, N, shift, nonlin)
+            d.dy = dy
+            sizes.add(lib.psh_grouped_linear_grad_workspace(ctypes.byref(d)))
+            needed.append(linear_plan.plan(d).space)
+    assert len(sizes) == 1 and max(needed) <= sizes.pop()
