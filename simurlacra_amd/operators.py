@@ -124,8 +124,9 @@ _is_tracing, _modes, _function_modes = torch._C._is_tracing, torch._C._len_torch
 
 
 def _recorded():
-    """ Whether torch is recording: by jit.trace, or by make_fx in one of the two places where it listens. """
-    return (_is_tracing() or torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None
+    """ Whether torch is recording: by jit.trace, by make_fx in one of the two places where it listens, or with tensors that have no memory. """
+    modes = torch._C._TorchDispatchModeKey
+    return (_is_tracing() or any(torch._C._get_dispatch_mode(m) is not None for m in (modes.PROXY, modes.FAKE))
             or torch._C._dispatch_tls_is_dispatch_key_included(torch._C.DispatchKey.PreDispatch))
 
 
@@ -134,7 +135,7 @@ def _seen_by_torch(*tensors):
     operations that it sees is refused: a recorded call would be empty memory whenever it is played back, and a tangent of forward
     differentiation would be dropped and the derivative read as zero. """
     if (_is_tracing() or _modes() or _function_modes()) and _recorded():
-        raise ValueErr(msg='the policy operators cannot be recorded (torch.jit.trace, make_fx): torch does not see what they do!')
+        raise ValueErr(msg='the policy operators cannot be recorded (torch.jit.trace, make_fx, FakeTensorMode): torch does not see what they do!')
     if _forward._current_level >= 0:
         for t in tensors:
             if isinstance(t, _Tensor) and _forward.unpack_dual(t).tangent is not None:
@@ -246,7 +247,7 @@ def _linear_forward(x, weight, bias, offsets, nonlin, wide=False):
     value = y
     if wide and dt == torch.bfloat16 and nonlin in ('tanh', 'sigmoid'):
         value = torch.empty((R, N), dtype=torch.float32, device=dev)
-        d.y_wide = _ptr(value)
+        d.y_wide = value.data_ptr()
     eng._call('psh_grouped_linear', C.byref(d))
     del keep
     return (y, value) if wide else y
@@ -270,13 +271,13 @@ def grouped_linear_grad(dy, y, x, weight, offsets, nonlin=None, want=(True, True
     dx = dw = db = None
     if want[0]:
         dx = x.new_empty(R, K)
-        d.dx = _ptr(dx)
+        d.dx = dx.data_ptr()
     if want[1]:
         dw = x.new_empty(G, N, K)
-        d.dweight = _ptr(dw)
+        d.dweight = dw.data_ptr()
     if want[2]:
         db = x.new_empty(G, N)
-        d.dbias = _ptr(db)
+        d.dbias = db.data_ptr()
     space = _give_workspace(eng, d, 'psh_grouped_linear_grad_workspace', x)
     eng._call('psh_grouped_linear_grad', C.byref(d))
     del keep, space
@@ -370,7 +371,7 @@ def _conv_forward(x, weight, bias, offsets, groups, state, silu):
     eng, d, keep, S, R, D, P, K, dt, dev = _conv_desc(x, weight, bias, offsets, groups, state, silu, False)
     y = x.new_empty(R, D)
     last = x.new_empty(S, D, K - 1)
-    d.y, d.last, d.stride_last = y.data_ptr(), _ptr(last), D*(K - 1)
+    d.y, d.last, d.stride_last = y.data_ptr(), last.data_ptr(), D*(K - 1)
     eng._call('psh_causal_conv', C.byref(d))
     del keep
     return y, last
@@ -484,11 +485,11 @@ def _scan_forward(u, delta, A, B, Cm, D, z, delta_bias, offsets, groups, state, 
     eng, d, keep, S, R, ch, P, N, dt, W, dev = _scan_desc(u, delta, A, B, Cm, D, z, delta_bias, offsets, groups, state, False)
     y = u.new_empty(R, ch)
     last = A.new_empty(S, ch, N)
-    d.y, d.last, d.stride_last = y.data_ptr(), _ptr(last), ch*N
+    d.y, d.last, d.stride_last = y.data_ptr(), last.data_ptr(), ch*N
     check = None
     if keep_check:
         check = _workspace(_size(eng, 'psh_selective_scan_check', d), dev)
-        d.check = _ptr(check)
+        d.check = check.data_ptr()
     space = _give_workspace(eng, d, 'psh_selective_scan_workspace', u)
     eng._call('psh_selective_scan', C.byref(d))
     del keep, space

@@ -179,6 +179,15 @@ def test_traces_are_refused(engine, k, tracer):
     assert len(engine.calls) == 1
 
 
+@pytest.mark.parametrize('k', range(len(NAMES)), ids=NAMES)
+def test_calls_for_their_shapes_alone_are_refused(engine, k):
+    """ results without memory, of tensors that have some """
+    name, f, tensors = entry_points()[k]
+    with FakeTensorMode(allow_non_fake_inputs=True), pytest.raises(ValueErr, match='recorded'):
+        f(**tensors)
+    assert not engine.calls
+
+
 def test_traces_of_differentiated_calls_are_refused(engine):
     name, f, tensors = entry_points()[0]
     with pytest.raises(ValueErr, match='recorded'):
